@@ -608,6 +608,126 @@ int nq_gdn_conv1d(const void *x, int64_t x_row_stride, const void *weight, int k
                   const int32_t *state_indices, int64_t num_slots, int initial_state_from_slot,
                   void *out, int64_t out_row_stride, int channels, int dtype, void *stream);
 
+/*
+ * Attention over chosen spans of the cache: a sliding window with sinks, and
+ * trees of drafted tokens.  No counterpart in the reference, whose attention
+ * (layers/attention.py:64-74) is causal over the whole context.
+ *
+ * The query token at position p of its sequence (0-based among its cached
+ * tokens) sees key j
+ *   windowed: when j <= p and (j > p - window or j < num_sinks)
+ *             (window >= 1, num_sinks >= 0);
+ *   in a tree: when j < C, C = Lk - Lq the tokens cached before the tree, or
+ *             when bit (j - C) % 64 of word (j - C) / 64 of the token's row of
+ *             tree_mask is set (bits of other nodes than the tree's are
+ *             ignored; a node sees itself only if its own bit is set).
+ * A query token that sees nothing gives zeros.  Keys and values that a token
+ * does not see do not reach its output, be they NaN or infinite.
+ *
+ * All three: head_dim 128 or 256, groups of up to 16 query heads, q and out
+ * F16/BF16 (q 16-byte aligned, out 8-byte), K/V of the type of q or
+ * NQ_FP8_E4M3 with k_scale/v_scale float[num_kv_heads]; softmax_scale > 0.
+ * Paged K/V: block_tables [num_seqs, >= max_blocks_per_seq] int32 with row
+ * stride bt_stride, block_size a multiple of 32; entries of pages that hold no
+ * visible key of the sequence's queries are not used, and keys of pages outside
+ * [0, num_blocks) are invisible.  gate may be NULL; otherwise out is gated as
+ * nq_paged_decode_gated gates it (8-byte aligned, type of out).
+ * Rows of out past the last sequence's are left as they were.
+ *
+ * workspace (256-byte aligned; its contents need no clearing) holds the partial
+ * outputs of sequences that several workgroups share.  When it is smaller than
+ * a launch of these sizes needs, and need is given, nothing is launched, *need
+ * is set to those bytes and 1 returned.  Calls that overlap may not share one.
+ */
+
+/*
+ * Attention of trees of drafted tokens over the paged cache, which already
+ * holds their keys and values: sequence s's nodes are the rows
+ * [cu_seqlens_q[s], cu_seqlens_q[s+1]) of q [total_q, Hq, D], node i cached at
+ * position C + i, its cache cu_seqlens_k[s+1] - cu_seqlens_k[s] tokens.
+ * tree_mask [total_q, mask_words] int64 with rows of mask_row_stride words,
+ * mask_words >= ceil(max_seqlen_q / 64); at most 256 nodes per tree.
+ * max_seqlen_q / max_seqlen_k: the largest tree and cache (none beyond them is
+ * read or written).
+ */
+int nq_tree_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+                      const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                      int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables, int64_t bt_stride,
+                      int max_blocks_per_seq, int64_t num_blocks, const int64_t *tree_mask,
+                      int64_t mask_row_stride, int mask_words, void *out, int64_t out_row_stride,
+                      int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                      int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                      int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
+                      int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                      int64_t workspace_bytes, int64_t *need, void *stream);
+
+/*
+ * Windowed causal prefill: nq_varlen_prefill's arguments (rows of q packed by
+ * cu_seqlens_q, row i of a sequence at position i + Lk - Lq, K/V packed by
+ * cu_seqlens_k -- total_k rows of stride kv_row_stride -- or paged when
+ * block_tables is given) with the window and its sinks.
+ */
+int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                      const void *v, int64_t kv_row_stride, int64_t total_k, const int32_t *cu_seqlens_q,
+                      const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
+                      const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                      int64_t num_blocks, int window, int num_sinks, void *out, int64_t out_row_stride,
+                      int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                      int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                      int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
+                      int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                      int64_t workspace_bytes, int64_t *need, void *stream);
+
+/*
+ * Windowed paged decode: one query token per sequence, the last of its
+ * context_lens[b] cached tokens (rows with context_len <= 0 produce zeros).
+ */
+int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                     const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                     int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
+                     void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
+                     int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                     float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
+                     const float *v_scale, const void *gate, int64_t gate_batch_stride,
+                     int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,
+                     void *stream);
+
+/*
+ * Copies of cache pages, the same in every slab (layer and K or V) of the pool
+ * kv_cache [num_slabs, num_blocks, block_size, row_bytes] (any element type;
+ * rows 16-byte aligned): the first num_tokens[i] rows (all of them when
+ * num_tokens is NULL; clamped to the page) of page src_blocks[i] to page
+ * dst_blocks[i], i < num_pairs.  Pairs with an id outside [0, num_blocks), or
+ * the same page twice, are skipped.  A page that is written may appear in no
+ * other pair: the pairs run in any order.
+ */
+int nq_copy_kv_blocks(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int block_size,
+                      int64_t row_bytes, const int32_t *src_blocks, const int32_t *dst_blocks,
+                      const int32_t *num_tokens, int64_t num_pairs, void *stream);
+
+/*
+ * The end of a tree's verification: the accepted path, and its cache rows moved
+ * to where the sequence goes on, in every slab of the pool (as above).
+ * Sequence s's nodes are rows [cu_seqlens_q[s], cu_seqlens_q[s+1]) of parents
+ * (the parent's index among them, below the node's own), tokens (the drafted
+ * ones) and target_tokens (what the model chose after each node); node 0 is the
+ * root, the last token sampled before.  From the root, the path goes on to the
+ * first child whose token is the current node's target, until there is none.
+ * path [num_seqs, max_seqlen_q] receives its node indices, -1 behind them,
+ * num_accepted their number (the root among them; 0 for a sequence without
+ * nodes), next_tokens the last one's target (-1 without nodes).
+ * Then the row of position C + path[r] goes to position C + r, C =
+ * cu_seqlens_k[s+1] - cu_seqlens_k[s] - nodes; positions without a page are
+ * skipped.  target_tokens == NULL: path and num_accepted are inputs (indices
+ * that rise; the path ends before one that does not).  At most 256 nodes.
+ */
+int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int block_size, int64_t row_bytes,
+                   const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                   const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int num_seqs, int64_t total_q,
+                   int max_seqlen_q, const int32_t *parents, const int64_t *tokens,
+                   const int64_t *target_tokens, int32_t *path, int32_t *num_accepted, int64_t *next_tokens,
+                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif

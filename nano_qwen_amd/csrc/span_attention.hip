@@ -1,0 +1,1098 @@
+// Attention over chosen spans of the cache, for gfx950: a sliding window with
+// sinks (prefill and decode), and trees of drafted tokens.  No counterpart in
+// the reference, whose attention (layers/attention.py:64-74) is causal over
+// the whole context.
+//
+// Rows.  Sequence s has Lq query tokens at positions P + t, P = Lk - Lq, of
+// its Lk cached tokens (Lq = 1: decode).  Row r = t * G + i is query head
+// kvh * G + i of token t: the rows of one kv head, tokens and heads packed, so
+// that a tile of M rows reads each K/V byte once for all of them whatever the
+// group size, and a tree of n nodes fills M = n * G rows.
+//
+// Visible keys of the row of token t, position p = P + t:
+//   window: j <= p and (j > p - window or j < sinks);
+//   tree:   j < C = Lk - Lq (the context), or node j - C in the row's mask.
+// Either way they lie in at most two runs of 32-key tiles -- the sinks' and
+// the rest -- so an item (row tile of a sequence) is a list of tiles: the
+// first `ts` tiles, then those from `tlo` on.  Keys of a tile that only some
+// rows see are masked; whole tiles outside the list are never read, so pages
+// that hold no visible key may be missing from the table.
+//
+// Products as in the other attention kernels: S^T = K Q^T and O^T += V^T P^T
+// on v_mfma_f32_16x16x32, whose S^T accumulator is the B operand of the second
+// product; V^T through transposing LDS reads; fp8 K/V stay codes in LDS and
+// are widened (exactly) in registers, with the scales on the scores and the
+// output.  Softmax in the log2 domain, statistics and sums in fp32; the
+// maximum of a row moves only when it grows by more than 2^8 (P <= 256, so
+// rounding P to 16 bits loses no more than it does at P <= 1).
+//
+// NaN and infinities in keys or values that a row does not see do not reach
+// it: masked scores are replaced before use, and a masked tile whose values
+// are not all finite takes them out of the product and adds them back to the
+// rows that see them (fix_values).
+#include <algorithm>
+
+#include "nq_device.hpp"
+
+namespace nq {
+namespace {
+
+constexpr int kKeys = 32;         // keys per tile
+constexpr float kRescale = 8.0f;  // log2 growth of a row maximum that moves it
+constexpr int kMaxNodes = 256;    // of a tree: 8 mask words of 32 bits per row
+
+// 16-byte chunk c of key row r of a 16-bit tile lies at chunk c ^ swz(r), so
+// that the operand reads (16 rows x one chunk of K; 4 rows x 2 chunks of V^T)
+// meet no bank twice; fp8 tiles of D-byte rows likewise in 16-byte units.
+__device__ inline int swz_k(int row) { return row & 15; }
+__device__ inline int swz_v(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
+template <int D>
+__device__ inline int swz8(int row) {
+  const int b = ((row >> 3) ^ (row >> 4)) & 1;
+  return D == 128 ? (((row >> 1) & 3) | (b << 2)) : ((row & 7) | (b << 3));
+}
+
+struct SpanArgs {
+  const uint8_t *q;
+  int64_t q_rs, q_hs;  // bytes
+  const uint8_t *k;
+  const uint8_t *v;
+  int64_t kv_rs;        // bytes per K/V row (token)
+  const int32_t *cu_q;  // null: one row per sequence (decode)
+  const int32_t *cu_k;  // prefix sums of the lengths; decode: the lengths themselves
+  int total_q, total_k;  // rows of q and, packed K/V, of k: sequences are clamped to them
+  int max_q, max_k;      // most query tokens and keys of a sequence (further ones are never touched)
+  const int32_t *block_tables;  // null: packed K/V
+  int64_t bt_stride;
+  int max_blocks, num_blocks;
+  uint8_t *out;
+  int64_t o_rs, o_hs;
+  const uint8_t *gate;  // null, or the output gate, of the type of out
+  int64_t g_rs, g_hs;
+  int Hq, Hkv, G, block_size, num_seqs;
+  int window, sinks;     // window 0: trees
+  const uint64_t *mask;  // [total_q, words] rows of mask_rs words
+  int64_t mask_rs;
+  int words;
+  float scale_log2;
+  const float *k_scale;
+  const float *v_scale;
+  // Equal ranges: n_ranges per kv head (0: one item per workgroup), the partial
+  // outputs of range w's slots 2 w and 2 w + 1 (fp32, normalised, as the lanes
+  // hold them), their rows' log2-sum-exp, and what they are.
+  int n_ranges;
+  float *part_o;
+  float *part_l;
+  int4 *part_desc;  // (sequence, row tile, kind, 0)
+};
+constexpr int kPieceNone = -1, kPieceMore = 0, kPieceLast = 1;
+
+// Launch shape: RW waves of QS x 16 rows each that share every tile (M rows),
+// a ring of SLOTS tiles.
+//  * one wave (M = 16): decode and the smallest trees.  Its ring is its own:
+//    no barriers, and K and V of SLOTS tiles are in flight at all times.
+//  * four waves of 16 or 32 rows (eight of 16 at head_dim 256).  A barrier per
+//    tile; copies run SLOTS - 1 tiles ahead.
+template <int D_, bool FP8, int RW_, int QS_, int SLOTS_>
+struct Shape {
+  static constexpr int D = D_, RW = RW_, QS = QS_, SLOTS = SLOTS_;
+  static constexpr int M = RW * QS * 16;
+  static constexpr int SRC_ROWB = FP8 ? D : 2 * D;
+  static constexpr int TILE_B = kKeys * SRC_ROWB, SLOT_B = 2 * TILE_B;
+  static constexpr int LPR = SRC_ROWB / 16;        // lanes (16-byte pieces) per row
+  static constexpr int COPS = TILE_B / 1024 / RW;  // copies per wave of a K (or V) tile
+  static constexpr int RING_B = SLOTS * SLOT_B;
+  static constexpr int MASK_WORDS = kMaxNodes / 32 + 1;  // LDS row of a token's mask (odd: no bank pattern)
+  static constexpr int TOKENS = M + 1;                   // of a row tile, at most
+  static constexpr int LDS_B = RING_B + TOKENS * MASK_WORDS * 4;
+  static constexpr int NKK = D / 32, NJ = D / 16;
+  static_assert(COPS >= 1, "every wave copies");
+};
+
+// ---------------------------------------------------------------- items
+struct Seq {
+  int s, q0, Lq, k0, Lk;
+};
+__device__ __forceinline__ Seq seq_of(const SpanArgs &a, int s, bool uniform) {
+  Seq x{};
+  x.s = s;
+  if (!a.cu_q) {
+    x.q0 = s;
+    x.Lq = 1;
+    x.Lk = uniform ? ld_const(a.cu_k + s) : a.cu_k[s];
+  } else {
+    const int qa = uniform ? ld_const(a.cu_q + s) : a.cu_q[s], qb = uniform ? ld_const(a.cu_q + s + 1) : a.cu_q[s + 1];
+    const int ka = uniform ? ld_const(a.cu_k + s) : a.cu_k[s], kb = uniform ? ld_const(a.cu_k + s + 1) : a.cu_k[s + 1];
+    x.q0 = max(0, min(qa, a.total_q));
+    x.Lq = max(0, min(min(qb, a.total_q) - x.q0, a.max_q));
+    x.k0 = max(0, min(ka, a.total_k));
+    x.Lk = a.block_tables ? kb - ka : min(kb, a.total_k) - x.k0;
+  }
+  x.Lk = max(0, min(x.Lk, a.max_k));
+  return x;
+}
+// floor(n / d) for 0 <= n < 2^22, 1 <= d < 2^22: the float estimate is within
+// one of the quotient.
+__device__ __forceinline__ int small_div(int n, int d) {
+  int q = static_cast<int>(static_cast<float>(n) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+  if (q * d > n)
+    --q;
+  else if ((q + 1) * d <= n)
+    ++q;
+  return q;
+}
+// The tiles of a row tile whose tokens are ta .. tb.
+struct Tiles {
+  int ts, tlo, n;  // tiles 0 .. ts - 1, then tlo, tlo + 1, ...: n in all
+};
+__device__ __forceinline__ Tiles tiles_of(const SpanArgs &a, const Seq &q, int ta, int tb) {
+  Tiles t{0, 0, 0};
+  if (a.window == 0) {
+    t.n = (q.Lk + kKeys - 1) / kKeys;
+    return t;
+  }
+  const int P = q.Lk - q.Lq;
+  const int end = P + tb + 1;  // keys before it may be seen
+  if (end <= 0) return t;
+  t.ts = (min(a.sinks, end) + kKeys - 1) / kKeys;
+  t.tlo = max(t.ts, max(0, P + ta - a.window + 1) / kKeys);
+  t.n = t.ts + max(0, (end + kKeys - 1) / kKeys - t.tlo);
+  return t;
+}
+// Cost of each row tile of a sequence in key tiles: an item's fixed cost and
+// its tiles (of several windowed row tiles: the most that one can have).
+template <class S>
+struct Cost {
+  // one wave: Q and first-tile latency, in the time of a tile; more waves: the
+  // same in their faster tiles
+  static constexpr int kItem = S::RW == 1 ? 1 : 4;
+  static constexpr int kMinRange = 2;
+};
+template <class S>
+__device__ __forceinline__ int row_tiles(const SpanArgs &a, const Seq &q) {
+  return (q.Lq * a.G + S::M - 1) / S::M;
+}
+template <class S>
+__device__ __forceinline__ int item_cost(const SpanArgs &a, const Seq &q) {
+  if (q.Lq <= 0) return 0;
+  int n;
+  if (q.Lq * a.G <= S::M) {
+    n = tiles_of(a, q, 0, q.Lq - 1).n;
+  } else {
+    n = (q.Lk + kKeys - 1) / kKeys;
+    if (a.window > 0)
+      n = min(n, (min(a.sinks, q.Lk) + kKeys - 1) / kKeys + (min(a.window, q.Lk) + S::M + 2 * kKeys - 2) / kKeys);
+  }
+  return Cost<S>::kItem + n;
+}
+
+// ---------------------------------------------------------------- the kernel
+template <class T, bool FP8, class S>
+__device__ __forceinline__ void span_body(const SpanArgs &a) {
+  constexpr int D = S::D, RW = S::RW, QS = S::QS, M = S::M, SLOTS = S::SLOTS, COPS = S::COPS;
+  constexpr int NKK = S::NKK, NJ = S::NJ, TILE_B = S::TILE_B, SLOT_B = S::SLOT_B, SRC_ROWB = S::SRC_ROWB;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int lane = threadIdx.x & 63;
+  const int rw = RW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  const bool paged = a.block_tables != nullptr;
+  const bool ranges = a.n_ranges > 0;
+
+  // kv head and range (or item) of this workgroup.  Workgroup L runs on XCD
+  // L % 8: a kv head stays on one XCD (or, of fewer than 8, on 8 / Hkv, which
+  // take contiguous ranges, or items in turn), so that the row tiles that read
+  // the same keys share an L2.
+  const int L = blockIdx.x;
+  int h, w;
+  if (a.Hkv < 8 && 8 % a.Hkv == 0) {
+    const int per = 8 / a.Hkv, x = L & 7;
+    h = x % a.Hkv;
+    w = ranges ? (x / a.Hkv) * (a.n_ranges / per) + (L >> 3) : (L >> 3) * per + x / a.Hkv;
+  } else {
+    h = L % a.Hkv;
+    w = L / a.Hkv;
+  }
+
+  // Positions [pos0, pos1) of the batch's row tiles laid end to end, each as
+  // its cost (whole items: 1).
+  auto weight_of = [&](const Seq &q) -> int { return ranges ? item_cost<S>(a, q) : (q.Lq > 0 ? 1 : 0); };
+  int pos0 = w, pos1 = w + 1;
+  int w_of = 0;  // the range's partials
+  if (ranges) {
+    int total = 0;
+    for (int b = 0; b < a.num_seqs; b += 64) {
+      int c = 0;
+      if (b + lane < a.num_seqs) {
+        const Seq q = seq_of(a, b + lane, false);
+        c = row_tiles<S>(a, q) * weight_of(q);
+      }
+      total += wave_sum_i32(c);
+    }
+    w_of = h * a.n_ranges + w;
+    const int W = min(a.n_ranges, max(1, total / Cost<S>::kMinRange));
+    pos0 = w < W ? static_cast<int>(static_cast<int64_t>(w) * total / W) : 0;
+    pos1 = w < W ? static_cast<int>(static_cast<int64_t>(w + 1) * total / W) : 0;
+  }
+  // The range's two partial pieces, written for the merge when it is done.
+  int4 desc0{0, 0, kPieceNone, 0}, desc1{0, 0, kPieceNone, 0};
+  auto leave = [&]() {
+    if (ranges && rw == 0 && lane == 0) {
+      a.part_desc[2 * w_of] = desc0;
+      a.part_desc[2 * w_of + 1] = desc1;
+    }
+  };
+  if (pos0 >= pos1) {
+    leave();
+    return;
+  }
+  // The row tile at pos0: sequence s, row tile rt, which starts at position X.
+  int s = a.num_seqs, rt = 0, X = 0;
+  {
+    int base = 0;
+    for (int b = 0; b < a.num_seqs; b += 64) {
+      int c = 0, wt = 1;
+      if (b + lane < a.num_seqs) {
+        const Seq q = seq_of(a, b + lane, false);
+        wt = weight_of(q);
+        c = row_tiles<S>(a, q) * wt;
+      }
+      const int incl = base + wave_iscan(c);
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > pos0);
+      if (hit != 0) {
+        const int l = static_cast<int>(__builtin_ctzll(hit));
+        s = b + l;
+        const int start = __builtin_amdgcn_readlane(incl - c, l);
+        const int cost = __builtin_amdgcn_readlane(wt, l);
+        rt = static_cast<int>(static_cast<unsigned>(pos0 - start) / static_cast<unsigned>(cost));
+        X = start + rt * cost;
+        break;
+      }
+      base = __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  if (s >= a.num_seqs) {
+    leave();
+    return;
+  }
+
+  // ---------------------------------------------------------------- copies
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)(smem)));
+  uint32_t *const lds_mask = reinterpret_cast<uint32_t *>(smem + S::RING_B);
+  const int kv_rs = static_cast<int>(a.kv_rs);
+  const int tiles_per_blk = paged ? a.block_size / kKeys : 0x40000000;
+  // Lane l's piece of copy c lands at row drow, piece l % LPR of the tile; it
+  // fetches the piece that the swizzle puts there.
+  uint32_t src_k[COPS], src_v[COPS];
+#pragma unroll
+  for (int c = 0; c < COPS; ++c) {
+    const int drow = (rw * COPS + c) * (64 / S::LPR) + lane / S::LPR;
+    const uint32_t row_off = static_cast<uint32_t>(drow * kv_rs);
+    if constexpr (FP8) {
+      src_k[c] = src_v[c] = row_off + (((lane % S::LPR) ^ swz8<D>(drow)) << 4);
+    } else {
+      src_k[c] = row_off + (((lane % S::LPR) ^ swz_k(drow)) << 4);
+      src_v[c] = row_off + (((lane % S::LPR) ^ swz_v(drow)) << 4);
+    }
+  }
+  // The piece being copied: list positions st_i .. st_end - 1 of its tiles, in
+  // runs that share a page (or, packed, a stretch of the list).
+  int st_i = 0, st_end = 0, st_run = 0;  // next list position, the piece's end, tiles left in the run
+  int st_ts = 0, st_tlo = 0, st_Lk = 0;
+  int st_key = 0;           // first key of the next tile
+  const uint8_t *st_k = a.k;  // its K source (row 0, at the kv head)
+  bool st_ok = false;
+  const int32_t *st_bt = nullptr;
+  int st_blk = -1;          // value of the table entry that the next run needs
+  int64_t st_base = 0;      // packed: byte offset of the sequence's first key
+  uint32_t st_dst = lds0;
+  uint64_t bad = 0;         // list position mod 64 of tiles in missing pages
+  const int64_t v_minus_k = a.v - a.k;
+  auto tile_at = [&](int i) { return i < st_ts ? i : i - st_ts + st_tlo; };
+  auto entry = [&](int tile) -> int {
+    const int e = small_div(tile, tiles_per_blk);
+    return e < a.max_blocks ? ld_const(st_bt + e) : -1;
+  };
+  auto copy_start = [&](const Seq &q, const Tiles &t, int lo, int hi) {
+    st_i = lo;
+    st_end = hi;
+    st_run = 0;
+    st_ts = t.ts;
+    st_tlo = t.tlo;
+    st_Lk = q.Lk;
+    bad = 0;
+    if (paged) {
+      st_bt = a.block_tables + static_cast<int64_t>(q.s) * a.bt_stride;
+      if (lo < hi) st_blk = entry(tile_at(lo));
+    } else {
+      st_base = static_cast<int64_t>(q.k0) * kv_rs + h * SRC_ROWB;
+    }
+  };
+  // Source and readable bytes of the next tile's copies (0 bytes: zeros).
+  auto next_tile = [&](const uint8_t *&src, uint32_t &nrec) {
+    src = a.k;
+    nrec = 0;
+    if (st_i >= st_end) return;
+    if (st_run == 0) {
+      const int tile = tile_at(st_i);
+      st_key = tile * kKeys;
+      const int list = (st_i < st_ts ? min(st_ts, st_end) : st_end) - st_i;  // tiles in a row of the list
+      if (paged) {
+        const int in_blk = tile - small_div(tile, tiles_per_blk) * tiles_per_blk;
+        st_run = min(list, tiles_per_blk - in_blk);
+        st_ok = st_blk >= 0 && st_blk < a.num_blocks;
+        st_k = a.k + (static_cast<int64_t>(st_ok ? st_blk : 0) * a.block_size + in_blk * kKeys) * kv_rs + h * SRC_ROWB;
+        if (st_i + st_run < st_end) st_blk = entry(tile_at(st_i + st_run));  // used a run from now
+      } else {
+        st_run = list;
+        st_ok = true;
+        st_k = a.k + st_base + static_cast<int64_t>(st_key) * kv_rs;
+      }
+    }
+    if (st_ok) {
+      src = st_k;
+      nrec = static_cast<uint32_t>(min(kKeys, st_Lk - st_key) * kv_rs);
+    }
+    bad = (bad & ~(1ull << (st_i & 63))) | (static_cast<uint64_t>(!st_ok) << (st_i & 63));
+    st_k += kKeys * kv_rs;
+    st_key += kKeys;
+    --st_run;
+    ++st_i;
+  };
+  auto copy_k = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
+    const u32x4 r = rsrc_words(src, nrec);
+#pragma unroll
+    for (int c = 0; c < COPS; ++c) dma16_opaque(dst + (rw * COPS + c) * 1024, r, src_k[c]);
+  };
+  auto copy_v = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
+    const u32x4 r = rsrc_words(src + (nrec ? v_minus_k : 0), nrec);
+#pragma unroll
+    for (int c = 0; c < COPS; ++c) dma16_opaque(dst + TILE_B + (rw * COPS + c) * 1024, r, src_v[c]);
+  };
+
+  // ---------------------------------------------------------------- operands
+  // K operand kk: key rows m and m + 16, dims 32 kk + 8 g ..; V^T operand j:
+  // keys 4 g + i and 16 + 4 g + i (the order of P), dims 16 j + m.
+  uint32_t kbase_l, kx_l, vbase_l, vx_l;
+  if constexpr (FP8) {
+    const int s8 = 2 * swz8<D>(m);
+    kbase_l = m * D + ((g ^ (s8 & 3)) << 3);
+    kx_l = (s8 & ~3) << 3;
+    const int rho = (lane & 15) >> 1, vp = lane & 1;
+    const int r = rho < 4 ? 4 * g + rho : 12 + 4 * g + rho;
+    vbase_l = r * D + (vp << 3);
+    vx_l = (2 * swz8<D>(r)) << 3;
+  } else {
+    kbase_l = m * 2 * D + ((g ^ (swz_k(m) & 3)) << 4);
+    kx_l = (swz_k(m) & 12) << 4;
+    const int vk = (lane >> 2) & 3, vq = lane & 3;
+    const int r0 = 4 * g + vk;
+    vbase_l = r0 * 2 * D + (((vq >> 1) ^ (swz_v(r0) & 1)) << 4) + (vq & 1) * 8;
+    vx_l = (swz_v(r0) & 14) << 4;
+  }
+  auto widen8 = [](const u32x2 &c) {
+    return u32x4{T::template fp8x2<false>(c[0]), T::template fp8x2<true>(c[0]), T::template fp8x2<false>(c[1]),
+                 T::template fp8x2<true>(c[1])};
+  };
+  auto k_op = [&](uint32_t kt, int kk, int ks) -> u32x4 {
+    if constexpr (FP8) {
+      constexpr int KF = D == 128 ? 2 : 4;  // swz8: rows m + 16 flip this bit of kk
+      const uint32_t at = (((ks ? kk ^ KF : kk) << 5) ^ kx_l) + (kt + kbase_l);
+      return widen8(ks ? lds_load_b64<16 * D>(at) : lds_load_b64<0>(at));
+    } else {
+      const uint32_t at = ((kk << 6) ^ kx_l) + (kt + kbase_l);
+      return ks ? lds_load_b128<16 * 2 * D>(at) : lds_load_b128<0>(at);
+    }
+  };
+  auto v_op = [&](uint32_t kt, int j) -> u32x4 {
+    if constexpr (FP8) {
+      return widen8(lds_load_tr8(((j << 4) ^ vx_l) + (kt + TILE_B + vbase_l)));
+    } else {
+      const uint32_t at = ((j << 5) ^ vx_l) + (kt + TILE_B + vbase_l);
+      const u32x2 lo = lds_load_tr16<0>(at), hi = lds_load_tr16<16 * 2 * D>(at);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  };
+
+  const float sl2 = a.scale_log2 * (FP8 ? ld_const(a.k_scale + h) : 1.f);
+  const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
+
+  // ---------------------------------------------------------------- items
+  for (;;) {
+    const Seq q = seq_of(a, s, true);
+    const int n_rt = row_tiles<S>(a, q);
+    const int r_first = rt * M;                         // rows of the tile
+    const int r_last = min(r_first + M, q.Lq * a.G) - 1;
+    const int t_first = small_div(r_first, a.G), t_last = small_div(r_last, a.G);
+    const Tiles tl = tiles_of(a, q, t_first, t_last);
+    int lo = 0, hi = tl.n;
+    bool first_here = true;  // the item's start lies in this range
+    if (ranges) {
+      const int x0 = X + Cost<S>::kItem;
+      lo = max(0, min(tl.n, pos0 - x0));
+      hi = max(0, min(tl.n, pos1 - x0));
+      first_here = X >= pos0;
+    }
+    const int P = q.Lk - q.Lq;
+    if (hi > lo || (tl.n == 0 && first_here)) {
+      const int n = hi - lo;
+      const bool whole = lo == 0 && hi == tl.n;
+      // this wave's rows and their tokens (a wave past the last row works on
+      // copies of it and stores nothing)
+      const int r0 = r_first + rw * QS * 16;
+      const bool wave_live = r0 <= r_last;
+      const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
+      copy_start(q, tl, lo, hi);
+      uint32_t slot = lds0;  // ring slot of the tile computed next
+      const uint8_t *src;
+      uint32_t nrec;
+      constexpr int kAhead = RW == 1 ? SLOTS : SLOTS - 1;
+      st_dst = lds0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        next_tile(src, nrec);
+        copy_k(lds0 + i * SLOT_B, src, nrec);
+        copy_v(lds0 + i * SLOT_B, src, nrec);
+      }
+      st_dst = lds0 + (RW == 1 ? 0 : kAhead * SLOT_B);
+
+      int tok[QS], head[QS];  // of this lane's rows
+      u32x4 qf[QS][NKK];
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs) {
+        const int r = min(r0 + 16 * qs + m, r_last);
+        tok[qs] = small_div(r, a.G);
+        head[qs] = h * a.G + r - tok[qs] * a.G;
+        const uint8_t *qp = a.q + static_cast<int64_t>(q.q0 + tok[qs]) * a.q_rs + head[qs] * a.q_hs;
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) qf[qs][kk] = load16(qp + (8 * g + 32 * kk) * 2);
+      }
+      if (a.window == 0) {
+        // the masks of the tile's tokens, 32-bit words
+        const int w32 = 2 * a.words, cnt = (t_last - t_first + 1) * w32;
+        const uint32_t *mp = reinterpret_cast<const uint32_t *>(a.mask);
+        for (int i = threadIdx.x; i < cnt; i += 64 * RW) {
+          const int t = small_div(i, w32), c = i - t * w32;
+          lds_mask[t * S::MASK_WORDS + c] = mp[(static_cast<int64_t>(q.q0 + t_first + t) * a.mask_rs) * 2 + c];
+        }
+        if constexpr (RW == 1)
+          wave_lds_sync();
+        else
+          __syncthreads();
+      }
+      float m_use[QS], lsum[QS];
+      f32x4 o[QS][NJ];
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs) {
+        m_use[qs] = kNegInf;
+        lsum[qs] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[qs][j] = f32x4{0, 0, 0, 0};
+      }
+
+      // Keys of the tile at `key0` that row block qs of this lane sees: bit
+      // 4 ks + r for key 16 ks + 4 g + r.
+      auto seen = [&](int qs, int key0, bool ok) -> uint32_t {
+        uint32_t v = 0;
+        if (a.window > 0) {
+          const int top = P + tok[qs], bot = top - a.window;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+            v |= (key <= top && (key > bot || key < a.sinks)) ? 1u << i : 0u;
+          }
+        } else {
+          const int rel = key0 - P, w32 = 2 * a.words;
+          const uint32_t *mr = lds_mask + (tok[qs] - t_first) * S::MASK_WORDS;
+          uint32_t bits;
+          if (rel < 0) {
+            bits = rel <= -32 ? ~0u : (mr[0] << -rel) | ((1u << -rel) - 1u);
+          } else {
+            const int c = rel >> 5, sh = rel & 31;
+            const uint32_t b0 = c < w32 ? mr[c] : 0u, b1 = c + 1 < w32 ? mr[c + 1] : 0u;
+            bits = sh ? (b0 >> sh) | (b1 << (32 - sh)) : b0;
+          }
+          const int left = q.Lk - key0;
+          if (left < 32) bits &= (1u << left) - 1u;
+          v = ((bits >> (4 * g)) & 15u) | (((bits >> (16 + 4 * g)) & 15u) << 4);
+        }
+        return ok ? v : 0u;
+      };
+
+      // Scores -> P of the tile (units packed for the second product), with
+      // the rows' maxima and sums; returns nothing else.
+      f32x4 sc[QS][2];
+      u32x4 pb[QS];
+      uint32_t vis[QS];
+      auto softmax = [&](bool masked) {
+        float mloc[QS];
+        bool grow = false;
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (!((vis[qs] >> i) & 1u)) sc[qs][i >> 2][i & 3] = kNegInf;
+          }
+          mloc[qs] = max3_raw(max3_raw(sc[qs][0][0], sc[qs][0][1], sc[qs][0][2]),
+                              max3_raw(sc[qs][0][3], sc[qs][1][0], sc[qs][1][1]),
+                              vmax_raw(sc[qs][1][2], sc[qs][1][3])) * sl2;
+          grow |= mloc[qs] > m_use[qs] + kRescale;
+        }
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) {
+            const float mn = fmaxf(m_use[qs], max32_raw(max16_raw(mloc[qs])));
+            const float alpha = m_use[qs] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m_use[qs] - mn);
+            lsum[qs] *= alpha;
+            m_use[qs] = mn;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[qs][j] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          const float ref = m_use[qs] == kNegInf ? 0.f : m_use[qs];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -ref));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -ref));
+            lsum[qs] += e0 + e1;
+            pb[qs][t] = T::pack2(e0, e1);
+          }
+        }
+      };
+      auto scores = [&](uint32_t kt) {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) sc[qs][0] = sc[qs][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const u32x4 kf = k_op(kt, kk, ks);
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) sc[qs][ks] = T::mfma16x16x32(kf, qf[qs][kk], sc[qs][ks]);
+          }
+      };
+      auto values = [&](uint32_t kt) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const u32x4 vf = v_op(kt, j);
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(vf, pb[qs], o[qs][j]);
+        }
+      };
+      // The same for a tile that not every row sees whole: 0 * NaN must not
+      // reach a row through a key it does not see.  Values that are not finite
+      // are taken out of the product; a product of their indicators with the
+      // visible keys' then tells which rows see one.
+      auto fix_values = [&](uint32_t kt) {
+        constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
+        constexpr uint32_t kMant = T::dtype == NQ_BF16 ? 0x007fu : 0x03ffu;
+        constexpr uint32_t kOne = T::kOne2 & 0xffffu;
+        u32x4 ones[QS];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            ones[qs][t] = (((vis[qs] >> (2 * t)) & 1u) ? kOne : 0u) | (((vis[qs] >> (2 * t + 1)) & 1u) ? kOne << 16 : 0u);
+#pragma unroll 1
+        for (int j = 0; j < NJ; ++j) {
+          u32x4 vf = v_op(kt, j);
+          u32x4 nan{0, 0, 0, 0}, up{0, 0, 0, 0}, down{0, 0, 0, 0};
+          uint32_t any = 0;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t x = (vf[t] >> (16 * half)) & 0xffffu;
+              if ((x & kExp) == kExp) {
+                any = 1;
+                vf[t] &= half ? 0x0000ffffu : 0xffff0000u;
+                const uint32_t one = kOne << (16 * half);
+                if (x & kMant) nan[t] |= one;
+                else if (x & 0x8000u) down[t] |= one;
+                else up[t] |= one;
+              }
+            }
+          const bool odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+#pragma unroll
+          for (int jj = 0; jj < NJ; ++jj)  // a constant index: o stays in registers
+            if (jj == j) {
+#pragma unroll
+              for (int qs = 0; qs < QS; ++qs) {
+                o[qs][jj] = T::mfma16x16x32(vf, pb[qs], o[qs][jj]);
+                if (odd) {
+                  const f32x4 zero{0, 0, 0, 0};
+                  const f32x4 cn = T::mfma16x16x32(nan, ones[qs], zero), cu = T::mfma16x16x32(up, ones[qs], zero),
+                              cd = T::mfma16x16x32(down, ones[qs], zero);
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    if (cu[r] > 0.f) o[qs][jj][r] += __builtin_huge_valf();
+                    if (cd[r] > 0.f) o[qs][jj][r] -= __builtin_huge_valf();
+                    if (cn[r] > 0.f) o[qs][jj][r] = __builtin_nanf("");
+                  }
+                }
+              }
+            }
+        }
+      };
+      // Whether the tile's values are all finite (the wave's operands of them
+      // cover the whole tile).
+      auto finite = [&](uint32_t kt) -> bool {
+        constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
+        uint32_t any = 0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const u32x4 vf = v_op(kt, j);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            any |= ((vf[t] & kExp) == kExp || (vf[t] & (kExp << 16)) == kExp << 16) ? 1u : 0u;
+        }
+        return __builtin_amdgcn_ballot_w64(any != 0) == 0;
+      };
+      // What the wave does with the tile at list position i: 0 nothing, 1 every
+      // key is seen by every row, 2 masked.
+      auto kind_of = [&](int i, int key0) -> int {
+        if (!wave_live) return 0;
+        if ((bad >> (i & 63)) & 1) return 0;
+        if (a.window == 0) return key0 + kKeys <= P ? 1 : 2;
+        const int pa = P + ta, pz = P + tb;
+        if (key0 > pz || (key0 + kKeys - 1 <= pa - a.window && key0 >= a.sinks)) return 0;
+        return key0 + kKeys - 1 <= pa && (key0 > pz - a.window || key0 + kKeys <= a.sinks) ? 1 : 2;
+      };
+
+      for (int i = lo; i < hi; ++i) {
+        const int key0 = (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys;
+        if constexpr (RW == 1) {
+          wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // K of this tile (younger: its V and the tiles after it)
+          asm volatile("" ::: "memory");
+          const int kind = kind_of(i, key0);
+          if (kind != 0) scores(slot);
+          wait_lgkmcnt0();  // the K operands are read: the slot's K is free
+          next_tile(src, nrec);
+          copy_k(slot, src, nrec);
+          if (kind == 2) vis[0] = seen(0, key0, true);
+          if (kind != 0) softmax(kind == 2);
+          wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
+          asm volatile("" ::: "memory");
+          if (kind == 2 && !finite(slot))
+            fix_values(slot);
+          else if (kind != 0)
+            values(slot);
+          wait_lgkmcnt0();
+          copy_v(slot, src, nrec);
+        } else {
+          wait_vmcnt<2 * COPS * (kAhead - 1)>();  // this wave's part of the tile
+          wait_lgkmcnt0();                        // and its reads of the tile before
+          raw_barrier();
+          next_tile(src, nrec);
+          copy_k(st_dst, src, nrec);
+          copy_v(st_dst, src, nrec);
+          st_dst = st_dst == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : st_dst + SLOT_B;
+          const int kind = kind_of(i, key0);
+          if (kind != 0) {
+            scores(slot);
+            if (kind == 2) {
+#pragma unroll
+              for (int qs = 0; qs < QS; ++qs) vis[qs] = seen(qs, key0, true);
+            }
+            softmax(kind == 2);
+            if (kind == 2 && !finite(slot))
+              fix_values(slot);
+            else
+              values(slot);
+          }
+        }
+        slot = slot == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : slot + SLOT_B;
+      }
+
+      // ---- epilogue: lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs) {
+        const float l = sum32(sum16(lsum[qs]));
+        const float inv = (l > 0.f ? 1.0f / l : 0.f) * vscale;
+        const int r = r0 + 16 * qs + m;
+        if (!whole) {
+          const int64_t unit = (static_cast<int64_t>(2 * w_of + (lo > 0 ? 0 : 1)) * RW + rw) * QS + qs;
+          f32x4 *po = reinterpret_cast<f32x4 *>(a.part_o) + unit * NJ * 64 + lane;
+          if (r <= r_last) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) po[j * 64] = o[qs][j] * inv;
+            if (g == 0) a.part_l[unit * 16 + m] = l == 0.f ? kNegInf : m_use[qs] + __log2f(l);
+          }
+        } else if (r <= r_last) {
+          uint8_t *op = a.out + static_cast<int64_t>(q.q0 + tok[qs]) * a.o_rs + head[qs] * a.o_hs + 8 * g;
+          const uint8_t *gp = a.gate + static_cast<int64_t>(q.q0 + tok[qs]) * a.g_rs + head[qs] * a.g_hs + 8 * g;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const f32x4 v = o[qs][j] * inv;
+            *reinterpret_cast<u32x2 *>(op + 32 * j) =
+                a.gate ? gate4<T>(v, *reinterpret_cast<const u32x2 *>(gp + 32 * j))
+                       : u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+          }
+        }
+      }
+      if (!whole) (lo > 0 ? desc0 : desc1) = int4{s, rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
+    }
+    // the next row tile of the range
+    if (!ranges) break;
+    X += item_cost<S>(a, q);
+    if (++rt >= n_rt) {
+      rt = 0;
+      Seq nx;
+      do {
+        if (++s >= a.num_seqs) break;
+        nx = seq_of(a, s, true);
+      } while (nx.Lq <= 0);
+      if (s >= a.num_seqs) break;
+    }
+    if (X >= pos1) break;
+    // every copy has landed and every read is done before the next item's
+    // copies take the slots
+    wait_vmcnt<0>();
+    wait_lgkmcnt0();
+    if constexpr (RW > 1) raw_barrier();
+  }
+  leave();
+  wait_vmcnt<0>();  // no copy outlives the workgroup's LDS
+}
+
+template <class T, bool FP8, class S>
+__global__ __launch_bounds__(64 * S::RW) __attribute__((amdgpu_waves_per_eu(S::RW == 1 ? 1 : 2)))
+void span_attention_kernel(const SpanArgs a) {
+  span_body<T, FP8, S>(a);
+}
+
+// Merge of the items that ranges cut: workgroup (range, part) takes the item
+// whose first piece lies in the range's slot 1; its other pieces are the slots
+// 0 of the next ranges, up to the one marked last.
+template <class T, class S>
+__global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
+  constexpr int NJ = S::NJ, M = S::M, kUnroll = 8;
+  const int w = blockIdx.x, h = w / a.n_ranges, w_end = (h + 1) * a.n_ranges;
+  const int4 d = a.part_desc[2 * w + 1];
+  if (d.z == kPieceNone) return;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int e = blockIdx.y * 4 + (threadIdx.x >> 6);  // (row block, 16-dim block)
+  const int unit = e / NJ, j = e % NJ;
+  int pieces = 1;
+  for (int b = w + 1;; b += 64) {
+    const uint64_t last = __builtin_amdgcn_ballot_w64(b + lane < w_end && a.part_desc[2 * min(b + lane, w_end - 1)].z == kPieceLast);
+    if (last != 0) {
+      pieces += static_cast<int>(__builtin_ctzll(last)) + 1;
+      break;
+    }
+    if (b + 64 >= w_end) return;  // not reached: every cut item has a last piece
+    pieces += 64;
+  }
+  const Seq q = seq_of(a, d.x, true);
+  const int r = d.y * M + unit * 16 + m;
+  if (r >= q.Lq * a.G) return;
+  float mx = kNegInf, W = 0.f;
+  f32x4 acc{0, 0, 0, 0};
+  for (int c = 0; c < pieces; c += kUnroll) {
+    float l[kUnroll];
+    f32x4 p[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      l[u] = kNegInf;
+      if (c + u < pieces) {
+        const int64_t at = static_cast<int64_t>(2 * (w + c + u) + (c + u == 0 ? 1 : 0)) * S::RW * S::QS + unit;
+        l[u] = a.part_l[at * 16 + m];
+        p[u] = reinterpret_cast<const f32x4 *>(a.part_o)[(at * NJ + j) * 64 + lane];
+      }
+    }
+    float mc = mx;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) mc = fmaxf(mc, l[u]);
+    const float mu = mc == kNegInf ? 0.f : mc;
+    const float f = __builtin_amdgcn_exp2f(mx - mu);
+    W *= f;
+    acc *= f;
+    mx = mc;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (l[u] != kNegInf) {
+        const float x = __builtin_amdgcn_exp2f(l[u] - mu);
+        W += x;
+        acc += p[u] * x;
+      }
+  }
+  acc *= W > 0.f ? 1.0f / W : 0.f;
+  const int t = small_div(r, a.G), head = h * a.G + r - t * a.G;
+  uint8_t *op = a.out + static_cast<int64_t>(q.q0 + t) * a.o_rs + head * a.o_hs + 32 * j + 8 * g;
+  *reinterpret_cast<u32x2 *>(op) =
+      a.gate ? gate4<T>(acc, *reinterpret_cast<const u32x2 *>(a.gate + static_cast<int64_t>(q.q0 + t) * a.g_rs +
+                                                              head * a.g_hs + 32 * j + 8 * g))
+             : u32x2{T::pack2(acc[0], acc[1]), T::pack2(acc[2], acc[3])};
+}
+
+// ---------------------------------------------------------------- launch
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+template <class T, bool FP8, class S>
+int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t workspace_bytes, int64_t *need,
+           hipStream_t stream) {
+  // row tiles of the batch, at most: every sequence's last one may be partial
+  const int64_t by_total = static_cast<int64_t>(a.total_q) * a.G / S::M + a.num_seqs;
+  const int64_t items = std::min(by_total, a.num_seqs * ((max_rows + S::M - 1) / S::M));
+  const int64_t slots = static_cast<int64_t>(device_cus()) * per_cu;
+  const int64_t max_cost = (static_cast<int64_t>(a.max_k) + kKeys - 1) / kKeys + Cost<S>::kItem;
+  a.n_ranges = 0;
+  // Equal ranges while whole items would leave the chip uneven.
+  if (items * a.Hkv < 4 * slots && by_total * max_cost < (int64_t{1} << 31)) {
+    const int per = a.Hkv < 8 && 8 % a.Hkv == 0 ? 8 / a.Hkv : 1;
+    const int64_t most = by_total * max_cost / Cost<S>::kMinRange + 1;  // ranges that can have work
+    int64_t W = std::max<int64_t>(1, std::min(slots / a.Hkv, most));
+    W = (W + per - 1) / per * per;
+    const int64_t n = W * a.Hkv * 2;
+    const int64_t o_bytes = align256(n * S::M * S::D * 4), l_bytes = align256(n * S::M * 4);
+    const int64_t bytes = o_bytes + l_bytes + align256(n * 16);
+    if (!workspace || workspace_bytes < bytes) {
+      if (!need)
+        return fail(NQ_EINVAL, "span attention: workspace %lld bytes < %lld", (long long)workspace_bytes,
+                    (long long)bytes);
+      *need = bytes;
+      return 1;
+    }
+    if (!aligned(workspace, 256)) return fail(NQ_EINVAL, "span attention: workspace must be 256-byte aligned");
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    a.n_ranges = static_cast<int>(W);
+    a.part_o = reinterpret_cast<float *>(ws);
+    a.part_l = reinterpret_cast<float *>(ws + o_bytes);
+    a.part_desc = reinterpret_cast<int4 *>(ws + o_bytes + l_bytes);
+    span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(W * a.Hkv)), 64 * S::RW, S::LDS_B, stream>>>(a);
+    const int rc = check_launch("span attention");
+    if (rc != NQ_OK || W <= 1) return rc;
+    span_merge_kernel<T, S><<<dim3(static_cast<unsigned>(W * a.Hkv), S::RW * S::QS * S::NJ / 4), 256, 0, stream>>>(a);
+    return check_launch("span attention (merge)");
+  }
+  const int per = a.Hkv < 8 && 8 % a.Hkv == 0 ? 8 / a.Hkv : 1;
+  const int64_t grid = (items + per - 1) / per * per * a.Hkv;
+  if (grid > 0x7fffffff) return fail(NQ_EINVAL, "span attention: %lld work items", (long long)grid);
+  span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(grid)), 64 * S::RW, S::LDS_B, stream>>>(a);
+  return check_launch("span attention");
+}
+
+template <class T, bool FP8>
+int launch_shape(const SpanArgs &a, int D, int64_t max_rows, void *ws, int64_t ws_bytes, int64_t *need, hipStream_t s) {
+  if (D == 256) {
+    if (max_rows <= 16)
+      return launch<T, FP8, Shape<256, FP8, 1, 1, 2>>(a, max_rows, FP8 ? 4 : 2, ws, ws_bytes, need, s);
+    if (max_rows <= 64)
+      return launch<T, FP8, Shape<256, FP8, 4, 1, FP8 ? 4 : 2>>(a, max_rows, 2, ws, ws_bytes, need, s);
+    return launch<T, FP8, Shape<256, FP8, 8, 1, 4>>(a, max_rows, 1, ws, ws_bytes, need, s);
+  }
+  if (max_rows <= 16)
+    return launch<T, FP8, Shape<128, FP8, 1, 1, FP8 ? 4 : 2>>(a, max_rows, 4, ws, ws_bytes, need, s);
+  if (max_rows <= 64) return launch<T, FP8, Shape<128, FP8, 4, 1, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
+  return launch<T, FP8, Shape<128, FP8, 4, 2, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
+}
+
+// What the three entry points share: checks and the launch of `a`, whose
+// pointers, byte strides and mode are set.
+int run(const char *what, SpanArgs a, int head_dim, int64_t max_rows, int q_dtype, int kv_dtype, void *workspace,
+        int64_t workspace_bytes, int64_t *need, void *stream) {
+  const bool fp8 = kv_dtype == NQ_FP8_E4M3;
+  if (a.num_seqs < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hkv > 65535 || a.total_q < 0)
+    return fail(NQ_EINVAL, "%s: bad sequence or head counts", what);
+  if (a.Hq % a.Hkv != 0)
+    return fail(NQ_EINVAL, "%s: num_q_heads %d not a multiple of num_kv_heads %d", what, a.Hq, a.Hkv);
+  a.G = a.Hq / a.Hkv;
+  if (a.G > 16) return fail(NQ_EUNSUPPORTED, "%s: GQA group %d > 16", what, a.G);
+  if (head_dim != 128 && head_dim != 256)
+    return fail(NQ_EUNSUPPORTED, "%s: head_dim %d (built: 128, 256)", what, head_dim);
+  if (q_dtype != NQ_BF16 && q_dtype != NQ_F16)
+    return fail(NQ_EUNSUPPORTED, "%s: q dtype %d (need f16/bf16)", what, q_dtype);
+  if (!fp8 && kv_dtype != q_dtype)
+    return fail(NQ_EUNSUPPORTED, "%s: kv dtype %d with q dtype %d", what, kv_dtype, q_dtype);
+  if (fp8 && (!a.k_scale || !a.v_scale)) return fail(NQ_EINVAL, "%s: fp8 K/V needs scales", what);
+  if (!(a.scale_log2 > 0.f)) return fail(NQ_EINVAL, "%s: softmax_scale must be positive", what);
+  if (a.num_seqs == 0 || a.total_q == 0) return NQ_OK;
+  if (!a.q || !a.k || !a.v || !a.cu_k || !a.out) return fail(NQ_EINVAL, "%s: null pointer", what);
+  if (a.block_tables) {
+    if (a.block_size <= 0 || a.block_size % kKeys != 0 || a.block_size > 1 << 26)
+      return fail(NQ_EUNSUPPORTED, "%s: block_size %d must be a multiple of 32", what, a.block_size);
+    if (a.max_blocks <= 0 || a.bt_stride < a.max_blocks) return fail(NQ_EINVAL, "%s: block table width", what);
+  }
+  if (a.q_rs % 16 || a.q_hs % 16 || !aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || a.kv_rs % 16 ||
+      a.o_rs % 8 || a.o_hs % 8 || !aligned(a.out, 8))
+    return fail(NQ_EINVAL, "%s: alignment (q, K/V rows: 16 bytes; out: 8)", what);
+  if (a.kv_rs <= 0 || a.kv_rs > (1 << 20)) return fail(NQ_EINVAL, "%s: K/V row stride %lld bytes", what, (long long)a.kv_rs);
+  if (a.gate && (a.g_rs % 8 || a.g_hs % 8 || !aligned(a.gate, 8)))
+    return fail(NQ_EINVAL, "%s: gate must be 8-byte aligned", what);
+  // rows of a sequence and tiles of its keys are divided by small_div
+  if (max_rows <= 0 || max_rows >= 1 << 22 || static_cast<int64_t>(a.total_q) * a.G > (int64_t{1} << 30))
+    return fail(NQ_EINVAL, "%s: %lld rows per kv head", what, (long long)max_rows);
+  if (a.max_k < 0 || a.max_k >= 1 << 26) return fail(NQ_EINVAL, "%s: %d tokens in a sequence", what, a.max_k);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (q_dtype == NQ_BF16)
+    return fp8 ? launch_shape<BF16, true>(a, head_dim, max_rows, workspace, workspace_bytes, need, s)
+               : launch_shape<BF16, false>(a, head_dim, max_rows, workspace, workspace_bytes, need, s);
+  return fp8 ? launch_shape<F16, true>(a, head_dim, max_rows, workspace, workspace_bytes, need, s)
+             : launch_shape<F16, false>(a, head_dim, max_rows, workspace, workspace_bytes, need, s);
+}
+
+}  // namespace
+}  // namespace nq
+
+using namespace nq;
+
+extern "C" int nq_tree_attention(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+                                 const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                 int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables, int64_t bt_stride,
+                                 int max_blocks_per_seq, int64_t num_blocks, const int64_t *tree_mask,
+                                 int64_t mask_row_stride, int mask_words, void *out, int64_t out_row_stride,
+                                 int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                                 int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                                 int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
+                                 int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                                 int64_t workspace_bytes, int64_t *need, void *stream) {
+  const char *what = "tree_attention";
+  if (max_seqlen_q < 0 || max_seqlen_q > kMaxNodes)
+    return fail(NQ_EUNSUPPORTED, "%s: trees of %d nodes (at most %d)", what, max_seqlen_q, kMaxNodes);
+  if (mask_words < (max_seqlen_q + 63) / 64 || mask_words > kMaxNodes / 64 || mask_row_stride < mask_words)
+    return fail(NQ_EINVAL, "%s: %d mask words for %d nodes", what, mask_words, max_seqlen_q);
+  if (num_seqs > 0 && total_q > 0 && (!block_tables || !tree_mask || !cu_seqlens_q || !aligned(tree_mask, 8)))
+    return fail(NQ_EINVAL, "%s: null (or unaligned) pointer", what);
+  if (total_q > 0x7fffffff) return fail(NQ_EINVAL, "%s: %lld rows", what, (long long)total_q);
+  if (max_seqlen_q == 0) return NQ_OK;
+  SpanArgs a{};
+  a.q = static_cast<const uint8_t *>(q);
+  a.q_rs = q_row_stride * 2;
+  a.q_hs = q_head_stride * 2;
+  a.k = static_cast<const uint8_t *>(k_cache);
+  a.v = static_cast<const uint8_t *>(v_cache);
+  a.kv_rs = static_cast<int64_t>(num_kv_heads) * head_dim * elem_size(kv_dtype);
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.total_q = static_cast<int>(total_q);
+  a.max_q = max_seqlen_q;
+  a.max_k = static_cast<int>(std::min<int64_t>(max_seqlen_k, static_cast<int64_t>(max_blocks_per_seq) * block_size));
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = static_cast<int>(std::min<int64_t>(num_blocks, 0x7fffffff));
+  a.out = static_cast<uint8_t *>(out);
+  a.o_rs = out_row_stride * 2;
+  a.o_hs = out_head_stride * 2;
+  a.gate = static_cast<const uint8_t *>(gate);
+  a.g_rs = gate_row_stride * 2;
+  a.g_hs = gate_head_stride * 2;
+  a.Hq = num_q_heads;
+  a.Hkv = num_kv_heads;
+  a.block_size = block_size;
+  a.num_seqs = num_seqs;
+  a.mask = reinterpret_cast<const uint64_t *>(tree_mask);
+  a.mask_rs = mask_row_stride;
+  a.words = mask_words;
+  a.scale_log2 = softmax_scale * kLog2e;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  return run(what, a, head_dim, static_cast<int64_t>(max_seqlen_q) * (num_kv_heads > 0 ? num_q_heads / num_kv_heads : 1),
+             q_dtype, kv_dtype, workspace, workspace_bytes, need, stream);
+}
+
+extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                                 const void *v, int64_t kv_row_stride, int64_t total_k, const int32_t *cu_seqlens_q,
+                                 const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
+                                 const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                 int64_t num_blocks, int window, int num_sinks, void *out, int64_t out_row_stride,
+                                 int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                                 int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                                 int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
+                                 int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                                 int64_t workspace_bytes, int64_t *need, void *stream) {
+  const char *what = "window_prefill";
+  if (window <= 0 || num_sinks < 0) return fail(NQ_EINVAL, "%s: window %d, sinks %d", what, window, num_sinks);
+  if (num_seqs > 0 && total_q > 0 && !cu_seqlens_q) return fail(NQ_EINVAL, "%s: null pointer", what);
+  if (total_q > 0x7fffffff || total_k > 0x7fffffff || max_seqlen_q < 0)
+    return fail(NQ_EINVAL, "%s: %lld rows, %lld keys", what, (long long)total_q, (long long)total_k);
+  if (max_seqlen_q == 0) return NQ_OK;
+  SpanArgs a{};
+  a.q = static_cast<const uint8_t *>(q);
+  a.q_rs = q_row_stride * 2;
+  a.q_hs = q_head_stride * 2;
+  a.k = static_cast<const uint8_t *>(k);
+  a.v = static_cast<const uint8_t *>(v);
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  a.kv_rs = (block_tables ? row : kv_row_stride) * elem_size(kv_dtype);
+  if (!block_tables && kv_row_stride < row)
+    return fail(NQ_EINVAL, "%s: K/V row stride %lld < %lld", what, (long long)kv_row_stride, (long long)row);
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.total_q = static_cast<int>(total_q);
+  a.max_q = max_seqlen_q;
+  a.total_k = static_cast<int>(total_k);
+  a.max_k = block_tables ? static_cast<int>(std::min<int64_t>(max_seqlen_k,
+                                                              static_cast<int64_t>(max_blocks_per_seq) * block_size))
+                         : max_seqlen_k;
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = static_cast<int>(std::min<int64_t>(num_blocks, 0x7fffffff));
+  a.out = static_cast<uint8_t *>(out);
+  a.o_rs = out_row_stride * 2;
+  a.o_hs = out_head_stride * 2;
+  a.gate = static_cast<const uint8_t *>(gate);
+  a.g_rs = gate_row_stride * 2;
+  a.g_hs = gate_head_stride * 2;
+  a.Hq = num_q_heads;
+  a.Hkv = num_kv_heads;
+  a.block_size = block_size;
+  a.num_seqs = num_seqs;
+  a.window = std::min(window, 1 << 28);
+  a.sinks = std::min(num_sinks, 1 << 28);
+  a.scale_log2 = softmax_scale * kLog2e;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  return run(what, a, head_dim, static_cast<int64_t>(max_seqlen_q) * (num_kv_heads > 0 ? num_q_heads / num_kv_heads : 1),
+             q_dtype, kv_dtype, workspace, workspace_bytes, need, stream);
+}
+
+extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                                const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                                int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
+                                void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
+                                int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                                float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
+                                const float *v_scale, const void *gate, int64_t gate_batch_stride,
+                                int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,
+                                void *stream) {
+  const char *what = "window_decode";
+  if (window <= 0 || num_sinks < 0) return fail(NQ_EINVAL, "%s: window %d, sinks %d", what, window, num_sinks);
+  if (batch > 0 && !block_tables) return fail(NQ_EINVAL, "%s: null pointer", what);
+  SpanArgs a{};
+  a.q = static_cast<const uint8_t *>(q);
+  a.q_rs = q_batch_stride * 2;
+  a.q_hs = q_head_stride * 2;
+  a.k = static_cast<const uint8_t *>(k_cache);
+  a.v = static_cast<const uint8_t *>(v_cache);
+  a.kv_rs = static_cast<int64_t>(num_kv_heads) * head_dim * elem_size(kv_dtype);
+  a.cu_k = context_lens;
+  a.total_q = batch;
+  a.max_q = 1;
+  a.max_k = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(max_blocks_per_seq) * block_size, (1 << 26) - 1));
+  a.block_tables = block_tables;
+  a.bt_stride = bt_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = static_cast<int>(std::min<int64_t>(num_blocks, 0x7fffffff));
+  a.out = static_cast<uint8_t *>(out);
+  a.o_rs = out_batch_stride * 2;
+  a.o_hs = out_head_stride * 2;
+  a.gate = static_cast<const uint8_t *>(gate);
+  a.g_rs = gate_batch_stride * 2;
+  a.g_hs = gate_head_stride * 2;
+  a.Hq = num_q_heads;
+  a.Hkv = num_kv_heads;
+  a.block_size = block_size;
+  a.num_seqs = batch;
+  a.window = std::min(window, 1 << 28);
+  a.sinks = std::min(num_sinks, 1 << 28);
+  a.scale_log2 = softmax_scale * kLog2e;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  return run(what, a, head_dim, num_kv_heads > 0 ? num_q_heads / num_kv_heads : 1, q_dtype, kv_dtype, workspace,
+             workspace_bytes, need, stream);
+}

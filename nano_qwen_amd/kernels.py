@@ -37,6 +37,7 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _prefill_queues: dict[tuple[int, int], torch.Tensor] = {}
 _prefill_parts: dict[tuple[int, int], torch.Tensor] = {}
 _gdn_segments: dict[tuple[int, int], torch.Tensor] = {}
+_span_parts: dict[tuple[int, int], torch.Tensor] = {}
 _retired: list[torch.Tensor] = []
 # Zeroed arrival counters of the one-launch decode: a pool per device, one half
 # for streams (_decode_counters, and _shared_counters for captures that found no
@@ -85,14 +86,14 @@ def _grow(table, key, nbytes, dtype, device, zero=False):
 def release_workspaces(device=None) -> int:
     """Drop the kernels' per-stream buffers (decode split-K workspaces and
     arrival counters, prefill queue counters and partial outputs, GDN segment
-    states) and every retired buffer, of ``device`` or of all devices; returns
+    states, windowed and tree attention's partial outputs) and every retired buffer, of ``device`` or of all devices; returns
     how many were dropped.  Only safe once no HIP graph captured with them will
     be replayed again (a replay would write freed memory) and while no other
     thread calls the kernels.  Later calls allocate fresh buffers (the counters
     start at zero again)."""
     idx = None if device is None else _key(device)[0]
     n = 0
-    for table in (_workspaces, _prefill_queues, _prefill_parts, _gdn_segments, _decode_counters,
+    for table in (_workspaces, _prefill_queues, _prefill_parts, _gdn_segments, _span_parts, _decode_counters,
                   _shared_counters, _capture_counters):
         for key in [k for k in table if idx is None or k[0] == idx]:
             del table[key]
@@ -710,6 +711,273 @@ def gdn_conv1d(x, weight, conv_state, state_indices, cu_seqlens=None, out=None):
     return out
 
 
+# ------------------------------------------------- windows, trees and pages
+# (no counterpart in the reference, whose attention is causal over the whole
+# context and whose pages never move)
+
+def _check_one_device(what, first, *others):
+    require_cuda(first, *others, what=what)
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"{what}: tensors on several devices")
+    return dev
+
+
+def _rows_of(what, name, t, shape, dtype):
+    """(pointer, row stride, head stride) of a ``[rows, heads, dim]`` tensor of ``shape``."""
+    t3 = t.squeeze(1) if t.dim() == 4 and t.shape[1] == 1 else t
+    if t3.shape != shape or t3.stride(-1) != 1 or t3.dtype != dtype:
+        raise RuntimeError(f"{what}: {name} must be {list(shape)} of {dtype} with a contiguous last dim")
+    return t3.data_ptr(), t3.stride(0), t3.stride(1)
+
+
+def _paged_args(what, d, k_cache, v_cache, block_table, n):
+    """(blocks, block_size, kv heads) of paged K/V and their table, checked."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != d or \
+            not (k_cache.is_contiguous() and v_cache.is_contiguous()) or v_cache.dtype != k_cache.dtype:
+        raise RuntimeError(f"{what}: caches must be contiguous [num_blocks, block_size, Hkv, {d}] of one dtype")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n or \
+            block_table.shape[1] == 0 or block_table.stride(1) != 1:
+        raise RuntimeError(f"{what}: block_table must be int32 [sequences, width] with contiguous rows")
+    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+
+
+def _scale_args(what, kv_dtype, hkv, k_scale, v_scale):
+    if kv_dtype != torch.float8_e4m3fn:
+        return None, None
+    for t in (k_scale, v_scale):
+        if t is None or t.dtype != torch.float32 or t.numel() != hkv or not t.is_contiguous():
+            raise RuntimeError(f"{what}: fp8 K/V needs k_scale and v_scale, contiguous float32 [{hkv}]")
+    return k_scale.data_ptr(), v_scale.data_ptr()
+
+
+def _check_cu(what, n1, *tensors):
+    for t in tensors:
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n1 or not t.is_contiguous():
+            raise RuntimeError(f"{what}: cu_seqlens must be contiguous int32 [sequences + 1]")
+
+
+def _launch_span(what, fn, device, args):
+    """Calls ``fn(*args, workspace, bytes, need, stream)``, which asks once for a workspace of its size: the
+    stream's own, or during a capture one of the graph's (whose replays may then overlap other calls)."""
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch_span(what, fn, device, args)
+    key = device, raw_stream(device)
+    need = ctypes.c_int64()
+    capturing = key[1] != 0 and _capturing(key)    # the null stream cannot be captured
+    with _launch_locks[hash(key) & 63]:
+        ws = None if capturing else _span_parts.get(key)
+        while True:
+            rc = fn(*args, ptr(ws), 0 if ws is None else ws.numel(), need, key[1])
+            if rc != 1:
+                break
+            if capturing:
+                ws = torch.empty(need.value, dtype=torch.uint8, device=torch.device("cuda", device))
+            else:
+                ws = _grow(_span_parts, key, need.value, torch.uint8, torch.device("cuda", device))
+    check(rc, what)
+
+
+def tree_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                   block_table, tree_mask, k_scale=None, v_scale=None, out=None, gate=None):
+    """Attention of trees of drafted tokens over the paged cache; ``q [T, Hq, D]`` -> ``[T, Hq, D]``.
+
+    Sequence s's nodes are the rows ``cu_seqlens_q[s] : cu_seqlens_q[s + 1]``, their keys and values already
+    stored as its last cached tokens, in that order; ``cu_seqlens_k`` counts the cached tokens, nodes included.
+    Every node sees the tokens before the tree, and node j of its own tree where bit ``j % 64`` of
+    ``tree_mask[row, j // 64]`` (int64 ``[T, words]``, or ``[T]`` for one word) is set: usually its ancestors
+    and itself (``tree_masks``).  At most 256 nodes per tree.  ``gate`` as for ``varlen_prefill``.
+    """
+    what = "tree_attention"
+    dev = _check_one_device(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, tree_mask, k_scale,
+                            v_scale, out, gate)
+    if q.dim() != 3:
+        raise RuntimeError(f"{what}: q must be [T, Hq, D]")
+    tq, hq, d = q.shape
+    n = cu_seqlens_q.numel() - 1
+    _check_cu(what, n + 1, cu_seqlens_q, cu_seqlens_k)
+    nb, bs, hkv = _paged_args(what, d, k_cache, v_cache, block_table, n)
+    mask = tree_mask[:, None] if tree_mask.dim() == 1 else tree_mask
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != tq or \
+            (mask.shape[1] > 1 and mask.stride(1) != 1):
+        raise RuntimeError(f"{what}: tree_mask must be int64 [T, words] with contiguous rows")
+    if out is None:
+        out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
+    qa, oa = _rows_of(what, "q", q, q.shape, q.dtype), _rows_of(what, "out", out, q.shape, q.dtype)
+    ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
+    words = mask.shape[1]
+    _launch_span(what, lib().nq_tree_attention, dev, (
+        *qa, k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+        int(max_seqlen_q), int(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb,
+        mask.data_ptr(), mask.stride(0) if tq > 1 else words, words, *oa, n, tq, hq, hkv, d, bs, float(softmax_scale),
+        dtype_code(q.dtype), dtype_code(k_cache.dtype), *_scale_args(what, k_cache.dtype, hkv, k_scale, v_scale), *ga))
+    return out
+
+
+def window_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, window,
+                   num_sinks=0, block_table=None, k_scale=None, v_scale=None, out=None, gate=None):
+    """``varlen_prefill`` (causal) where the token at position p sees the ``window`` tokens up to itself and the
+    sequence's first ``num_sinks``: keys ``j <= p`` with ``j > p - window`` or ``j < num_sinks``.
+
+    Table entries of pages that no token of the call sees are not used (``ModelRunner.release_window_blocks``).
+    """
+    what = "window_prefill"
+    dev = _check_one_device(what, q, k, v, cu_seqlens_q, cu_seqlens_k, block_table, k_scale, v_scale, out, gate)
+    if q.dim() != 3:
+        raise RuntimeError(f"{what}: q must be [T, Hq, D]")
+    tq, hq, d = q.shape
+    n = cu_seqlens_q.numel() - 1
+    _check_cu(what, n + 1, cu_seqlens_q, cu_seqlens_k)
+    if block_table is None:
+        if k.dim() != 3 or k.shape != v.shape or k.shape[2] != d or k.stride(2) != 1 or v.stride(2) != 1 or \
+                k.stride(1) != d or v.stride(1) != d or k.stride(0) != v.stride(0) or k.dtype != v.dtype:
+            raise RuntimeError(f"{what}: packed k/v must be [Tk, Hkv, {d}] with contiguous heads and equal strides")
+        hkv, pa, kv_rs, tk = k.shape[1], (None, 0, 0, 0), k.stride(0), k.shape[0]
+        nb = bs = 0
+        if tk <= 1:
+            kv_rs = hkv * d
+    else:
+        nb, bs, hkv = _paged_args(what, d, k, v, block_table, n)
+        pa, kv_rs, tk = (block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb), 0, 0
+    if out is None:
+        out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
+    qa, oa = _rows_of(what, "q", q, q.shape, q.dtype), _rows_of(what, "out", out, q.shape, q.dtype)
+    ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
+    _launch_span(what, lib().nq_window_prefill, dev, (
+        *qa, k.data_ptr(), v.data_ptr(), kv_rs, tk, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+        int(max_seqlen_q), int(max_seqlen_k), *pa, int(window), int(num_sinks), *oa, n, tq, hq, hkv, d, bs,
+        float(softmax_scale), dtype_code(q.dtype), dtype_code(k.dtype),
+        *_scale_args(what, k.dtype, hkv, k_scale, v_scale), *ga))
+    return out
+
+
+def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, window, num_sinks=0,
+                  k_scale=None, v_scale=None, out=None, gate=None, k=None, v=None, slot_mapping=None):
+    """``paged_decode`` where the new token sees the last ``window`` cached tokens (itself among them) and the
+    sequence's first ``num_sinks``.
+
+    ``q [B, 1, Hq, D]`` (or ``[B, Hq, D]``); returns ``out`` shaped like ``q``.  With ``k, v [B, Hkv, D]`` and
+    ``slot_mapping [B]`` the new token is stored first, as ``store_kvcache`` stores it.
+    """
+    what = "window_decode"
+    dev = _check_one_device(what, q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out, gate, k, v,
+                            slot_mapping)
+    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1):
+        raise RuntimeError(f"{what}: q must be [B, 1, Hq, D] or [B, Hq, D]")
+    B, hq, d = q.shape[0], q.shape[-2], q.shape[-1]
+    nb, bs, hkv = _paged_args(what, d, k_cache, v_cache, block_table, B)
+    if cache_seqlens.dtype != torch.int32 or cache_seqlens.numel() != B or not cache_seqlens.is_contiguous():
+        raise RuntimeError(f"{what}: cache_seqlens must be contiguous int32 [B]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    shape = torch.Size((B, hq, d))
+    qa, oa = _rows_of(what, "q", q, shape, q.dtype), _rows_of(what, "out", out, shape, q.dtype)
+    ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, shape, q.dtype)
+    scales = _scale_args(what, k_cache.dtype, hkv, k_scale, v_scale)
+    if k is not None:
+        store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    _launch_span(what, lib().nq_window_decode, dev, (
+        *qa, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[1], cache_seqlens.data_ptr(), int(window), int(num_sinks), *oa, B, hq, hkv, d, bs, nb,
+        float(softmax_scale), dtype_code(q.dtype), dtype_code(k_cache.dtype), *scales, *ga))
+    return out
+
+
+def _pool(what, kv_cache):
+    """(slabs, blocks, block_size, bytes of a row) of a pool ``[..., num_blocks, block_size, Hkv, D]``."""
+    if kv_cache.dim() < 4 or not kv_cache.is_contiguous():
+        raise RuntimeError(f"{what}: kv_cache must be contiguous [..., num_blocks, block_size, Hkv, D]")
+    *lead, nb, bs, hkv, d = kv_cache.shape
+    slabs = 1
+    for x in lead:
+        slabs *= x
+    return slabs, nb, bs, hkv * d * kv_cache.element_size()
+
+
+def _id_list(what, name, t, n):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be contiguous int32 [{n}]")
+    return t.data_ptr()
+
+
+def copy_kv_blocks(kv_cache, src_blocks, dst_blocks, num_tokens=None):
+    """Pages ``src_blocks [n]`` to pages ``dst_blocks [n]`` in every layer's K and V, in one launch.
+
+    ``kv_cache`` is the runner's pool ``[2, L, num_blocks, block_size, Hkv, D]`` or any contiguous
+    ``[..., num_blocks, block_size, Hkv, D]``.  ``num_tokens [n]`` copies the first rows of each page only (a
+    fork's last, partly filled page).  Pairs with an id outside the pool are skipped.  A page that is written may
+    appear in no other pair: the pairs are copied in any order.  int32 tensors on the pool's device.
+    """
+    what = "copy_kv_blocks"
+    dev = _check_one_device(what, kv_cache, src_blocks, dst_blocks, num_tokens)
+    slabs, nb, bs, row = _pool(what, kv_cache)
+    n = src_blocks.numel()
+    args = (_id_list(what, "src_blocks", src_blocks, n), _id_list(what, "dst_blocks", dst_blocks, n),
+            None if num_tokens is None else _id_list(what, "num_tokens", num_tokens, n))
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return copy_kv_blocks(kv_cache, src_blocks, dst_blocks, num_tokens)
+    check(lib().nq_copy_kv_blocks(kv_cache.data_ptr(), slabs, nb, bs, row, *args, n, raw_stream(dev)), what)
+
+
+def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, parents=None, tokens=None,
+                target_tokens=None, path=None, num_accepted=None):
+    """The accepted path of every verified tree, its K/V rows moved to where the sequences go on.
+
+    Sequence s's nodes are rows ``cu_seqlens_q[s] : cu_seqlens_q[s + 1]`` of ``parents [T]`` (int32, indices among
+    its own nodes, below the node's own), ``tokens [T]`` (the drafted ones) and ``target_tokens [T]`` (what the
+    model chose after each node; both int64).  Node 0 is the root, the last token sampled before.  From the root
+    the path goes on to the first child whose token is the current node's target.  Returns ``path [B,
+    max_seqlen_q]`` (int32 node indices, -1 behind them), ``num_accepted [B]`` (int32, the root among them) and
+    ``next_tokens [B]`` (int64: the last accepted node's target).  Then, in every layer's K and V of ``kv_cache``
+    (as for ``copy_kv_blocks``), the row of node ``path[s, r]`` moves to the position of node r, so that the
+    sequence's cache is its tokens before the tree and the accepted ones.
+
+    A caller that accepts by another rule passes ``path`` and ``num_accepted`` in place of the three (indices that
+    rise), and gets them back with ``None``.
+    """
+    what = "commit_tree"
+    dev = _check_one_device(what, kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, parents, tokens, target_tokens,
+                            path, num_accepted)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, parents, tokens,
+                               target_tokens, path, num_accepted)
+    slabs, nb, bs, row = _pool(what, kv_cache)
+    n, mq = cu_seqlens_q.numel() - 1, int(max_seqlen_q)
+    _check_cu(what, n + 1, cu_seqlens_q, cu_seqlens_k)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise RuntimeError(f"{what}: block_table must be int32 [sequences, width] with contiguous rows")
+    next_tokens = None
+    if path is None:
+        if parents is None or tokens is None or target_tokens is None or num_accepted is not None:
+            raise RuntimeError(f"{what}: give parents, tokens and target_tokens, or path and num_accepted")
+        total = tokens.numel()
+        for t, dtype in ((parents, torch.int32), (tokens, torch.int64), (target_tokens, torch.int64)):
+            if t.dtype != dtype or t.dim() != 1 or t.shape[0] != total or not t.is_contiguous():
+                raise RuntimeError(f"{what}: parents (int32), tokens and target_tokens (int64) must be contiguous [T]")
+        path = torch.empty(n, mq, dtype=torch.int32, device=kv_cache.device)
+        num_accepted = torch.empty(n, dtype=torch.int32, device=kv_cache.device)
+        next_tokens = torch.empty(n, dtype=torch.int64, device=kv_cache.device)
+    else:
+        if num_accepted is None or parents is not None or tokens is not None or target_tokens is not None:
+            raise RuntimeError(f"{what}: give parents, tokens and target_tokens, or path and num_accepted")
+        if path.dtype != torch.int32 or path.shape != (n, mq) or not path.is_contiguous() or \
+                num_accepted.dtype != torch.int32 or num_accepted.shape != (n,) or not num_accepted.is_contiguous():
+            raise RuntimeError(f"{what}: path [B, max_seqlen_q] and num_accepted [B] must be contiguous int32")
+        total = 0x7fffffff    # no rows of nodes are read
+    rc = lib().nq_commit_tree(kv_cache.data_ptr(), slabs, nb, bs, row, block_table.data_ptr(), block_table.stride(0),
+                              block_table.shape[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), n, total, mq,
+                              ptr(parents), ptr(tokens), ptr(target_tokens), path.data_ptr(), num_accepted.data_ptr(),
+                              ptr(next_tokens), raw_stream(dev))
+    check(rc, what)
+    return path, num_accepted, next_tokens
+
+
 __all__ = ["store_kvcache", "paged_decode", "varlen_prefill", "prepare_decode", "decode_plan", "qk_norm_rope_store",
-           "output_gate", "gdn_decode", "gdn_prefill", "gated_rmsnorm", "gdn_conv1d",
-           "decode_workspace", "prefill_workspace", "release_workspaces", "decode_schedule", "_lib"]
+           "output_gate", "gdn_decode", "gdn_prefill", "gated_rmsnorm", "gdn_conv1d", "tree_attention",
+           "window_prefill", "window_decode", "copy_kv_blocks", "commit_tree", "decode_workspace",
+           "prefill_workspace", "release_workspaces", "decode_schedule", "_lib"]
