@@ -28,8 +28,8 @@
 //
 // NaN and infinities in keys or values that a row does not see do not reach
 // it: masked scores are replaced before use, and a masked tile whose values
-// are not all finite takes them out of the product and adds them back to the
-// rows that see them (fix_values).
+// are not all finite takes them out of the product and gives them back to the
+// rows that see them (odd_values, poison, clean).
 #include <algorithm>
 
 #include "nq_device.hpp"
@@ -104,7 +104,7 @@ struct Shape {
   static constexpr int RING_B = SLOTS * SLOT_B;
   static constexpr int MASK_WORDS = kMaxNodes / 32 + 1;  // LDS row of a token's mask (odd: no bank pattern)
   static constexpr int TOKENS = M + 1;                   // of a row tile, at most
-  static constexpr int LDS_B = RING_B + TOKENS * MASK_WORDS * 4;
+  static constexpr int LDS_B = RING_B + TOKENS * MASK_WORDS * 4 + 16 * 4;  // ring, masks, flags of odd tiles
   static constexpr int NKK = D / 32, NJ = D / 16;
   static_assert(COPS >= 1, "every wave copies");
 };
@@ -437,8 +437,8 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
     if (hi > lo || (tl.n == 0 && first_here)) {
       const int n = hi - lo;
       const bool whole = lo == 0 && hi == tl.n;
-      // this wave's rows and their tokens (a wave past the last row works on
-      // copies of it and stores nothing)
+      // this wave's rows and their tokens (a wave past the last row has nothing
+      // to do but its copies)
       const int r0 = r_first + rw * QS * 16;
       const bool wave_live = r0 <= r_last;
       const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
@@ -492,7 +492,7 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
 
       // Keys of the tile at `key0` that row block qs of this lane sees: bit
       // 4 ks + r for key 16 ks + 4 g + r.
-      auto seen = [&](int qs, int key0, bool ok) -> uint32_t {
+      auto seen = [&](int qs, int key0) -> uint32_t {
         uint32_t v = 0;
         if (a.window > 0) {
           const int top = P + tok[qs], bot = top - a.window;
@@ -516,7 +516,7 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           if (left < 32) bits &= (1u << left) - 1u;
           v = ((bits >> (4 * g)) & 15u) | (((bits >> (16 + 4 * g)) & 15u) << 4);
         }
-        return ok ? v : 0u;
+        return v;
       };
 
       // Scores -> P of the tile (units packed for the second product), with
@@ -582,79 +582,107 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(vf, pb[qs], o[qs][j]);
         }
       };
-      // The same for a tile that not every row sees whole: 0 * NaN must not
-      // reach a row through a key it does not see.  Values that are not finite
-      // are taken out of the product; a product of their indicators with the
-      // visible keys' then tells which rows see one.
-      auto fix_values = [&](uint32_t kt) {
-        constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
-        constexpr uint32_t kMant = T::dtype == NQ_BF16 ? 0x007fu : 0x03ffu;
-        constexpr uint32_t kOne = T::kOne2 & 0xffffu;
-        u32x4 ones[QS];
-#pragma unroll
-        for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            ones[qs][t] = (((vis[qs] >> (2 * t)) & 1u) ? kOne : 0u) | (((vis[qs] >> (2 * t + 1)) & 1u) ? kOne << 16 : 0u);
+      // A tile that not every row sees whole: 0 * NaN must not reach a row
+      // through a key it does not see.  When such a tile holds values that are
+      // not finite (`odd_values`), `poison` adds them to the outputs of the rows
+      // that see them and `clean` takes them out of the tile.  The waves that
+      // share the tile check and clean a part of it each.
+      constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
+      constexpr uint32_t kMant = T::dtype == NQ_BF16 ? 0x007fu : 0x03ffu;
+      // top bit of every half (fp8: byte) of w that is not finite: its exponent
+      // (and, of e4m3, its mantissa) is all ones, and the carry reaches that bit
+      auto odd_bits = [](uint32_t w) -> uint32_t {
+        if constexpr (FP8) return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        constexpr uint32_t e = kExp | kExp << 16, lsb = (kMant + 1) | (kMant + 1) << 16;
+        return ((w & e) + lsb) & 0x80008000u;
+      };
+      constexpr int kPart = TILE_B / RW / 64;  // bytes of the tile's values per lane
+      auto part_of = [&](uint32_t kt, int c) { return kt + TILE_B + (rw * (kPart / 16) + c) * 1024 + lane * 16; };
+      uint32_t *const lds_odd = lds_mask + S::TOKENS * S::MASK_WORDS;
+      auto odd_values = [&](uint32_t kt) -> bool {
+        uint32_t any = 0;
+#pragma unroll 2
+        for (int c = 0; c < kPart / 16; ++c) {
+          const u32x4 x = lds_load_b128<0>(part_of(kt, c));
+          any |= odd_bits(x[0]) | odd_bits(x[1]) | odd_bits(x[2]) | odd_bits(x[3]);
+        }
+        bool odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+        if constexpr (RW > 1) {
+          if (lane == 0) lds_odd[rw] = odd;
+          wait_lgkmcnt0();
+          raw_barrier();
+          odd = __builtin_amdgcn_ballot_w64(lane < RW && lds_odd[lane & (RW - 1)] != 0) != 0;
+        }
+        return odd;
+      };
+      auto clean = [&](uint32_t kt) {
+        wait_lgkmcnt0();
+        if constexpr (RW > 1) raw_barrier();  // every wave has looked at the tile
 #pragma unroll 1
-        for (int j = 0; j < NJ; ++j) {
-          u32x4 vf = v_op(kt, j);
-          u32x4 nan{0, 0, 0, 0}, up{0, 0, 0, 0}, down{0, 0, 0, 0};
-          uint32_t any = 0;
+        for (int c = 0; c < kPart / 16; ++c) {
+          u32x4 x = lds_load_b128<0>(part_of(kt, c));
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t b = odd_bits(x[t]);
+            x[t] &= ~((b - (b >> (FP8 ? 7 : 15))) | b);
+          }
+          lds_store_b128(part_of(kt, c), x);
+        }
+        wait_lgkmcnt0();
+        if constexpr (RW > 1) raw_barrier();
+      };
+      // This lane's outputs (dims 16 j + 4 g + r of its rows) from every value
+      // that is not finite and whose key the row sees.  Rare: written for size.
+      auto poison = [&](uint32_t kt) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t x = (vf[t] >> (16 * half)) & 0xffffu;
-              if ((x & kExp) == kExp) {
-                any = 1;
-                vf[t] &= half ? 0x0000ffffu : 0xffff0000u;
-                const uint32_t one = kOne << (16 * half);
-                if (x & kMant) nan[t] |= one;
-                else if (x & 0x8000u) down[t] |= one;
-                else up[t] |= one;
-              }
-            }
-          const bool odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+        for (int qs = 0; qs < QS; ++qs) {
+          uint64_t nan = 0, up = 0, down = 0;  // bit 4 j + r
+#pragma unroll 1
+          for (int key = 0; key < kKeys; ++key) {
+            const uint32_t theirs = __shfl(vis[qs], ((key >> 2) & 3) * 16 + m);  // of the lane that holds the key
+            if (!((theirs >> (4 * (key >> 4) + (key & 3))) & 1u)) continue;
+#pragma unroll 1
+            for (int j = 0; j < NJ; ++j) {
+              if constexpr (FP8) {
+                const uint32_t at = kt + TILE_B + key * D + ((j ^ swz8<D>(key)) << 4) + 4 * g;
+                const uint32_t x = *reinterpret_cast<const __attribute__((address_space(3))) uint32_t *>(
+                    static_cast<uintptr_t>(at));
 #pragma unroll
-          for (int jj = 0; jj < NJ; ++jj)  // a constant index: o stays in registers
-            if (jj == j) {
+                for (int r = 0; r < 4; ++r)
+                  nan |= static_cast<uint64_t>(((x >> (8 * r)) & 0x7fu) == 0x7fu) << (4 * j + r);
+              } else {
+                const u32x2 x = lds_load_b64<0>(kt + TILE_B + key * 2 * D + (((2 * j + (g >> 1)) ^ swz_v(key)) << 4) +
+                                                (g & 1) * 8);
 #pragma unroll
-              for (int qs = 0; qs < QS; ++qs) {
-                o[qs][jj] = T::mfma16x16x32(vf, pb[qs], o[qs][jj]);
-                if (odd) {
-                  const f32x4 zero{0, 0, 0, 0};
-                  const f32x4 cn = T::mfma16x16x32(nan, ones[qs], zero), cu = T::mfma16x16x32(up, ones[qs], zero),
-                              cd = T::mfma16x16x32(down, ones[qs], zero);
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    if (cu[r] > 0.f) o[qs][jj][r] += __builtin_huge_valf();
-                    if (cd[r] > 0.f) o[qs][jj][r] -= __builtin_huge_valf();
-                    if (cn[r] > 0.f) o[qs][jj][r] = __builtin_nanf("");
-                  }
+                for (int r = 0; r < 4; ++r) {
+                  const uint32_t e = (x[r >> 1] >> (16 * (r & 1))) & 0xffffu;
+                  const uint64_t odd = (e & kExp) == kExp, is_nan = odd && (e & kMant) != 0;
+                  nan |= is_nan << (4 * j + r);
+                  up |= static_cast<uint64_t>(odd && !is_nan && !(e & 0x8000u)) << (4 * j + r);
+                  down |= static_cast<uint64_t>(odd && !is_nan && (e & 0x8000u)) << (4 * j + r);
                 }
               }
             }
+          }
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              // added as bits (a bit's sign extension and the value's): no select per output
+              const int bit = (4 * j + r) & 31;
+              auto term = [&](uint64_t set, uint32_t value) {
+                const uint32_t half = static_cast<uint32_t>(4 * j + r < 32 ? set : set >> 32);
+                return u2f(static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(half), bit, 1)) & value);
+              };
+              o[qs][j][r] += term(nan, 0x7fc00000u);
+              if constexpr (!FP8) o[qs][j][r] = (o[qs][j][r] + term(up, 0x7f800000u)) + term(down, 0xff800000u);
+            }
         }
       };
-      // Whether the tile's values are all finite (the wave's operands of them
-      // cover the whole tile).
-      auto finite = [&](uint32_t kt) -> bool {
-        constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
-        uint32_t any = 0;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const u32x4 vf = v_op(kt, j);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            any |= ((vf[t] & kExp) == kExp || (vf[t] & (kExp << 16)) == kExp << 16) ? 1u : 0u;
-        }
-        return __builtin_amdgcn_ballot_w64(any != 0) == 0;
-      };
-      // What the wave does with the tile at list position i: 0 nothing, 1 every
-      // key is seen by every row, 2 masked.
-      auto kind_of = [&](int i, int key0) -> int {
-        if (!wave_live) return 0;
+      // What the tokens ta .. tb make of the tile at list position i: 0 nothing (no
+      // key of it is seen, or its page is missing), 1 every row sees every key,
+      // 2 masked.
+      auto kind_of = [&](int i, int key0, int ta, int tb) -> int {
         if ((bad >> (i & 63)) & 1) return 0;
         if (a.window == 0) return key0 + kKeys <= P ? 1 : 2;
         const int pa = P + ta, pz = P + tb;
@@ -667,19 +695,20 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         if constexpr (RW == 1) {
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // K of this tile (younger: its V and the tiles after it)
           asm volatile("" ::: "memory");
-          const int kind = kind_of(i, key0);
+          const int kind = kind_of(i, key0, ta, tb);
           if (kind != 0) scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
           next_tile(src, nrec);
           copy_k(slot, src, nrec);
-          if (kind == 2) vis[0] = seen(0, key0, true);
+          if (kind == 2) vis[0] = seen(0, key0);
           if (kind != 0) softmax(kind == 2);
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
           asm volatile("" ::: "memory");
-          if (kind == 2 && !finite(slot))
-            fix_values(slot);
-          else if (kind != 0)
-            values(slot);
+          if (kind == 2 && __builtin_expect(odd_values(slot), 0)) {
+            poison(slot);
+            clean(slot);
+          }
+          if (kind != 0) values(slot);
           wait_lgkmcnt0();
           copy_v(slot, src, nrec);
         } else {
@@ -690,19 +719,25 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           copy_k(st_dst, src, nrec);
           copy_v(st_dst, src, nrec);
           st_dst = st_dst == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : st_dst + SLOT_B;
-          const int kind = kind_of(i, key0);
+          const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
           if (kind != 0) {
             scores(slot);
             if (kind == 2) {
 #pragma unroll
-              for (int qs = 0; qs < QS; ++qs) vis[qs] = seen(qs, key0, true);
+              for (int qs = 0; qs < QS; ++qs) vis[qs] = seen(qs, key0);
             }
             softmax(kind == 2);
-            if (kind == 2 && !finite(slot))
-              fix_values(slot);
-            else
-              values(slot);
           }
+          // (for all of the workgroup's waves alike)
+          if (kind_of(i, key0, t_first, t_last) == 2 && __builtin_expect(odd_values(slot), 0)) {
+            if (kind == 1) {
+#pragma unroll
+              for (int qs = 0; qs < QS; ++qs) vis[qs] = 0xffu;
+            }
+            if (kind != 0) poison(slot);
+            clean(slot);
+          }
+          if (kind != 0) values(slot);
         }
         slot = slot == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : slot + SLOT_B;
       }

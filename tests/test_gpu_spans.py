@@ -104,3 +104,50 @@ def test_tree_arbitrary_masks(cuda):
     out = c.to(cuda).tree_attention(mask)
     check(out, *tree_reference(c, mask), BF)
     assert (out[3] == 0).all() and (out[-1] == 0).all()
+
+
+def _odd(case, g, share=0.02):
+    """NaN and infinities in some of the cached values and keys; fp8 has NaN only."""
+    nb, bs = case.k.shape[:2]
+    for cache, vals, share in ((case.k, [float("nan")], share / 6), (case.v, [float("nan"), float("inf"), float("-inf")], share)):
+        raw = cache.view(torch.uint8) if case.fp8 else cache
+        for i, h in enumerate(case.have):
+            for j in range(h):
+                if torch.rand((), generator=g) < share:
+                    at = raw[case.table[i, j // bs].long(), j % bs, int(torch.randint(0, case.hkv, (), generator=g))]
+                    dims = torch.randint(0, case.d, (3,), generator=g)
+                    x = vals[int(torch.randint(0, len(vals), (), generator=g))]
+                    at[dims] = 0x7F if case.fp8 else x
+    return case
+
+
+def _check_odd(out, visible_rows, case, dtype):
+    """Rows that see nothing odd are as close as ever, and every output is finite or not as the oracle's."""
+    ref, mag = visible_rows
+    o = out.double().cpu()
+    fine = torch.isfinite(ref)
+    assert fine.any() and not fine.all()
+    assert torch.equal(fine, torch.isfinite(o))
+    assert torch.equal(torch.isnan(ref), torch.isnan(o))
+    assert torch.equal(ref[~fine & ~torch.isnan(ref)], o[~fine & ~torch.isnan(ref)])
+    ok = fine & torch.isfinite(mag)
+    check(torch.where(ok, o, 0.0), torch.where(ok, ref, 0.0), torch.where(ok, mag, 0.0), dtype)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype,fp8", [(8, 2, 128, BF, False), (2, 2, 128, HF, False), (4, 2, 256, HF, False),
+                                                (8, 1, 256, BF, False), (8, 2, 128, BF, True), (4, 1, 256, HF, True)])
+def test_masked_nan_and_infinity(cuda, hq, hkv, d, dtype, fp8):
+    """Odd values reach the rows that see them, and no others: in windows (prefill and decode) and trees."""
+    for seed, new, pre, window, sinks in ((1, [50, 30], [60, 200], 24, 3), (2, [1, 1, 1, 1, 1, 1], [30, 80, 130, 200, 9, 64], 20, 2),
+                                          (3, [150], [0], 12, 1)):
+        c = Case(new, pre, hq, hkv, d, dtype, block=32, fp8=fp8, seed=seed)
+        _odd(c, torch.Generator().manual_seed(seed), 0.01).to(cuda)
+        ref = c.window_reference(window, sinks)
+        _check_odd(c.window_prefill(window, sinks), ref, c, dtype)
+        if max(new) == 1:
+            _check_odd(c.window_decode(window, sinks), ref, c, dtype)
+    for seed, new in ((4, [2, 3, 1, 2] * 4), (5, [60, 40]), (6, [8, 7, 6])):
+        trees, mask = tree_masks(new, seed)
+        c = Case(new, [0] * len(new), hq, hkv, d, dtype, block=32, fp8=fp8, seed=seed)
+        _odd(c, torch.Generator().manual_seed(seed), 0.06).to(cuda)
+        _check_odd(c.tree_attention(mask), tree_reference(c, mask), c, dtype)
