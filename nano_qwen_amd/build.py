@@ -43,7 +43,7 @@ def _flags():
     ]
 
 
-# Per-source extra flags.  The prefill kernels keep their MFMA accumulators
+# Per-source extra flags.  The prefill kernels (windowed ones too) keep their MFMA accumulators
 # in VGPR form: with the default heuristics the 64-row kernel spends about
 # 175 AGPR<->VGPR moves per key tile.  Their work-queue atomics stay plain
 # atomics: the atomic optimizer rewrites one into a wave-wide add whose
@@ -51,6 +51,7 @@ def _flags():
 # flight right after it instead of where the fetched index is used.
 EXTRA_FLAGS = {
     "varlen_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"],
+    "span_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -31,6 +31,7 @@
 // are not all finite takes them out of the product and gives them back to the
 // rows that see them (odd_values, poison, clean).
 #include <algorithm>
+#include <type_traits>
 
 #include "nq_device.hpp"
 
@@ -394,25 +395,36 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
     return u32x4{T::template fp8x2<false>(c[0]), T::template fp8x2<true>(c[0]), T::template fp8x2<false>(c[1]),
                  T::template fp8x2<true>(c[1])};
   };
-  auto k_op = [&](uint32_t kt, int kk, int ks) -> u32x4 {
+  // as read from LDS: 16-bit values, or fp8 codes that `op` widens
+  using KV = std::conditional_t<FP8, u32x2, u32x4>;
+  auto op = [&](const KV &x) -> u32x4 {
+    if constexpr (FP8)
+      return widen8(x);
+    else
+      return x;
+  };
+  auto k_read = [&](uint32_t kt, int kk, int ks) -> KV {
     if constexpr (FP8) {
       constexpr int KF = D == 128 ? 2 : 4;  // swz8: rows m + 16 flip this bit of kk
       const uint32_t at = (((ks ? kk ^ KF : kk) << 5) ^ kx_l) + (kt + kbase_l);
-      return widen8(ks ? lds_load_b64<16 * D>(at) : lds_load_b64<0>(at));
+      return ks ? lds_load_b64<16 * D>(at) : lds_load_b64<0>(at);
     } else {
       const uint32_t at = ((kk << 6) ^ kx_l) + (kt + kbase_l);
       return ks ? lds_load_b128<16 * 2 * D>(at) : lds_load_b128<0>(at);
     }
   };
-  auto v_op = [&](uint32_t kt, int j) -> u32x4 {
+  auto v_read = [&](uint32_t kt, int j) -> KV {
     if constexpr (FP8) {
-      return widen8(lds_load_tr8(((j << 4) ^ vx_l) + (kt + TILE_B + vbase_l)));
+      return lds_load_tr8(((j << 4) ^ vx_l) + (kt + TILE_B + vbase_l));
     } else {
       const uint32_t at = ((j << 5) ^ vx_l) + (kt + TILE_B + vbase_l);
       const u32x2 lo = lds_load_tr16<0>(at), hi = lds_load_tr16<16 * 2 * D>(at);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
   };
+  // keeps the compiler from turning an operand's offset into one loop-invariant
+  // register per operand
+  auto unhoist = [&]() { asm volatile("" : "+v"(kx_l), "+v"(vx_l)); };
 
   const float sl2 = a.scale_log2 * (FP8 ? ld_const(a.k_scale + h) : 1.f);
   const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
@@ -437,8 +449,8 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
     if (hi > lo || (tl.n == 0 && first_here)) {
       const int n = hi - lo;
       const bool whole = lo == 0 && hi == tl.n;
-      // this wave's rows and their tokens (a wave past the last row has nothing
-      // to do but its copies)
+      // this wave's rows and their tokens (a wave past the last row sees no key
+      // and stores nothing)
       const int r0 = r_first + rw * QS * 16;
       const bool wave_live = r0 <= r_last;
       const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
@@ -480,6 +492,12 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         else
           __syncthreads();
       }
+      // The compiler waits for Q here, once (it counts the loads that it knows,
+      // and waits for the copies in flight with them), not in the loop.
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
       float m_use[QS], lsum[QS];
       f32x4 o[QS][NJ];
 #pragma unroll
@@ -519,12 +537,14 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         return v;
       };
 
-      // Scores -> P of the tile (units packed for the second product), with
-      // the rows' maxima and sums; returns nothing else.
-      f32x4 sc[QS][2];
-      u32x4 pb[QS];
+      f32x4 sc[QS][2];  // scores of the tile whose P is formed next
+      u32x4 pb[QS];     // P, in the second product's operand form
       uint32_t vis[QS];
-      auto softmax = [&](bool masked) {
+      // The rows' maxima over the tile's scores (masked where `vis` says so)
+      // against the running ones.  A maximum moves when some score exceeds it by
+      // more than kRescale; then every row's is brought up to date, alpha holds
+      // the factors for o, and the result is true.
+      auto check = [&](bool masked, float (&alpha)[QS]) -> bool {
         float mloc[QS];
         bool grow = false;
 #pragma unroll
@@ -539,28 +559,29 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
                               vmax_raw(sc[qs][1][2], sc[qs][1][3])) * sl2;
           grow |= mloc[qs] > m_use[qs] + kRescale;
         }
-        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-#pragma unroll
-          for (int qs = 0; qs < QS; ++qs) {
-            const float mn = fmaxf(m_use[qs], max32_raw(max16_raw(mloc[qs])));
-            const float alpha = m_use[qs] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m_use[qs] - mn);
-            lsum[qs] *= alpha;
-            m_use[qs] = mn;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) o[qs][j] *= alpha;
-          }
-        }
+        if (__builtin_amdgcn_ballot_w64(grow) == 0) return false;
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) {
-          const float ref = m_use[qs] == kNegInf ? 0.f : m_use[qs];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -ref));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -ref));
-            lsum[qs] += e0 + e1;
-            pb[qs][t] = T::pack2(e0, e1);
-          }
+          const float mn = fmaxf(m_use[qs], max32_raw(max16_raw(mloc[qs])));
+          alpha[qs] = m_use[qs] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m_use[qs] - mn);
+          lsum[qs] *= alpha[qs];
+          m_use[qs] = mn;
         }
+        return true;
+      };
+      auto rescale = [&](const float (&alpha)[QS]) {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) o[qs][j] *= alpha[qs];
+      };
+      // Elements 2 t, 2 t + 1 of a row block: P, its sum, packed.
+      auto p_unit = [&](int qs, int t) -> uint32_t {
+        const float ref = m_use[qs] == kNegInf ? 0.f : m_use[qs];
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -ref));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -ref));
+        lsum[qs] += e0 + e1;
+        return T::pack2(e0, e1);
       };
       auto scores = [&](uint32_t kt) {
 #pragma unroll
@@ -569,18 +590,10 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) {
-            const u32x4 kf = k_op(kt, kk, ks);
+            const u32x4 kf = op(k_read(kt, kk, ks));
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) sc[qs][ks] = T::mfma16x16x32(kf, qf[qs][kk], sc[qs][ks]);
           }
-      };
-      auto values = [&](uint32_t kt) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const u32x4 vf = v_op(kt, j);
-#pragma unroll
-          for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(vf, pb[qs], o[qs][j]);
-        }
       };
       // A tile that not every row sees whole: 0 * NaN must not reach a row
       // through a key it does not see.  When such a tile holds values that are
@@ -690,9 +703,11 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         return key0 + kKeys - 1 <= pa && (key0 > pz - a.window || key0 + kKeys <= a.sinks) ? 1 : 2;
       };
 
-      for (int i = lo; i < hi; ++i) {
-        const int key0 = (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys;
-        if constexpr (RW == 1) {
+      auto key_of = [&](int i) { return (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys; };
+      float alpha[QS];
+      if constexpr (RW == 1) {
+        for (int i = lo; i < hi; ++i) {
+          const int key0 = key_of(i);
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // K of this tile (younger: its V and the tiles after it)
           asm volatile("" ::: "memory");
           const int kind = kind_of(i, key0, ta, tb);
@@ -701,45 +716,164 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           next_tile(src, nrec);
           copy_k(slot, src, nrec);
           if (kind == 2) vis[0] = seen(0, key0);
-          if (kind != 0) softmax(kind == 2);
+          if (kind != 0) {
+            if (check(kind == 2, alpha)) rescale(alpha);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) pb[0][t] = p_unit(0, t);
+          }
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
           asm volatile("" ::: "memory");
           if (kind == 2 && __builtin_expect(odd_values(slot), 0)) {
             poison(slot);
             clean(slot);
           }
-          if (kind != 0) values(slot);
+          if (kind != 0) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[0][j] = T::mfma16x16x32(op(v_read(slot, j)), pb[0], o[0][j]);
+          }
           wait_lgkmcnt0();
           copy_v(slot, src, nrec);
-        } else {
-          wait_vmcnt<2 * COPS * (kAhead - 1)>();  // this wave's part of the tile
-          wait_lgkmcnt0();                        // and its reads of the tile before
-          raw_barrier();
+          slot = slot == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : slot + SLOT_B;
+        }
+      } else if (n > 0) {
+        // One tile per step, three tiles at work: P of tile i is formed among the
+        // products of P V of tile i - 1, and the V operands of tile i are read
+        // among the products of K Q of tile i + 1, so that the matrix core, the
+        // exponentials and the LDS reads overlap within a wave.
+        constexpr int NP = NJ * QS, U = 4 * QS, PPU = NP / U;  // products of P V, units of P, products per unit
+        constexpr int CV = FP8 ? 4 * NJ / U : 0;               // conversions per unit
+        constexpr int NQ = NKK * 2 * QS, PPV = NQ / NJ;        // products of K Q, of them per V operand
+        static_assert(PPU == 2 || PPU == 4, "2 or 4 products per unit of P");
+        static_assert(PPV == 1 || PPV == 2, "one V operand per one or two products");
+        KV vf[NJ];  // V operands of the tile whose products are pending
+        bool pend = false;
+        auto next_slot = [&](uint32_t x) { return x == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : x + SLOT_B; };
+        auto step = [&](auto first_tag, int i) {
+          constexpr bool FIRST = decltype(first_tag)::value;
+          const int key0 = key_of(i);
+          const bool mixed = kind_of(i, key0, t_first, t_last) == 2;  // for all of the workgroup's waves alike
+          unhoist();
+          if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
+          const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
+          if (kind != 1) {
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) vis[qs] = kind == 2 ? seen(qs, key0) : 0u;
+          }
+          pend = check(kind != 1, alpha);
           next_tile(src, nrec);
           copy_k(st_dst, src, nrec);
           copy_v(st_dst, src, nrec);
-          st_dst = st_dst == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : st_dst + SLOT_B;
-          const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
-          if (kind != 0) {
-            scores(slot);
-            if (kind == 2) {
+          st_dst = next_slot(st_dst);
+          KV kf[NKK][2];
+          {
+            const uint32_t slot_next = next_slot(slot);
 #pragma unroll
-              for (int qs = 0; qs < QS; ++qs) vis[qs] = seen(qs, key0);
+            for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) kf[kk][ks] = k_read(slot_next, kk, ks);
+            uint32_t pw[QS][4];
+            if constexpr (FIRST) {
+#pragma unroll
+              for (int u = 0; u < U; ++u) pw[u / 4][u % 4] = p_unit(u / 4, u % 4);
+            } else {
+              u32x4 vw[NJ];
+              constexpr int JPU = NJ / U > 0 ? NJ / U : 1;  // V operands per unit (rounded up)
+#pragma unroll
+              for (int j = 0; j < JPU; ++j) vw[j] = op(vf[j]);
+#pragma unroll
+              for (int x = 0; x < NP; ++x) {
+                const int j = x / QS, qs = x % QS, u = x / PPU;
+                if (FP8 && x % PPU == 0) {
+#pragma unroll
+                  for (int jn = (u + 1) * NJ / U; jn < (u + 2) * NJ / U && jn < NJ; ++jn)
+                    if (jn >= JPU) vw[jn] = op(vf[jn]);
+                }
+                o[qs][j] = T::mfma16x16x32(FP8 ? vw[j] : op(vf[j]), pb[qs], o[qs][j]);
+                if (x % PPU == PPU - 1) pw[u / 4][u % 4] = p_unit(u / 4, u % 4);
+              }
+              if (FP8) __builtin_amdgcn_sched_group_barrier(0x002, CV, 0);  // VALU: the first operands
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x002, 2 + CV / 2, 0);       // VALU
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);                // transcendental
+                if (PPU == 4) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x002, 3 + CV - CV / 2, 0);  // VALU
+                if (PPU == 4) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+                // DS read (K): halfway; fp8 codes (half the registers) after the first unit
+                if (u == (FP8 ? 0 : U / 2 - 1)) __builtin_amdgcn_sched_group_barrier(0x100, 2 * NKK, 0);
+              }
             }
-            softmax(kind == 2);
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) pb[qs] = u32x4{pw[qs][0], pw[qs][1], pw[qs][2], pw[qs][3]};
           }
-          // (for all of the workgroup's waves alike)
-          if (kind_of(i, key0, t_first, t_last) == 2 && __builtin_expect(odd_values(slot), 0)) {
-            if (kind == 1) {
+          __builtin_amdgcn_sched_barrier(0);  // the two sections are scheduled apart
+          if (mixed && __builtin_expect(odd_values(slot), 0)) {
+            if (kind != 0) {
+              if (kind == 1) {
 #pragma unroll
-              for (int qs = 0; qs < QS; ++qs) vis[qs] = 0xffu;
+                for (int qs = 0; qs < QS; ++qs) vis[qs] = 0xffu;
+              }
+              if (pend) rescale(alpha);  // o holds the tiles before: brought up to date first
+              pend = false;
+              poison(slot);
             }
-            if (kind != 0) poison(slot);
             clean(slot);
           }
-          if (kind != 0) values(slot);
+          {
+            f32x4 sn[QS][2];
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) sn[qs][0] = sn[qs][1] = f32x4{0, 0, 0, 0};
+            u32x4 kw[NKK][2];  // fp8: each K operand widened while the one before it is at work
+            if constexpr (FP8) kw[0][0] = op(kf[0][0]);
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) {
+              const int kk = x / (2 * QS), ks = (x / QS) % 2, qs = x % QS;
+              if (FP8 && qs == 0 && 2 * kk + ks + 1 < 2 * NKK) {
+                const int nx = 2 * kk + ks + 1;
+                kw[nx >> 1][nx & 1] = op(kf[nx >> 1][nx & 1]);
+              }
+              sn[qs][ks] = T::mfma16x16x32(FP8 ? kw[kk][ks] : op(kf[kk][ks]), qf[qs][kk], sn[qs][ks]);
+              if (x % PPV == 0) vf[x / PPV] = v_read(slot, x / PPV);
+            }
+            constexpr int CK = FP8 ? 4 / QS : 0;  // conversions per product
+            if (FP8) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // VALU: the first K operand
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // MFMA
+              __builtin_amdgcn_sched_group_barrier(0x100, 2 / PPV, 0);  // DS read
+              if (FP8) __builtin_amdgcn_sched_group_barrier(0x002, CK, 0);
+            }
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+              sc[qs][0] = sn[qs][0];
+              sc[qs][1] = sn[qs][1];
+            }
+          }
+          slot = next_slot(slot);
+        };
+        wait_vmcnt<2 * COPS * (kAhead - 1)>();  // this wave's part of the first tile
+        raw_barrier();
+        unhoist();
+        scores(slot);
+        // Tile i + 1 has landed, and tile i - 1's slot is free.
+        auto sync = [&]() {
+          wait_vmcnt<2 * COPS * (kAhead - 2)>();
+          wait_lgkmcnt0();
+          raw_barrier();
+        };
+        sync();
+        step(std::true_type{}, lo);
+        for (int i = lo + 1; i < hi; ++i) {
+          sync();
+          step(std::false_type{}, i);
         }
-        slot = slot == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : slot + SLOT_B;
+        if (pend) rescale(alpha);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(op(vf[j]), pb[qs], o[qs][j]);
       }
 
       // ---- epilogue: lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
@@ -916,7 +1050,7 @@ int launch_shape(const SpanArgs &a, int D, int64_t max_rows, void *ws, int64_t w
     if (max_rows <= 16)
       return launch<T, FP8, Shape<256, FP8, 1, 1, 2>>(a, max_rows, FP8 ? 4 : 2, ws, ws_bytes, need, s);
     if (max_rows <= 64)
-      return launch<T, FP8, Shape<256, FP8, 4, 1, FP8 ? 4 : 2>>(a, max_rows, 2, ws, ws_bytes, need, s);
+      return launch<T, FP8, Shape<256, FP8, 4, 1, 4>>(a, max_rows, FP8 ? 2 : 1, ws, ws_bytes, need, s);
     return launch<T, FP8, Shape<256, FP8, 8, 1, 4>>(a, max_rows, 1, ws, ws_bytes, need, s);
   }
   if (max_rows <= 16)
