@@ -499,10 +499,12 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
       float m_use[QS], lsum[QS];
+      float mref[QS];  // what P's exponents subtract: m_use, or 0 while a row has seen nothing
       f32x4 o[QS][NJ];
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
         m_use[qs] = kNegInf;
+        mref[qs] = 0.f;
         lsum[qs] = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[qs][j] = f32x4{0, 0, 0, 0};
@@ -566,6 +568,7 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           alpha[qs] = m_use[qs] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m_use[qs] - mn);
           lsum[qs] *= alpha[qs];
           m_use[qs] = mn;
+          mref[qs] = mn == kNegInf ? 0.f : mn;
         }
         return true;
       };
@@ -577,9 +580,8 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       };
       // Elements 2 t, 2 t + 1 of a row block: P, its sum, packed.
       auto p_unit = [&](int qs, int t) -> uint32_t {
-        const float ref = m_use[qs] == kNegInf ? 0.f : m_use[qs];
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -ref));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -ref));
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -mref[qs]));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -mref[qs]));
         lsum[qs] += e0 + e1;
         return T::pack2(e0, e1);
       };
@@ -704,6 +706,23 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       };
 
       auto key_of = [&](int i) { return (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys; };
+      // List positions [first, first + count) where kind_of is 1 for tokens ta .. tb
+      // while no page is missing (of a window; sinks that it does not reach are
+      // left to kind_of).
+      struct Plain {
+        int first;
+        unsigned count;
+      };
+      auto plain_of = [&](int ta, int tb) -> Plain {
+        int t0 = 0, t1;  // tiles
+        if (a.window > 0) {
+          t0 = max(tl.ts == tl.tlo ? 0 : tl.tlo, (max(P + tb - a.window, -kKeys) + kKeys) / kKeys);
+          t1 = max(0, P + ta + 1) / kKeys;
+        } else {
+          t1 = max(0, P) / kKeys;
+        }
+        return Plain{t0 - tl.tlo + tl.ts, static_cast<unsigned>(max(0, t1 - t0))};
+      };
       float alpha[QS];
       if constexpr (RW == 1) {
         for (int i = lo; i < hi; ++i) {
@@ -746,20 +765,42 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         static_assert(PPU == 2 || PPU == 4, "2 or 4 products per unit of P");
         static_assert(PPV == 1 || PPV == 2, "one V operand per one or two products");
         KV vf[NJ];  // V operands of the tile whose products are pending
+        const Plain plain_w = wave_live ? plain_of(ta, tb) : Plain{0, 0}, plain_wg = plain_of(t_first, t_last);
         bool pend = false;
         auto next_slot = [&](uint32_t x) { return x == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : x + SLOT_B; };
         auto step = [&](auto first_tag, int i) {
           constexpr bool FIRST = decltype(first_tag)::value;
-          const int key0 = key_of(i);
-          const bool mixed = kind_of(i, key0, t_first, t_last) == 2;  // for all of the workgroup's waves alike
           unhoist();
           if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
-          const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
-          if (kind != 1) {
+          const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && bad == 0;
+          if (!whole_tile) {
+            const int key0 = key_of(i);
+            const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
 #pragma unroll
-            for (int qs = 0; qs < QS; ++qs) vis[qs] = kind == 2 ? seen(qs, key0) : 0u;
+            for (int qs = 0; qs < QS; ++qs) vis[qs] = kind == 0 ? 0u : kind == 1 ? 0xffu : seen(qs, key0);
           }
-          pend = check(kind != 1, alpha);
+          pend = check(!whole_tile, alpha);
+          // (for all of the workgroup's waves alike)
+          if (!(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && bad == 0) &&
+              kind_of(i, key_of(i), t_first, t_last) == 2 && __builtin_expect(odd_values(slot), 0)) {
+            // o is brought up to date before the odd values join it
+            if constexpr (!FIRST) {
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(op(vf[j]), pb[qs], o[qs][j]);
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) vf[j] = KV{};
+            }
+            if (pend) rescale(alpha);
+            pend = false;
+            if (whole_tile) {
+#pragma unroll
+              for (int qs = 0; qs < QS; ++qs) vis[qs] = 0xffu;
+            }
+            poison(slot);
+            clean(slot);
+          }
           next_tile(src, nrec);
           copy_k(st_dst, src, nrec);
           copy_v(st_dst, src, nrec);
@@ -809,18 +850,6 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
             for (int qs = 0; qs < QS; ++qs) pb[qs] = u32x4{pw[qs][0], pw[qs][1], pw[qs][2], pw[qs][3]};
           }
           __builtin_amdgcn_sched_barrier(0);  // the two sections are scheduled apart
-          if (mixed && __builtin_expect(odd_values(slot), 0)) {
-            if (kind != 0) {
-              if (kind == 1) {
-#pragma unroll
-                for (int qs = 0; qs < QS; ++qs) vis[qs] = 0xffu;
-              }
-              if (pend) rescale(alpha);  // o holds the tiles before: brought up to date first
-              pend = false;
-              poison(slot);
-            }
-            clean(slot);
-          }
           {
             f32x4 sn[QS][2];
 #pragma unroll
