@@ -82,6 +82,7 @@ struct SpanArgs {
   // outputs of range w's slots 2 w and 2 w + 1 (fp32, normalised, as the lanes
   // hold them), their rows' log2-sum-exp, and what they are.
   int n_ranges;
+  int stride;  // whole items: from a workgroup's item to its next
   float *part_o;
   float *part_l;
   int4 *part_desc;  // (sequence, row tile, kind, 0)
@@ -105,16 +106,30 @@ struct Shape {
   static constexpr int RING_B = SLOTS * SLOT_B;
   static constexpr int MASK_WORDS = kMaxNodes / 32 + 1;  // LDS row of a token's mask (odd: no bank pattern)
   static constexpr int TOKENS = M + 1;                   // of a row tile, at most
-  static constexpr int LDS_B = RING_B + TOKENS * MASK_WORDS * 4 + 16 * 4;  // ring, masks, flags of odd tiles
+  static constexpr int SEQS = 256;  // sequences whose bounds are kept in LDS
+  // ring, masks, flags of odd tiles, sequences' bounds and positions
+  static constexpr int MASK_AT = RING_B, ODD_AT = MASK_AT + (TOKENS * MASK_WORDS * 4 + 15) / 16 * 16,
+                       SEQ_AT = ODD_AT + 128, POS_AT = SEQ_AT + SEQS * 16, LDS_B = POS_AT + SEQS * 4;
   static constexpr int NKK = D / 32, NJ = D / 16;
   static_assert(COPS >= 1, "every wave copies");
 };
+
+// The kernel's arguments, read from its argument segment where they are used:
+// held in registers, the many that only an item's start needs would crowd the
+// tile loop's out.  (The address is opaque, so that no read is moved.)
+typedef const __attribute__((address_space(4))) SpanArgs KernArgs;
+__device__ __forceinline__ KernArgs *kernel_args() {
+  KernArgs *p = (KernArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // ---------------------------------------------------------------- items
 struct Seq {
   int s, q0, Lq, k0, Lk;
 };
-__device__ __forceinline__ Seq seq_of(const SpanArgs &a, int s, bool uniform) {
+template <class A>
+__device__ __forceinline__ Seq seq_of(const A &a, int s, bool uniform) {
   Seq x{};
   x.s = s;
   if (!a.cu_q) {
@@ -142,11 +157,18 @@ __device__ __forceinline__ int small_div(int n, int d) {
     ++q;
   return q;
 }
+// Of scores as they leave the matrix core: instructions that the compiler knows,
+// so that it keeps the wait states between a product and its readers (inline
+// assembly has none).  A NaN among them is the result.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
 // The tiles of a row tile whose tokens are ta .. tb.
 struct Tiles {
   int ts, tlo, n;  // tiles 0 .. ts - 1, then tlo, tlo + 1, ...: n in all
 };
-__device__ __forceinline__ Tiles tiles_of(const SpanArgs &a, const Seq &q, int ta, int tb) {
+template <class A>
+__device__ __forceinline__ Tiles tiles_of(const A &a, const Seq &q, int ta, int tb) {
   Tiles t{0, 0, 0};
   if (a.window == 0) {
     t.n = (q.Lk + kKeys - 1) / kKeys;
@@ -169,12 +191,12 @@ struct Cost {
   static constexpr int kItem = S::RW == 1 ? 1 : 4;
   static constexpr int kMinRange = 2;
 };
-template <class S>
-__device__ __forceinline__ int row_tiles(const SpanArgs &a, const Seq &q) {
+template <class S, class A>
+__device__ __forceinline__ int row_tiles(const A &a, const Seq &q) {
   return (q.Lq * a.G + S::M - 1) / S::M;
 }
-template <class S>
-__device__ __forceinline__ int item_cost(const SpanArgs &a, const Seq &q) {
+template <class S, class A>
+__device__ __forceinline__ int item_cost(const A &a, const Seq &q) {
   if (q.Lq <= 0) return 0;
   int n;
   if (q.Lq * a.G <= S::M) {
@@ -189,15 +211,17 @@ __device__ __forceinline__ int item_cost(const SpanArgs &a, const Seq &q) {
 
 // ---------------------------------------------------------------- the kernel
 template <class T, bool FP8, class S>
-__device__ __forceinline__ void span_body(const SpanArgs &a) {
+__device__ __forceinline__ void span_body() {
   constexpr int D = S::D, RW = S::RW, QS = S::QS, M = S::M, SLOTS = S::SLOTS, COPS = S::COPS;
   constexpr int NKK = S::NKK, NJ = S::NJ, TILE_B = S::TILE_B, SLOT_B = S::SLOT_B, SRC_ROWB = S::SRC_ROWB;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63;
   const int rw = RW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const bool paged = a.block_tables != nullptr;
-  const bool ranges = a.n_ranges > 0;
+  KernArgs &a0 = *kernel_args();  // (of the prologue)
+  const bool paged = a0.block_tables != nullptr;
+  const int n_ranges = a0.n_ranges;
+  const bool ranges = n_ranges > 0;
 
   // kv head and range (or item) of this workgroup.  Workgroup L runs on XCD
   // L % 8: a kv head stays on one XCD (or, of fewer than 8, on 8 / Hkv, which
@@ -205,83 +229,138 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
   // the same keys share an L2.
   const int L = blockIdx.x;
   int h, w;
-  if (a.Hkv < 8 && 8 % a.Hkv == 0) {
-    const int per = 8 / a.Hkv, x = L & 7;
-    h = x % a.Hkv;
-    w = ranges ? (x / a.Hkv) * (a.n_ranges / per) + (L >> 3) : (L >> 3) * per + x / a.Hkv;
+  if (a0.Hkv < 8 && 8 % a0.Hkv == 0) {
+    const int per = 8 / a0.Hkv, x = L & 7;
+    h = x % a0.Hkv;
+    w = ranges ? (x / a0.Hkv) * (n_ranges / per) + (L >> 3) : (L >> 3) * per + x / a0.Hkv;
   } else {
-    h = L % a.Hkv;
-    w = L / a.Hkv;
+    h = L % a0.Hkv;
+    w = L / a0.Hkv;
   }
 
-  // Positions [pos0, pos1) of the batch's row tiles laid end to end, each as
-  // its cost (whole items: 1).
-  auto weight_of = [&](const Seq &q) -> int { return ranges ? item_cost<S>(a, q) : (q.Lq > 0 ? 1 : 0); };
-  int pos0 = w, pos1 = w + 1;
-  int w_of = 0;  // the range's partials
-  if (ranges) {
-    int total = 0;
-    for (int b = 0; b < a.num_seqs; b += 64) {
-      int c = 0;
-      if (b + lane < a.num_seqs) {
-        const Seq q = seq_of(a, b + lane, false);
-        c = row_tiles<S>(a, q) * weight_of(q);
-      }
-      total += wave_sum_i32(c);
+  // The batch's row tiles laid end to end, each as its cost (whole items: 1).
+  // Of up to SEQS sequences the bounds and the positions of their ends are kept
+  // in LDS, so that finding an item is no chain of round trips to memory.
+  int4 *const lds_seq = reinterpret_cast<int4 *>(smem + S::SEQ_AT);
+  int *const lds_pos = reinterpret_cast<int *>(smem + S::POS_AT);
+  const bool listed = a0.num_seqs <= S::SEQS;
+  auto weight_of = [&](KernArgs &a, const Seq &q) -> int { return ranges ? item_cost<S>(a, q) : (q.Lq > 0 ? 1 : 0); };
+  int total = 0;
+  for (int b = 0; b < a0.num_seqs; b += 64) {
+    int c = 0;
+    Seq q{};
+    if (b + lane < a0.num_seqs) {
+      q = seq_of(a0, b + lane, false);
+      c = row_tiles<S>(a0, q) * weight_of(a0, q);
     }
-    w_of = h * a.n_ranges + w;
-    const int W = min(a.n_ranges, max(1, total / Cost<S>::kMinRange));
+    const int incl = total + wave_iscan(c);
+    if (listed && rw == 0 && b + lane < a0.num_seqs) {
+      lds_seq[b + lane] = int4{q.q0, q.Lq, q.k0, q.Lk};
+      lds_pos[b + lane] = incl;
+    }
+    total = __builtin_amdgcn_readlane(incl, 63);
+  }
+  if (listed) {
+    if constexpr (RW == 1)
+      wave_lds_sync();
+    else
+      __syncthreads();
+  }
+  int pos0 = w, pos1 = total;  // this workgroup's positions: all of them, or every stride-th
+  int w_of = 0;                // the range's partials
+  if (ranges) {
+    w_of = h * n_ranges + w;
+    const int W = min(n_ranges, max(1, total / Cost<S>::kMinRange));
     pos0 = w < W ? static_cast<int>(static_cast<int64_t>(w) * total / W) : 0;
     pos1 = w < W ? static_cast<int>(static_cast<int64_t>(w + 1) * total / W) : 0;
   }
   // The range's two partial pieces, written for the merge when it is done.
   int4 desc0{0, 0, kPieceNone, 0}, desc1{0, 0, kPieceNone, 0};
-  auto leave = [&]() {
-    if (ranges && rw == 0 && lane == 0) {
-      a.part_desc[2 * w_of] = desc0;
-      a.part_desc[2 * w_of + 1] = desc1;
-    }
+  // The first item at or after position `pos` that this workgroup has to do
+  // something for (live: there is one).
+  struct Item {
+    bool live, careful;
+    Seq q;
+    int rt, lo, hi, next;  // its row tile, its part of the tiles, the next position
+    int r_first, r_last, t_first, t_last;
+    Tiles tl;
   };
-  if (pos0 >= pos1) {
-    leave();
-    return;
-  }
-  // The row tile at pos0: sequence s, row tile rt, which starts at position X.
-  int s = a.num_seqs, rt = 0, X = 0;
-  {
-    int base = 0;
-    for (int b = 0; b < a.num_seqs; b += 64) {
-      int c = 0, wt = 1;
-      if (b + lane < a.num_seqs) {
-        const Seq q = seq_of(a, b + lane, false);
-        wt = weight_of(q);
-        c = row_tiles<S>(a, q) * wt;
+  auto describe = [&](int pos) -> Item {
+    KernArgs &a = *kernel_args();
+    Item it{};
+    while (pos < pos1) {
+      // sequence and row tile at pos; X: where it starts
+      int X = 0;
+      int start = 0, cost = 1;
+      bool found = false;
+      if (listed) {
+        for (int b = 0; b < a.num_seqs; b += 64) {
+          const int e = min(b + lane, a.num_seqs - 1);
+          const uint64_t hit = __builtin_amdgcn_ballot_w64(lds_pos[e] > pos);
+          if (hit != 0) {
+            const int s = b + static_cast<int>(__builtin_ctzll(hit));
+            const int4 x = lds_seq[s];
+            it.q.s = s;
+            it.q.q0 = __builtin_amdgcn_readfirstlane(x.x);
+            it.q.Lq = __builtin_amdgcn_readfirstlane(x.y);
+            it.q.k0 = __builtin_amdgcn_readfirstlane(x.z);
+            it.q.Lk = __builtin_amdgcn_readfirstlane(x.w);
+            start = s > 0 ? __builtin_amdgcn_readfirstlane(lds_pos[s - 1]) : 0;
+            cost = weight_of(a, it.q);
+            found = true;
+            break;
+          }
+        }
+      } else {
+        int base = 0;
+        for (int b = 0; b < a.num_seqs; b += 64) {
+          int c = 0;
+          if (b + lane < a.num_seqs) {
+            const Seq q = seq_of(a, b + lane, false);
+            c = row_tiles<S>(a, q) * weight_of(a, q);
+          }
+          const int incl = base + wave_iscan(c);
+          const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > pos);
+          if (hit != 0) {
+            const int l = static_cast<int>(__builtin_ctzll(hit));
+            it.q = seq_of(a, b + l, true);
+            start = __builtin_amdgcn_readlane(incl - c, l);
+            cost = weight_of(a, it.q);
+            found = true;
+            break;
+          }
+          base = __builtin_amdgcn_readlane(incl, 63);
+        }
       }
-      const int incl = base + wave_iscan(c);
-      const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > pos0);
-      if (hit != 0) {
-        const int l = static_cast<int>(__builtin_ctzll(hit));
-        s = b + l;
-        const int start = __builtin_amdgcn_readlane(incl - c, l);
-        const int cost = __builtin_amdgcn_readlane(wt, l);
-        rt = static_cast<int>(static_cast<unsigned>(pos0 - start) / static_cast<unsigned>(cost));
-        X = start + rt * cost;
-        break;
+      if (!found) return it;
+      it.rt = static_cast<int>(static_cast<unsigned>(pos - start) / static_cast<unsigned>(cost));
+      X = start + it.rt * cost;
+      it.r_first = it.rt * M;
+      it.r_last = min(it.r_first + M, it.q.Lq * a.G) - 1;
+      it.t_first = small_div(it.r_first, a.G);
+      it.t_last = small_div(it.r_last, a.G);
+      it.tl = tiles_of(a, it.q, it.t_first, it.t_last);
+      it.lo = 0;
+      it.hi = it.tl.n;
+      it.next = pos + a.stride;
+      if (ranges) {
+        it.lo = max(0, min(it.tl.n, pos0 - X - Cost<S>::kItem));
+        it.hi = max(0, min(it.tl.n, pos1 - X - Cost<S>::kItem));
+        it.next = X + cost;
       }
-      base = __builtin_amdgcn_readlane(incl, 63);
+      // an item without tiles is written (zeros) where it starts
+      it.live = it.hi > it.lo || (it.tl.n == 0 && (!ranges || X >= pos0));
+      if (it.live) return it;
+      pos = it.next;
     }
-  }
-  if (s >= a.num_seqs) {
-    leave();
-    return;
-  }
+    return it;
+  };
 
   // ---------------------------------------------------------------- copies
   const uint32_t lds0 = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)(smem)));
-  uint32_t *const lds_mask = reinterpret_cast<uint32_t *>(smem + S::RING_B);
-  const int kv_rs = static_cast<int>(a.kv_rs);
-  const int tiles_per_blk = paged ? a.block_size / kKeys : 0x40000000;
+  uint32_t *const lds_mask = reinterpret_cast<uint32_t *>(smem + S::MASK_AT);
+  const int kv_rs = own_sgpr(static_cast<int>(a0.kv_rs));
   // Lane l's piece of copy c lands at row drow, piece l % LPR of the tile; it
   // fetches the piece that the swizzle puts there.
   uint32_t src_k[COPS], src_v[COPS];
@@ -296,54 +375,78 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       src_v[c] = row_off + (((lane % S::LPR) ^ swz_v(drow)) << 4);
     }
   }
-  // The piece being copied: list positions st_i .. st_end - 1 of its tiles, in
-  // runs that share a page (or, packed, a stretch of the list).
+  // The copies are a stream of ring entries, kAhead of them ahead of the tile
+  // at work, which runs on into the next item's tiles.  The item being copied:
+  // list positions st_i .. st_end - 1 of its tiles, in runs that share a page
+  // (or, packed, a stretch of the list).
   int st_i = 0, st_end = 0, st_run = 0;  // next list position, the piece's end, tiles left in the run
   int st_ts = 0, st_tlo = 0, st_Lk = 0;
   int st_key = 0;           // first key of the next tile
-  const uint8_t *st_k = a.k;  // its K source (row 0, at the kv head)
+  const uint8_t *st_k = a0.k;  // its K source (row 0, at the kv head)
   bool st_ok = false;
   const int32_t *st_bt = nullptr;
   int st_blk = -1;          // value of the table entry that the next run needs
   int64_t st_base = 0;      // packed: byte offset of the sequence's first key
-  uint32_t st_dst = lds0;
-  uint64_t bad = 0;         // list position mod 64 of tiles in missing pages
-  const int64_t v_minus_k = a.v - a.k;
-  auto tile_at = [&](int i) { return i < st_ts ? i : i - st_ts + st_tlo; };
-  auto entry = [&](int tile) -> int {
-    const int e = small_div(tile, tiles_per_blk);
-    return e < a.max_blocks ? ld_const(st_bt + e) : -1;
+  int st_pos = 0;           // entries issued so far
+  uint32_t st_dst = lds0;   // ring slot of the next one
+  uint64_t bad = 0;         // entry mod 64 of tiles in missing pages
+  // the item queued to be copied next, and the entry of its first tile once started
+  bool nx_queued = false;
+  int nx_lo = 0, nx_hi = 0, nx_ts = 0, nx_tlo = 0, nx_Lk = 0, nx_k0 = 0, nx_blk = -1, nx_first = 0;
+  const int32_t *nx_bt = nullptr;
+  const int64_t v_minus_k = own_sgpr(static_cast<int64_t>(a0.v - a0.k));
+  auto entry = [&](KernArgs &a, const int32_t *bt, int tile) -> int {
+    const int e = small_div(tile, a.block_size / kKeys);
+    return e < a.max_blocks ? ld_const(bt + e) : -1;
   };
-  auto copy_start = [&](const Seq &q, const Tiles &t, int lo, int hi) {
-    st_i = lo;
-    st_end = hi;
-    st_run = 0;
-    st_ts = t.ts;
-    st_tlo = t.tlo;
-    st_Lk = q.Lk;
-    bad = 0;
+  auto queue = [&](const Item &it) {
+    nx_queued = it.live && it.hi > it.lo;
+    if (!nx_queued) return;
+    KernArgs &a = *kernel_args();
+    nx_lo = it.lo;
+    nx_hi = it.hi;
+    nx_ts = it.tl.ts;
+    nx_tlo = it.tl.tlo;
+    nx_Lk = it.q.Lk;
+    nx_k0 = it.q.k0;
     if (paged) {
-      st_bt = a.block_tables + static_cast<int64_t>(q.s) * a.bt_stride;
-      if (lo < hi) st_blk = entry(tile_at(lo));
-    } else {
-      st_base = static_cast<int64_t>(q.k0) * kv_rs + h * SRC_ROWB;
+      nx_bt = a.block_tables + static_cast<int64_t>(it.q.s) * a.bt_stride;
+      nx_blk = entry(a, nx_bt, nx_lo < nx_ts ? nx_lo : nx_lo - nx_ts + nx_tlo);
     }
   };
   // Source and readable bytes of the next tile's copies (0 bytes: zeros).
   auto next_tile = [&](const uint8_t *&src, uint32_t &nrec) {
-    src = a.k;
+    src = st_k;
     nrec = 0;
-    if (st_i >= st_end) return;
+    const int at = st_pos++ & 63;
+    bad &= ~(1ull << at);
+    if (st_i >= st_end) {
+      if (!nx_queued) return;
+      nx_queued = false;
+      nx_first = st_pos - 1;
+      st_i = nx_lo;
+      st_end = nx_hi;
+      st_run = 0;
+      st_ts = nx_ts;
+      st_tlo = nx_tlo;
+      st_Lk = nx_Lk;
+      st_bt = nx_bt;
+      st_blk = nx_blk;
+      st_base = static_cast<int64_t>(nx_k0) * kv_rs + h * SRC_ROWB;
+    }
     if (st_run == 0) {
+      KernArgs &a = *kernel_args();
+      auto tile_at = [&](int i) { return i < st_ts ? i : i - st_ts + st_tlo; };
       const int tile = tile_at(st_i);
       st_key = tile * kKeys;
       const int list = (st_i < st_ts ? min(st_ts, st_end) : st_end) - st_i;  // tiles in a row of the list
       if (paged) {
+        const int tiles_per_blk = a.block_size / kKeys;
         const int in_blk = tile - small_div(tile, tiles_per_blk) * tiles_per_blk;
         st_run = min(list, tiles_per_blk - in_blk);
         st_ok = st_blk >= 0 && st_blk < a.num_blocks;
         st_k = a.k + (static_cast<int64_t>(st_ok ? st_blk : 0) * a.block_size + in_blk * kKeys) * kv_rs + h * SRC_ROWB;
-        if (st_i + st_run < st_end) st_blk = entry(tile_at(st_i + st_run));  // used a run from now
+        if (st_i + st_run < st_end) st_blk = entry(a, st_bt, tile_at(st_i + st_run));  // used a run from now
       } else {
         st_run = list;
         st_ok = true;
@@ -353,8 +456,9 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
     if (st_ok) {
       src = st_k;
       nrec = static_cast<uint32_t>(min(kKeys, st_Lk - st_key) * kv_rs);
+    } else {
+      bad |= 1ull << at;
     }
-    bad = (bad & ~(1ull << (st_i & 63))) | (static_cast<uint64_t>(!st_ok) << (st_i & 63));
     st_k += kKeys * kv_rs;
     st_key += kKeys;
     --st_run;
@@ -426,61 +530,115 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
   // register per operand
   auto unhoist = [&]() { asm volatile("" : "+v"(kx_l), "+v"(vx_l)); };
 
-  const float sl2 = a.scale_log2 * (FP8 ? ld_const(a.k_scale + h) : 1.f);
-  const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
+  const float sl2 = a0.scale_log2 * (FP8 ? ld_const(a0.k_scale + h) : 1.f);
+
+  constexpr int kAhead = RW == 1 ? SLOTS : SLOTS - 1;
+  const uint8_t *src;
+  uint32_t nrec;
+  auto next_slot = [&](uint32_t x) { return x == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : x + SLOT_B; };
+  auto issue = [&]() {
+    next_tile(src, nrec);
+    copy_k(st_dst, src, nrec);
+    copy_v(st_dst, src, nrec);
+    st_dst = next_slot(st_dst);
+  };
 
   // ---------------------------------------------------------------- items
+  Item cur = describe(pos0);
+  queue(cur);
+  // the item whose output is still in registers
+  struct Done {
+    bool live, whole;
+    int q0, r0, r_last, unit;
+  };
+  Done done{};
+  int turn = 0;
+  float m_use[QS], lsum[QS];
+  float mref[QS];  // what P's exponents subtract: m_use, or 0 while a row has seen nothing
+  f32x4 o[QS][NJ];
   for (;;) {
-    const Seq q = seq_of(a, s, true);
-    const int n_rt = row_tiles<S>(a, q);
-    const int r_first = rt * M;                         // rows of the tile
-    const int r_last = min(r_first + M, q.Lq * a.G) - 1;
-    const int t_first = small_div(r_first, a.G), t_last = small_div(r_last, a.G);
-    const Tiles tl = tiles_of(a, q, t_first, t_last);
-    int lo = 0, hi = tl.n;
-    bool first_here = true;  // the item's start lies in this range
-    if (ranges) {
-      const int x0 = X + Cost<S>::kItem;
-      lo = max(0, min(tl.n, pos0 - x0));
-      hi = max(0, min(tl.n, pos1 - x0));
-      first_here = X >= pos0;
+    // this wave's rows and their tokens (a wave past the last row sees no key
+    // and stores nothing)
+    const Seq q = cur.q;
+    const int r0 = cur.r_first + rw * QS * 16, r_last = cur.r_last;
+    const bool wave_live = cur.live && r0 <= r_last;
+    const int t_first = cur.t_first, t_last = cur.t_last;
+    int tok[QS];  // of this lane's rows
+    u32x4 qf[QS][NKK];
+    // Its copies, as far as they are not under way: the first item's, and those
+    // behind items of few tiles, whose empty entries may lie in the slot that
+    // another wave still works on.
+    const bool tiles = cur.live && cur.hi > cur.lo;
+    if (RW > 1 && tiles && (nx_queued || st_pos < nx_first + kAhead)) {
+      wait_lgkmcnt0();
+      raw_barrier();
     }
-    const int P = q.Lk - q.Lq;
-    if (hi > lo || (tl.n == 0 && first_here)) {
-      const int n = hi - lo;
-      const bool whole = lo == 0 && hi == tl.n;
-      // this wave's rows and their tokens (a wave past the last row sees no key
-      // and stores nothing)
-      const int r0 = r_first + rw * QS * 16;
-      const bool wave_live = r0 <= r_last;
-      const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
-      copy_start(q, tl, lo, hi);
-      uint32_t slot = lds0;  // ring slot of the tile computed next
-      const uint8_t *src;
-      uint32_t nrec;
-      constexpr int kAhead = RW == 1 ? SLOTS : SLOTS - 1;
-      st_dst = lds0;
+    if (tiles && nx_queued) issue();
+    const int p0 = nx_first;  // entry of its first tile
+    Item nxt{};
+    if (cur.live) {
+      nxt = describe(cur.next);
+      queue(nxt);
+    }
+    if (tiles)
+      while (st_pos < p0 + kAhead) issue();
+    // Q, then the output of the item before while it arrives.  (No live item:
+    // some row's.)
+    KernArgs &a = *kernel_args();
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        next_tile(src, nrec);
-        copy_k(lds0 + i * SLOT_B, src, nrec);
-        copy_v(lds0 + i * SLOT_B, src, nrec);
-      }
-      st_dst = lds0 + (RW == 1 ? 0 : kAhead * SLOT_B);
-
-      int tok[QS], head[QS];  // of this lane's rows
-      u32x4 qf[QS][NKK];
+    for (int qs = 0; qs < QS; ++qs) {
+      const int r = cur.live ? min(r0 + 16 * qs + m, r_last) : 0;
+      tok[qs] = small_div(r, a.G);
+      const uint8_t *qp = a.q + static_cast<int64_t>(cur.live ? q.q0 + tok[qs] : 0) * a.q_rs +
+                          (h * a.G + r - tok[qs] * a.G) * a.q_hs;
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) qf[qs][kk] = load16(qp + (8 * g + 32 * kk) * 2);
+    }
+    if (done.live) {
+      const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
+      // lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
-        const int r = min(r0 + 16 * qs + m, r_last);
-        tok[qs] = small_div(r, a.G);
-        head[qs] = h * a.G + r - tok[qs] * a.G;
-        const uint8_t *qp = a.q + static_cast<int64_t>(q.q0 + tok[qs]) * a.q_rs + head[qs] * a.q_hs;
+        const float l = sum32(sum16(lsum[qs]));
+        const float inv = (l > 0.f ? 1.0f / l : 0.f) * vscale;
+        const int r = done.r0 + 16 * qs + m;
+        if (!done.whole) {
+          const int64_t unit = static_cast<int64_t>(done.unit) + qs;
+          f32x4 *po = reinterpret_cast<f32x4 *>(a.part_o) + unit * NJ * 64 + lane;
+          if (r <= done.r_last) {
 #pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) qf[qs][kk] = load16(qp + (8 * g + 32 * kk) * 2);
+            for (int j = 0; j < NJ; ++j) po[j * 64] = o[qs][j] * inv;
+            if (g == 0) a.part_l[unit * 16 + m] = l == 0.f ? kNegInf : m_use[qs] + __log2f(l);
+          }
+        } else if (r <= done.r_last) {
+          const int t = small_div(r, a.G), head = h * a.G + r - t * a.G;
+          uint8_t *op = a.out + static_cast<int64_t>(done.q0 + t) * a.o_rs + head * a.o_hs + 8 * g;
+          const uint8_t *gp = a.gate + static_cast<int64_t>(done.q0 + t) * a.g_rs + head * a.g_hs + 8 * g;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const f32x4 v = o[qs][j] * inv;
+            *reinterpret_cast<u32x2 *>(op + 32 * j) =
+                a.gate ? gate4<T>(v, *reinterpret_cast<const u32x2 *>(gp + 32 * j))
+                       : u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+          }
+        }
       }
-      if (a.window == 0) {
+    }
+    if (!cur.live) break;
+    {
+      const Tiles tl = cur.tl;
+      const int lo = cur.lo, hi = cur.hi, n = hi - lo;
+      const int P = q.Lk - q.Lq;
+      const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
+      uint32_t slot = lds0 + (static_cast<unsigned>(p0) % SLOTS) * SLOT_B;  // of the tile computed next
+      const int window = own_sgpr(a.window), sinks = own_sgpr(a.sinks);
+      const bool tree = window == 0, careful = cur.careful;
+      if (tree) {
         // the masks of the tile's tokens, 32-bit words
+        if constexpr (RW > 1) {  // the last item's have been read
+          wait_lgkmcnt0();
+          raw_barrier();
+        }
         const int w32 = 2 * a.words, cnt = (t_last - t_first + 1) * w32;
         const uint32_t *mp = reinterpret_cast<const uint32_t *>(a.mask);
         for (int i = threadIdx.x; i < cnt; i += 64 * RW) {
@@ -498,9 +656,6 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
-      float m_use[QS], lsum[QS];
-      float mref[QS];  // what P's exponents subtract: m_use, or 0 while a row has seen nothing
-      f32x4 o[QS][NJ];
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
         m_use[qs] = kNegInf;
@@ -510,19 +665,37 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         for (int j = 0; j < NJ; ++j) o[qs][j] = f32x4{0, 0, 0, 0};
       }
 
+      auto key_of = [&](int i) { return (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys; };
+      // List positions [first, first + count) of tiles that the tokens ta .. tb all
+      // see whole, while no page is missing (sinks that a window does not reach
+      // are not among them).
+      struct Plain {
+        int first;
+        unsigned count;
+      };
+      auto plain_of = [&](int ta, int tb) -> Plain {
+        int t0 = 0, t1;  // tiles
+        if (!tree) {
+          t0 = max(tl.ts == tl.tlo ? 0 : tl.tlo, (max(P + tb - window, -kKeys) + kKeys) / kKeys);
+          t1 = max(0, P + ta + 1) / kKeys;
+        } else {
+          t1 = max(0, P) / kKeys;
+        }
+        return Plain{t0 - tl.tlo + tl.ts, static_cast<unsigned>(max(0, t1 - t0))};
+      };
       // Keys of the tile at `key0` that row block qs of this lane sees: bit
       // 4 ks + r for key 16 ks + 4 g + r.
       auto seen = [&](int qs, int key0) -> uint32_t {
         uint32_t v = 0;
-        if (a.window > 0) {
-          const int top = P + tok[qs], bot = top - a.window;
+        if (!tree) {
+          const int top = P + tok[qs], bot = top - window;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
-            v |= (key <= top && (key > bot || key < a.sinks)) ? 1u << i : 0u;
+            v |= (key <= top && (key > bot || key < sinks)) ? 1u << i : 0u;
           }
         } else {
-          const int rel = key0 - P, w32 = 2 * a.words;
+          const int rel = key0 - P, w32 = 2 * kernel_args()->words;
           const uint32_t *mr = lds_mask + (tok[qs] - t_first) * S::MASK_WORDS;
           uint32_t bits;
           if (rel < 0) {
@@ -542,23 +715,49 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       f32x4 sc[QS][2];  // scores of the tile whose P is formed next
       u32x4 pb[QS];     // P, in the second product's operand form
       uint32_t vis[QS];
-      // The rows' maxima over the tile's scores (masked where `vis` says so)
-      // against the running ones.  A maximum moves when some score exceeds it by
+      // The scores of keys that the rows do not see, replaced.  (Of a window, keys
+      // past the sinks: one comparison of the distance to its first key.)
+      auto mask_tile = [&](int i, bool live) {
+        const int key0 = key_of(i);
+        if (!live || ((bad >> ((p0 + i - lo) & 63)) & 1)) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) {
+            vis[qs] = 0;
+            sc[qs][0] = sc[qs][1] = f32x4{kNegInf, kNegInf, kNegInf, kNegInf};
+          }
+          return;
+        }
+        if (!tree && !careful && key0 >= sinks) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) {
+            const int d0 = key0 + 4 * g - (P + tok[qs] - window + 1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int d = d0 + 16 * (e >> 2) + (e & 3);
+              sc[qs][e >> 2][e & 3] = static_cast<unsigned>(d) < static_cast<unsigned>(window) ? sc[qs][e >> 2][e & 3] : kNegInf;
+            }
+          }
+          return;
+        }
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          vis[qs] = seen(qs, key0);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!((vis[qs] >> e) & 1u)) sc[qs][e >> 2][e & 3] = kNegInf;
+        }
+      };
+      // The rows' maxima over the tile's scores against the running ones.  A maximum moves when some score exceeds it by
       // more than kRescale; then every row's is brought up to date, alpha holds
       // the factors for o, and the result is true.
-      auto check = [&](bool masked, float (&alpha)[QS]) -> bool {
+      auto check = [&](float (&alpha)[QS]) -> bool {
         float mloc[QS];
         bool grow = false;
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) {
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (!((vis[qs] >> i) & 1u)) sc[qs][i >> 2][i & 3] = kNegInf;
-          }
-          mloc[qs] = max3_raw(max3_raw(sc[qs][0][0], sc[qs][0][1], sc[qs][0][2]),
-                              max3_raw(sc[qs][0][3], sc[qs][1][0], sc[qs][1][1]),
-                              vmax_raw(sc[qs][1][2], sc[qs][1][3])) * sl2;
+          mloc[qs] = max3(max3(sc[qs][0][0], sc[qs][0][1], sc[qs][0][2]),
+                          max3(sc[qs][0][3], sc[qs][1][0], sc[qs][1][1]),
+                          __builtin_elementwise_maximum(sc[qs][1][2], sc[qs][1][3])) * sl2;
           grow |= mloc[qs] > m_use[qs] + kRescale;
         }
         if (__builtin_amdgcn_ballot_w64(grow) == 0) return false;
@@ -597,11 +796,12 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
             for (int qs = 0; qs < QS; ++qs) sc[qs][ks] = T::mfma16x16x32(kf, qf[qs][kk], sc[qs][ks]);
           }
       };
-      // A tile that not every row sees whole: 0 * NaN must not reach a row
-      // through a key it does not see.  When such a tile holds values that are
-      // not finite (`odd_values`), `poison` adds them to the outputs of the rows
-      // that see them and `clean` takes them out of the tile.  The waves that
-      // share the tile check and clean a part of it each.
+      // 0 * NaN must not reach a row through a key it does not see.  An item whose
+      // outputs are not all finite is done again, carefully: when a tile that not
+      // every row sees whole then holds values that are not finite
+      // (`odd_values`), `poison` adds them to the outputs of the rows that see
+      // them and `clean` takes them out of the tile.  The waves that share the
+      // tile check and clean a part of it each.
       constexpr uint32_t kExp = T::dtype == NQ_BF16 ? 0x7f80u : 0x7c00u;
       constexpr uint32_t kMant = T::dtype == NQ_BF16 ? 0x007fu : 0x03ffu;
       // top bit of every half (fp8: byte) of w that is not finite: its exponent
@@ -613,7 +813,7 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
       };
       constexpr int kPart = TILE_B / RW / 64;  // bytes of the tile's values per lane
       auto part_of = [&](uint32_t kt, int c) { return kt + TILE_B + (rw * (kPart / 16) + c) * 1024 + lane * 16; };
-      uint32_t *const lds_odd = lds_mask + S::TOKENS * S::MASK_WORDS;
+      uint32_t *const lds_odd = reinterpret_cast<uint32_t *>(smem + S::ODD_AT);
       auto odd_values = [&](uint32_t kt) -> bool {
         uint32_t any = 0;
 #pragma unroll 2
@@ -694,65 +894,33 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
             }
         }
       };
-      // What the tokens ta .. tb make of the tile at list position i: 0 nothing (no
-      // key of it is seen, or its page is missing), 1 every row sees every key,
-      // 2 masked.
-      auto kind_of = [&](int i, int key0, int ta, int tb) -> int {
-        if ((bad >> (i & 63)) & 1) return 0;
-        if (a.window == 0) return key0 + kKeys <= P ? 1 : 2;
-        const int pa = P + ta, pz = P + tb;
-        if (key0 > pz || (key0 + kKeys - 1 <= pa - a.window && key0 >= a.sinks)) return 0;
-        return key0 + kKeys - 1 <= pa && (key0 > pz - a.window || key0 + kKeys <= a.sinks) ? 1 : 2;
-      };
-
-      auto key_of = [&](int i) { return (i < tl.ts ? i : i - tl.ts + tl.tlo) * kKeys; };
-      // List positions [first, first + count) where kind_of is 1 for tokens ta .. tb
-      // while no page is missing (of a window; sinks that it does not reach are
-      // left to kind_of).
-      struct Plain {
-        int first;
-        unsigned count;
-      };
-      auto plain_of = [&](int ta, int tb) -> Plain {
-        int t0 = 0, t1;  // tiles
-        if (a.window > 0) {
-          t0 = max(tl.ts == tl.tlo ? 0 : tl.tlo, (max(P + tb - a.window, -kKeys) + kKeys) / kKeys);
-          t1 = max(0, P + ta + 1) / kKeys;
-        } else {
-          t1 = max(0, P) / kKeys;
-        }
-        return Plain{t0 - tl.tlo + tl.ts, static_cast<unsigned>(max(0, t1 - t0))};
-      };
       float alpha[QS];
       if constexpr (RW == 1) {
+        const Plain plain = plain_of(ta, tb);
         for (int i = lo; i < hi; ++i) {
-          const int key0 = key_of(i);
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // K of this tile (younger: its V and the tiles after it)
           asm volatile("" ::: "memory");
-          const int kind = kind_of(i, key0, ta, tb);
-          if (kind != 0) scores(slot);
+          scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
+          const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && bad == 0;
+          if (!whole_tile) mask_tile(i, true);
           next_tile(src, nrec);
           copy_k(slot, src, nrec);
-          if (kind == 2) vis[0] = seen(0, key0);
-          if (kind != 0) {
-            if (check(kind == 2, alpha)) rescale(alpha);
+          if (check(alpha)) rescale(alpha);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) pb[0][t] = p_unit(0, t);
-          }
+          for (int t = 0; t < 4; ++t) pb[0][t] = p_unit(0, t);
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
           asm volatile("" ::: "memory");
-          if (kind == 2 && __builtin_expect(odd_values(slot), 0)) {
+          if (careful && !whole_tile && odd_values(slot)) {
             poison(slot);
             clean(slot);
           }
-          if (kind != 0) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) o[0][j] = T::mfma16x16x32(op(v_read(slot, j)), pb[0], o[0][j]);
-          }
+          for (int j = 0; j < NJ; ++j) o[0][j] = T::mfma16x16x32(op(v_read(slot, j)), pb[0], o[0][j]);
           wait_lgkmcnt0();
           copy_v(slot, src, nrec);
-          slot = slot == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : slot + SLOT_B;
+          slot = next_slot(slot);
+          st_dst = next_slot(st_dst);
         }
       } else if (n > 0) {
         // One tile per step, three tiles at work: P of tile i is formed among the
@@ -767,22 +935,15 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
         KV vf[NJ];  // V operands of the tile whose products are pending
         const Plain plain_w = wave_live ? plain_of(ta, tb) : Plain{0, 0}, plain_wg = plain_of(t_first, t_last);
         bool pend = false;
-        auto next_slot = [&](uint32_t x) { return x == lds0 + (SLOTS - 1) * SLOT_B ? lds0 : x + SLOT_B; };
         auto step = [&](auto first_tag, int i) {
           constexpr bool FIRST = decltype(first_tag)::value;
           unhoist();
           if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
           const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && bad == 0;
-          if (!whole_tile) {
-            const int key0 = key_of(i);
-            const int kind = wave_live ? kind_of(i, key0, ta, tb) : 0;
-#pragma unroll
-            for (int qs = 0; qs < QS; ++qs) vis[qs] = kind == 0 ? 0u : kind == 1 ? 0xffu : seen(qs, key0);
-          }
-          pend = check(!whole_tile, alpha);
+          if (!whole_tile) mask_tile(i, wave_live);
+          pend = check(alpha);
           // (for all of the workgroup's waves alike)
-          if (!(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && bad == 0) &&
-              kind_of(i, key_of(i), t_first, t_last) == 2 && __builtin_expect(odd_values(slot), 0)) {
+          if (careful && !(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && bad == 0) && odd_values(slot)) {
             // o is brought up to date before the odd values join it
             if constexpr (!FIRST) {
 #pragma unroll
@@ -801,10 +962,7 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
             poison(slot);
             clean(slot);
           }
-          next_tile(src, nrec);
-          copy_k(st_dst, src, nrec);
-          copy_v(st_dst, src, nrec);
-          st_dst = next_slot(st_dst);
+          issue();
           KV kf[NKK][2];
           {
             const uint32_t slot_next = next_slot(slot);
@@ -905,61 +1063,53 @@ __device__ __forceinline__ void span_body(const SpanArgs &a) {
           for (int qs = 0; qs < QS; ++qs) o[qs][j] = T::mfma16x16x32(op(vf[j]), pb[qs], o[qs][j]);
       }
 
-      // ---- epilogue: lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
+      // outputs that are not finite: carefully, again (every wave alike)
+      float zero = 0.f;
 #pragma unroll
-      for (int qs = 0; qs < QS; ++qs) {
-        const float l = sum32(sum16(lsum[qs]));
-        const float inv = (l > 0.f ? 1.0f / l : 0.f) * vscale;
-        const int r = r0 + 16 * qs + m;
-        if (!whole) {
-          const int64_t unit = (static_cast<int64_t>(2 * w_of + (lo > 0 ? 0 : 1)) * RW + rw) * QS + qs;
-          f32x4 *po = reinterpret_cast<f32x4 *>(a.part_o) + unit * NJ * 64 + lane;
-          if (r <= r_last) {
+      for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) po[j * 64] = o[qs][j] * inv;
-            if (g == 0) a.part_l[unit * 16 + m] = l == 0.f ? kNegInf : m_use[qs] + __log2f(l);
-          }
-        } else if (r <= r_last) {
-          uint8_t *op = a.out + static_cast<int64_t>(q.q0 + tok[qs]) * a.o_rs + head[qs] * a.o_hs + 8 * g;
-          const uint8_t *gp = a.gate + static_cast<int64_t>(q.q0 + tok[qs]) * a.g_rs + head[qs] * a.g_hs + 8 * g;
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const f32x4 v = o[qs][j] * inv;
-            *reinterpret_cast<u32x2 *>(op + 32 * j) =
-                a.gate ? gate4<T>(v, *reinterpret_cast<const u32x2 *>(gp + 32 * j))
-                       : u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-          }
-        }
+          for (int r = 0; r < 4; ++r) zero = __builtin_fmaf(o[qs][j][r], 0.f, zero);
+      bool again = __builtin_amdgcn_ballot_w64(zero != 0.f) != 0;
+      if constexpr (RW > 1) {
+        // (flags by turns: a wave may be an item ahead of another's reads)
+        uint32_t *const flags = lds_odd + 8 + (turn & 1) * 8;
+        ++turn;
+        if (lane == 0) flags[rw] = again;
+        wait_lgkmcnt0();
+        raw_barrier();
+        again = __builtin_amdgcn_ballot_w64(lane < RW && flags[lane & (RW - 1)] != 0) != 0;
       }
-      if (!whole) (lo > 0 ? desc0 : desc1) = int4{s, rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
+      if (again && !careful) {
+        // the copies under way are given up, and the item is queued anew
+        wait_vmcnt<0>();
+        wait_lgkmcnt0();
+        if constexpr (RW > 1) raw_barrier();
+        st_i = st_end = 0;
+        cur.careful = true;
+        queue(cur);
+        done.live = false;
+        continue;
+      }
+      const bool whole = lo == 0 && hi == tl.n;
+      done = Done{true, whole, q.q0, r0, r_last, ((2 * w_of + (lo > 0 ? 0 : 1)) * RW + rw) * QS};
+      if (!whole) (lo > 0 ? desc0 : desc1) = int4{q.s, cur.rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
     }
-    // the next row tile of the range
-    if (!ranges) break;
-    X += item_cost<S>(a, q);
-    if (++rt >= n_rt) {
-      rt = 0;
-      Seq nx;
-      do {
-        if (++s >= a.num_seqs) break;
-        nx = seq_of(a, s, true);
-      } while (nx.Lq <= 0);
-      if (s >= a.num_seqs) break;
-    }
-    if (X >= pos1) break;
-    // every copy has landed and every read is done before the next item's
-    // copies take the slots
-    wait_vmcnt<0>();
-    wait_lgkmcnt0();
-    if constexpr (RW > 1) raw_barrier();
+    cur = nxt;
   }
-  leave();
+  if (ranges && rw == 0 && lane == 0) {
+    int4 *d = kernel_args()->part_desc + 2 * w_of;
+    d[0] = desc0;
+    d[1] = desc1;
+  }
   wait_vmcnt<0>();  // no copy outlives the workgroup's LDS
 }
 
 template <class T, bool FP8, class S>
 __global__ __launch_bounds__(64 * S::RW) __attribute__((amdgpu_waves_per_eu(S::RW == 1 ? 1 : 2)))
 void span_attention_kernel(const SpanArgs a) {
-  span_body<T, FP8, S>(a);
+  span_body<T, FP8, S>();
 }
 
 // Merge of the items that ranges cut: workgroup (range, part) takes the item
@@ -1066,9 +1216,12 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
     span_merge_kernel<T, S><<<dim3(static_cast<unsigned>(W * a.Hkv), S::RW * S::QS * S::NJ / 4), 256, 0, stream>>>(a);
     return check_launch("span attention (merge)");
   }
+  // Whole items, dealt out in turn to the workgroups that the chip holds at once
+  // (a multiple of 8 where kv heads share XCDs, and of the kv heads otherwise).
   const int per = a.Hkv < 8 && 8 % a.Hkv == 0 ? 8 / a.Hkv : 1;
-  const int64_t grid = (items + per - 1) / per * per * a.Hkv;
-  if (grid > 0x7fffffff) return fail(NQ_EINVAL, "span attention: %lld work items", (long long)grid);
+  const int64_t unit = static_cast<int64_t>(a.Hkv) * per;
+  const int64_t grid = unit * std::max<int64_t>(1, std::min((items + per - 1) / per, slots / unit));
+  a.stride = static_cast<int>(grid / a.Hkv);
   span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(grid)), 64 * S::RW, S::LDS_B, stream>>>(a);
   return check_launch("span attention");
 }
