@@ -109,7 +109,7 @@ struct Shape {
   static constexpr int SEQS = 256;  // sequences whose bounds are kept in LDS
   // ring, masks, flags of odd tiles, sequences' bounds and positions
   static constexpr int MASK_AT = RING_B, ODD_AT = MASK_AT + (TOKENS * MASK_WORDS * 4 + 15) / 16 * 16,
-                       SEQ_AT = ODD_AT + 128, POS_AT = SEQ_AT + SEQS * 16, LDS_B = POS_AT + SEQS * 4;
+                       SEQ_AT = ODD_AT + 128, POS_AT = SEQ_AT + SEQS * 16, LDS_B = POS_AT + SEQS * 8;
   static constexpr int NKK = D / 32, NJ = D / 16;
   static_assert(COPS >= 1, "every wave copies");
 };
@@ -157,6 +157,9 @@ __device__ __forceinline__ int small_div(int n, int d) {
     ++q;
   return q;
 }
+// A value that every lane has, in a scalar register (small_div leaves it in a
+// vector one).
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // Of scores as they leave the matrix core: instructions that the compiler knows,
 // so that it keeps the wait states between a product and its readers (inline
 // assembly has none).  A NaN among them is the result.
@@ -238,27 +241,40 @@ __device__ __forceinline__ void span_body() {
     w = L / a0.Hkv;
   }
 
-  // The batch's row tiles laid end to end, each as its cost (whole items: 1).
+  // The batch's row tiles laid end to end.  In equal ranges each counts as its
+  // cost.  Whole items are dealt out in rounds, every other round in reverse:
+  // first the row tiles whose window is full, which cost the same, then those
+  // nearer their sequence's start, each sequence's from the costly end (`ramp`
+  // of them), so that the workgroups' sums stay even.
   // Of up to SEQS sequences the bounds and the positions of their ends are kept
-  // in LDS, so that finding an item is no chain of round trips to memory.
+  // in LDS, so that finding an item is no chain of round trips to memory; with
+  // more of them whole items are dealt out in order.
   int4 *const lds_seq = reinterpret_cast<int4 *>(smem + S::SEQ_AT);
-  int *const lds_pos = reinterpret_cast<int *>(smem + S::POS_AT);
+  int2 *const lds_pos = reinterpret_cast<int2 *>(smem + S::POS_AT);
   const bool listed = a0.num_seqs <= S::SEQS;
   auto weight_of = [&](KernArgs &a, const Seq &q) -> int { return ranges ? item_cost<S>(a, q) : (q.Lq > 0 ? 1 : 0); };
-  int total = 0;
+  auto ramp_of = [&](KernArgs &a, const Seq &q, int tiles) -> int {
+    if (ranges || !listed || a.window == 0) return 0;
+    const int short_of = min(a.window - 1 - (q.Lk - q.Lq), q.Lq);  // tokens whose window is not full
+    return max(0, min(tiles, (short_of * a.G + M - 1) / M));
+  };
+  int total = 0, total_ramp = 0;
   for (int b = 0; b < a0.num_seqs; b += 64) {
-    int c = 0;
+    int c = 0, ramp = 0;
     Seq q{};
     if (b + lane < a0.num_seqs) {
       q = seq_of(a0, b + lane, false);
-      c = row_tiles<S>(a0, q) * weight_of(a0, q);
+      c = row_tiles<S>(a0, q);
+      ramp = ramp_of(a0, q, c);
+      c = (c - ramp) * weight_of(a0, q);
     }
-    const int incl = total + wave_iscan(c);
+    const int incl = total + wave_iscan(c), incl_ramp = total_ramp + wave_iscan(ramp);
     if (listed && rw == 0 && b + lane < a0.num_seqs) {
       lds_seq[b + lane] = int4{q.q0, q.Lq, q.k0, q.Lk};
-      lds_pos[b + lane] = incl;
+      lds_pos[b + lane] = int2{incl, incl_ramp};
     }
     total = __builtin_amdgcn_readlane(incl, 63);
+    total_ramp = __builtin_amdgcn_readlane(incl_ramp, 63);
   }
   if (listed) {
     if constexpr (RW == 1)
@@ -266,8 +282,9 @@ __device__ __forceinline__ void span_body() {
     else
       __syncthreads();
   }
-  int pos0 = w, pos1 = total;  // this workgroup's positions: all of them, or every stride-th
-  int w_of = 0;                // the range's partials
+  // Where this workgroup is: its next position (ranges), or its next round.
+  int pos0 = 0, pos1 = total + total_ramp;
+  int w_of = 0;  // the range's partials
   if (ranges) {
     w_of = h * n_ranges + w;
     const int W = min(n_ranges, max(1, total / Cost<S>::kMinRange));
@@ -276,41 +293,49 @@ __device__ __forceinline__ void span_body() {
   }
   // The range's two partial pieces, written for the merge when it is done.
   int4 desc0{0, 0, kPieceNone, 0}, desc1{0, 0, kPieceNone, 0};
-  // The first item at or after position `pos` that this workgroup has to do
-  // something for (live: there is one).
+  // The first item from `at` (a position or a round) on that this workgroup has
+  // to do something for (live: there is one).
   struct Item {
-    bool live, careful;
+    bool live;
     Seq q;
-    int rt, lo, hi, next;  // its row tile, its part of the tiles, the next position
+    int rt, lo, hi, at, next;  // its row tile, its part of the tiles, where it and the next are looked for
     int r_first, r_last, t_first, t_last;
     Tiles tl;
   };
-  auto describe = [&](int pos) -> Item {
+  auto describe = [&](int at) -> Item {
     KernArgs &a = *kernel_args();
     Item it{};
-    while (pos < pos1) {
-      // sequence and row tile at pos; X: where it starts
-      int X = 0;
-      int start = 0, cost = 1;
-      bool found = false;
+    for (;;) {
+      const int pos = ranges ? at : at * a.stride + ((at & 1) ? a.stride - 1 - w : w);
+      if (ranges ? pos >= pos1 : at * a.stride >= pos1) return it;
+      it.at = at;
+      it.next = at + 1;
+      if (pos >= pos1) {  // the last round is a part of one
+        at = it.next;
+        continue;
+      }
+      const bool ramp = pos >= total;
+      const int want = ramp ? pos - total : pos;
+      int start = 0, cost = 1;  // where the sequence's row tiles start, and each one's weight
       if (listed) {
-        for (int b = 0; b < a.num_seqs; b += 64) {
-          const int e = min(b + lane, a.num_seqs - 1);
-          const uint64_t hit = __builtin_amdgcn_ballot_w64(lds_pos[e] > pos);
-          if (hit != 0) {
-            const int s = b + static_cast<int>(__builtin_ctzll(hit));
-            const int4 x = lds_seq[s];
-            it.q.s = s;
-            it.q.q0 = __builtin_amdgcn_readfirstlane(x.x);
-            it.q.Lq = __builtin_amdgcn_readfirstlane(x.y);
-            it.q.k0 = __builtin_amdgcn_readfirstlane(x.z);
-            it.q.Lk = __builtin_amdgcn_readfirstlane(x.w);
-            start = s > 0 ? __builtin_amdgcn_readfirstlane(lds_pos[s - 1]) : 0;
-            cost = weight_of(a, it.q);
-            found = true;
-            break;
+        for (int b = 0;; b += 64) {
+          const int2 e = lds_pos[min(b + lane, a.num_seqs - 1)];
+          const uint64_t hit = __builtin_amdgcn_ballot_w64((ramp ? e.y : e.x) > want);
+          if (hit == 0) continue;  // (the last entry's is the total: past `want`)
+          const int s = b + static_cast<int>(__builtin_ctzll(hit));
+          const int4 x = lds_seq[s];
+          it.q.s = s;
+          it.q.q0 = __builtin_amdgcn_readfirstlane(x.x);
+          it.q.Lq = __builtin_amdgcn_readfirstlane(x.y);
+          it.q.k0 = __builtin_amdgcn_readfirstlane(x.z);
+          it.q.Lk = __builtin_amdgcn_readfirstlane(x.w);
+          if (s > 0) {
+            const int2 before = lds_pos[s - 1];
+            start = __builtin_amdgcn_readfirstlane(ramp ? before.y : before.x);
           }
+          break;
         }
+        cost = weight_of(a, it.q);
       } else {
         int base = 0;
         for (int b = 0; b < a.num_seqs; b += 64) {
@@ -320,29 +345,30 @@ __device__ __forceinline__ void span_body() {
             c = row_tiles<S>(a, q) * weight_of(a, q);
           }
           const int incl = base + wave_iscan(c);
-          const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > pos);
+          const uint64_t hit = __builtin_amdgcn_ballot_w64(incl > want);
           if (hit != 0) {
             const int l = static_cast<int>(__builtin_ctzll(hit));
             it.q = seq_of(a, b + l, true);
             start = __builtin_amdgcn_readlane(incl - c, l);
-            cost = weight_of(a, it.q);
-            found = true;
             break;
           }
           base = __builtin_amdgcn_readlane(incl, 63);
         }
+        cost = weight_of(a, it.q);
       }
-      if (!found) return it;
-      it.rt = static_cast<int>(static_cast<unsigned>(pos - start) / static_cast<unsigned>(cost));
-      X = start + it.rt * cost;
+      it.rt = uni(static_cast<int>(static_cast<unsigned>(want - start) / static_cast<unsigned>(cost)));
+      const int X = start + it.rt * cost;
+      if (!ranges && listed) {
+        const int n_ramp = ramp_of(a, it.q, row_tiles<S>(a, it.q));
+        it.rt = ramp ? n_ramp - 1 - it.rt : n_ramp + it.rt;
+      }
       it.r_first = it.rt * M;
       it.r_last = min(it.r_first + M, it.q.Lq * a.G) - 1;
-      it.t_first = small_div(it.r_first, a.G);
-      it.t_last = small_div(it.r_last, a.G);
+      it.t_first = uni(small_div(it.r_first, a.G));
+      it.t_last = uni(small_div(it.r_last, a.G));
       it.tl = tiles_of(a, it.q, it.t_first, it.t_last);
       it.lo = 0;
       it.hi = it.tl.n;
-      it.next = pos + a.stride;
       if (ranges) {
         it.lo = max(0, min(it.tl.n, pos0 - X - Cost<S>::kItem));
         it.hi = max(0, min(it.tl.n, pos1 - X - Cost<S>::kItem));
@@ -351,9 +377,8 @@ __device__ __forceinline__ void span_body() {
       // an item without tiles is written (zeros) where it starts
       it.live = it.hi > it.lo || (it.tl.n == 0 && (!ranges || X >= pos0));
       if (it.live) return it;
-      pos = it.next;
+      at = it.next;
     }
-    return it;
   };
 
   // ---------------------------------------------------------------- copies
@@ -375,94 +400,75 @@ __device__ __forceinline__ void span_body() {
       src_v[c] = row_off + (((lane % S::LPR) ^ swz_v(drow)) << 4);
     }
   }
+  const int64_t v_minus_k = own_sgpr(static_cast<int64_t>(a0.v - a0.k));
   // The copies are a stream of ring entries, kAhead of them ahead of the tile
-  // at work, which runs on into the next item's tiles.  The item being copied:
-  // list positions st_i .. st_end - 1 of its tiles, in runs that share a page
-  // (or, packed, a stretch of the list).
-  int st_i = 0, st_end = 0, st_run = 0;  // next list position, the piece's end, tiles left in the run
-  int st_ts = 0, st_tlo = 0, st_Lk = 0;
-  int st_key = 0;           // first key of the next tile
-  const uint8_t *st_k = a0.k;  // its K source (row 0, at the kv head)
-  bool st_ok = false;
-  const int32_t *st_bt = nullptr;
-  int st_blk = -1;          // value of the table entry that the next run needs
-  int64_t st_base = 0;      // packed: byte offset of the sequence's first key
-  int st_pos = 0;           // entries issued so far
-  uint32_t st_dst = lds0;   // ring slot of the next one
-  uint64_t bad = 0;         // entry mod 64 of tiles in missing pages
+  // at work, which runs on into the next item's tiles.  Lane l of `list` holds
+  // where the l-th of 64 tiles lies (in tiles of 32 rows; -1: its page is missing).
+  int st_pos = 0;          // entries issued so far
+  uint32_t st_dst = lds0;  // ring slot of the next one
+  int st_list = 0, st_l = 0, st_left = 0;  // the item being copied: its list, the next lane, tiles left
+  int st_at = 0, st_chunk = 0;             // the item, and the lists of 64 before this one
+  const uint8_t *st_base = a0.k;           // what its tiles count from (the kv head of row 0)
+  uint32_t st_last = 0;                    // bytes that the copies of its last tile may read
   // the item queued to be copied next, and the entry of its first tile once started
   bool nx_queued = false;
-  int nx_lo = 0, nx_hi = 0, nx_ts = 0, nx_tlo = 0, nx_Lk = 0, nx_k0 = 0, nx_blk = -1, nx_first = 0;
-  const int32_t *nx_bt = nullptr;
-  const int64_t v_minus_k = own_sgpr(static_cast<int64_t>(a0.v - a0.k));
-  auto entry = [&](KernArgs &a, const int32_t *bt, int tile) -> int {
-    const int e = small_div(tile, a.block_size / kKeys);
-    return e < a.max_blocks ? ld_const(bt + e) : -1;
+  int nx_list = 0, nx_left = 0, nx_at = 0, nx_first = 0;
+  const uint8_t *nx_base = a0.k;
+  uint32_t nx_last = 0;
+  bool bad_seen = false;  // some tile lay in a missing page: from then on every tile is looked up
+  auto list_of = [&](KernArgs &a, const Item &it, int chunk) -> int {
+    const int i = it.lo + 64 * chunk + lane;
+    int at = 0;
+    if (i < it.hi) {
+      const int tile = i < it.tl.ts ? i : i - it.tl.ts + it.tl.tlo;
+      at = tile;
+      if (paged) {
+        const int per = a.block_size / kKeys, e = small_div(tile, per);
+        const int blk = e < a.max_blocks ? a.block_tables[it.q.s * a.bt_stride + e] : -1;
+        at = blk >= 0 && blk < a.num_blocks ? blk * per + (tile - e * per) : -1;
+      }
+    }
+    bad_seen = uni(bad_seen | (__builtin_amdgcn_ballot_w64(at < 0) != 0)) != 0;
+    return at;
   };
   auto queue = [&](const Item &it) {
     nx_queued = it.live && it.hi > it.lo;
     if (!nx_queued) return;
     KernArgs &a = *kernel_args();
-    nx_lo = it.lo;
-    nx_hi = it.hi;
-    nx_ts = it.tl.ts;
-    nx_tlo = it.tl.tlo;
-    nx_Lk = it.q.Lk;
-    nx_k0 = it.q.k0;
-    if (paged) {
-      nx_bt = a.block_tables + static_cast<int64_t>(it.q.s) * a.bt_stride;
-      nx_blk = entry(a, nx_bt, nx_lo < nx_ts ? nx_lo : nx_lo - nx_ts + nx_tlo);
-    }
+    nx_list = list_of(a, it, 0);
+    nx_at = it.at;
+    nx_left = uni(it.hi - it.lo);
+    nx_base = a.k + (paged ? 0 : static_cast<int64_t>(it.q.k0) * kv_rs) + h * SRC_ROWB;
+    const int last = it.hi - 1 < it.tl.ts ? it.hi - 1 : it.hi - 1 - it.tl.ts + it.tl.tlo;
+    nx_last = uni(min(kKeys, it.q.Lk - last * kKeys) * kv_rs);
   };
-  // Source and readable bytes of the next tile's copies (0 bytes: zeros).
+  // Source and readable bytes of the next entry's copies (0 bytes: zeros).
   auto next_tile = [&](const uint8_t *&src, uint32_t &nrec) {
-    src = st_k;
+    src = st_base;
     nrec = 0;
-    const int at = st_pos++ & 63;
-    bad &= ~(1ull << at);
-    if (st_i >= st_end) {
-      if (!nx_queued) return;
+    if (st_left == 0 && nx_queued) {
       nx_queued = false;
-      nx_first = st_pos - 1;
-      st_i = nx_lo;
-      st_end = nx_hi;
-      st_run = 0;
-      st_ts = nx_ts;
-      st_tlo = nx_tlo;
-      st_Lk = nx_Lk;
-      st_bt = nx_bt;
-      st_blk = nx_blk;
-      st_base = static_cast<int64_t>(nx_k0) * kv_rs + h * SRC_ROWB;
+      nx_first = st_pos;
+      st_list = nx_list;
+      st_l = 0;
+      st_left = nx_left;
+      st_at = nx_at;
+      st_chunk = 0;
+      st_base = nx_base;
+      st_last = nx_last;
     }
-    if (st_run == 0) {
-      KernArgs &a = *kernel_args();
-      auto tile_at = [&](int i) { return i < st_ts ? i : i - st_ts + st_tlo; };
-      const int tile = tile_at(st_i);
-      st_key = tile * kKeys;
-      const int list = (st_i < st_ts ? min(st_ts, st_end) : st_end) - st_i;  // tiles in a row of the list
-      if (paged) {
-        const int tiles_per_blk = a.block_size / kKeys;
-        const int in_blk = tile - small_div(tile, tiles_per_blk) * tiles_per_blk;
-        st_run = min(list, tiles_per_blk - in_blk);
-        st_ok = st_blk >= 0 && st_blk < a.num_blocks;
-        st_k = a.k + (static_cast<int64_t>(st_ok ? st_blk : 0) * a.block_size + in_blk * kKeys) * kv_rs + h * SRC_ROWB;
-        if (st_i + st_run < st_end) st_blk = entry(a, st_bt, tile_at(st_i + st_run));  // used a run from now
-      } else {
-        st_run = list;
-        st_ok = true;
-        st_k = a.k + st_base + static_cast<int64_t>(st_key) * kv_rs;
-      }
+    ++st_pos;
+    if (st_left == 0) return;
+    if (st_l == 64) {
+      ++st_chunk;
+      st_l = 0;
+      st_list = list_of(*kernel_args(), describe(st_at), st_chunk);
     }
-    if (st_ok) {
-      src = st_k;
-      nrec = static_cast<uint32_t>(min(kKeys, st_Lk - st_key) * kv_rs);
-    } else {
-      bad |= 1ull << at;
-    }
-    st_k += kKeys * kv_rs;
-    st_key += kKeys;
-    --st_run;
-    ++st_i;
+    const int at = __builtin_amdgcn_readlane(st_list, st_l);
+    src = st_base + static_cast<int64_t>(static_cast<uint32_t>(max(at, 0))) * static_cast<uint32_t>(kKeys * kv_rs);
+    nrec = at < 0 ? 0u : st_left == 1 ? st_last : static_cast<uint32_t>(kKeys * kv_rs);
+    ++st_l;
+    --st_left;
   };
   auto copy_k = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
     const u32x4 r = rsrc_words(src, nrec);
@@ -470,7 +476,7 @@ __device__ __forceinline__ void span_body() {
     for (int c = 0; c < COPS; ++c) dma16_opaque(dst + (rw * COPS + c) * 1024, r, src_k[c]);
   };
   auto copy_v = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
-    const u32x4 r = rsrc_words(src + (nrec ? v_minus_k : 0), nrec);
+    const u32x4 r = rsrc_words(src + v_minus_k, nrec);
 #pragma unroll
     for (int c = 0; c < COPS; ++c) dma16_opaque(dst + TILE_B + (rw * COPS + c) * 1024, r, src_v[c]);
   };
@@ -545,6 +551,7 @@ __device__ __forceinline__ void span_body() {
 
   // ---------------------------------------------------------------- items
   Item cur = describe(pos0);
+  bool careful = false;  // (see odd_values)
   queue(cur);
   // the item whose output is still in registers
   struct Done {
@@ -575,15 +582,10 @@ __device__ __forceinline__ void span_body() {
     }
     if (tiles && nx_queued) issue();
     const int p0 = nx_first;  // entry of its first tile
-    Item nxt{};
-    if (cur.live) {
-      nxt = describe(cur.next);
-      queue(nxt);
-    }
     if (tiles)
       while (st_pos < p0 + kAhead) issue();
-    // Q, then the output of the item before while it arrives.  (No live item:
-    // some row's.)
+    // Q, with it the next item's list, then the output of the item before.  (No
+    // live item: some row's.)
     KernArgs &a = *kernel_args();
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
@@ -594,6 +596,7 @@ __device__ __forceinline__ void span_body() {
 #pragma unroll
       for (int kk = 0; kk < NKK; ++kk) qf[qs][kk] = load16(qp + (8 * g + 32 * kk) * 2);
     }
+    if (cur.live) queue(describe(cur.next));
     if (done.live) {
       const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
       // lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
@@ -629,10 +632,10 @@ __device__ __forceinline__ void span_body() {
       const Tiles tl = cur.tl;
       const int lo = cur.lo, hi = cur.hi, n = hi - lo;
       const int P = q.Lk - q.Lq;
-      const int ta = small_div(min(r0, r_last), a.G), tb = small_div(min(r0 + QS * 16 - 1, r_last), a.G);
+      const int ta = uni(small_div(min(r0, r_last), a.G)), tb = uni(small_div(min(r0 + QS * 16 - 1, r_last), a.G));
       uint32_t slot = lds0 + (static_cast<unsigned>(p0) % SLOTS) * SLOT_B;  // of the tile computed next
       const int window = own_sgpr(a.window), sinks = own_sgpr(a.sinks);
-      const bool tree = window == 0, careful = cur.careful;
+      const bool tree = window == 0;
       if (tree) {
         // the masks of the tile's tokens, 32-bit words
         if constexpr (RW > 1) {  // the last item's have been read
@@ -656,6 +659,7 @@ __device__ __forceinline__ void span_body() {
       for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
+      asm volatile("" : "+v"(nx_list));
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
         m_use[qs] = kNegInf;
@@ -681,7 +685,7 @@ __device__ __forceinline__ void span_body() {
         } else {
           t1 = max(0, P) / kKeys;
         }
-        return Plain{t0 - tl.tlo + tl.ts, static_cast<unsigned>(max(0, t1 - t0))};
+        return Plain{uni(t0 - tl.tlo + tl.ts), static_cast<unsigned>(uni(max(0, t1 - t0)))};
       };
       // Keys of the tile at `key0` that row block qs of this lane sees: bit
       // 4 ks + r for key 16 ks + 4 g + r.
@@ -717,9 +721,16 @@ __device__ __forceinline__ void span_body() {
       uint32_t vis[QS];
       // The scores of keys that the rows do not see, replaced.  (Of a window, keys
       // past the sinks: one comparison of the distance to its first key.)
+      auto missing = [&](int key0) -> bool {  // the tile's page
+        KernArgs &a = *kernel_args();
+        if (!paged) return false;
+        const int e = small_div(key0 / kKeys, a.block_size / kKeys);
+        const int blk = e < a.max_blocks ? ld_const(a.block_tables + q.s * a.bt_stride + e) : -1;
+        return blk < 0 || blk >= a.num_blocks;
+      };
       auto mask_tile = [&](int i, bool live) {
         const int key0 = key_of(i);
-        if (!live || ((bad >> ((p0 + i - lo) & 63)) & 1)) {
+        if (!live || (bad_seen && missing(key0))) {
 #pragma unroll
           for (int qs = 0; qs < QS; ++qs) {
             vis[qs] = 0;
@@ -902,7 +913,7 @@ __device__ __forceinline__ void span_body() {
           asm volatile("" ::: "memory");
           scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
-          const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && bad == 0;
+          const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && !bad_seen;
           if (!whole_tile) mask_tile(i, true);
           next_tile(src, nrec);
           copy_k(slot, src, nrec);
@@ -939,11 +950,11 @@ __device__ __forceinline__ void span_body() {
           constexpr bool FIRST = decltype(first_tag)::value;
           unhoist();
           if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
-          const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && bad == 0;
+          const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && !bad_seen;
           if (!whole_tile) mask_tile(i, wave_live);
           pend = check(alpha);
           // (for all of the workgroup's waves alike)
-          if (careful && !(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && bad == 0) && odd_values(slot)) {
+          if (careful && !(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && !bad_seen) && odd_values(slot)) {
             // o is brought up to date before the odd values join it
             if constexpr (!FIRST) {
 #pragma unroll
@@ -1086,8 +1097,8 @@ __device__ __forceinline__ void span_body() {
         wait_vmcnt<0>();
         wait_lgkmcnt0();
         if constexpr (RW > 1) raw_barrier();
-        st_i = st_end = 0;
-        cur.careful = true;
+        st_left = 0;
+        careful = true;
         queue(cur);
         done.live = false;
         continue;
@@ -1096,7 +1107,8 @@ __device__ __forceinline__ void span_body() {
       done = Done{true, whole, q.q0, r0, r_last, ((2 * w_of + (lo > 0 ? 0 : 1)) * RW + rw) * QS};
       if (!whole) (lo > 0 ? desc0 : desc1) = int4{q.s, cur.rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
     }
-    cur = nxt;
+    cur = describe(cur.next);
+    careful = false;
   }
   if (ranges && rw == 0 && lane == 0) {
     int4 *d = kernel_args()->part_desc + 2 * w_of;
@@ -1266,6 +1278,9 @@ int run(const char *what, SpanArgs a, int head_dim, int64_t max_rows, int q_dtyp
     if (a.block_size <= 0 || a.block_size % kKeys != 0 || a.block_size > 1 << 26)
       return fail(NQ_EUNSUPPORTED, "%s: block_size %d must be a multiple of 32", what, a.block_size);
     if (a.max_blocks <= 0 || a.bt_stride < a.max_blocks) return fail(NQ_EINVAL, "%s: block table width", what);
+    // a tile's place in the pool is an int
+    if (static_cast<int64_t>(a.num_blocks) * (a.block_size / kKeys) > 0x7fffffff)
+      return fail(NQ_EINVAL, "%s: a pool of %d pages of %d tokens", what, a.num_blocks, a.block_size);
   }
   if (a.q_rs % 16 || a.q_hs % 16 || !aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || a.kv_rs % 16 ||
       a.o_rs % 8 || a.o_hs % 8 || !aligned(a.out, 8))
