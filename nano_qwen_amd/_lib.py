@@ -115,9 +115,10 @@ _SIGS = {
                                   c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                   POINTER(c_int64), c_void_p]),
     "nq_window_decode": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
-                                 c_int, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int,
-                                 c_int64, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
-                                 c_void_p, c_int64, POINTER(c_int64), c_void_p]),
+                                 c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p,
+                                 c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, c_float, c_int, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64),
+                                 c_void_p]),
     "nq_copy_kv_blocks": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
                                   c_void_p]),
     "nq_commit_tree": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p,

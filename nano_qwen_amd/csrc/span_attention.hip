@@ -78,6 +78,12 @@ struct SpanArgs {
   float scale_log2;
   const float *k_scale;
   const float *v_scale;
+  // Decode: the new token's rows to store [num_seqs, Hkv, D] (null: none), of type new_dtype.
+  const uint8_t *k_new;
+  const uint8_t *v_new;
+  int64_t kn_rs, vn_rs;  // bytes
+  const int32_t *slot_mapping;
+  int new_dtype;
   // Equal ranges: n_ranges per kv head (0: one item per workgroup), the partial
   // outputs of range w's slots 2 w and 2 w + 1 (fp32, normalised, as the lanes
   // hold them), their rows' log2-sum-exp, and what they are.
@@ -109,7 +115,8 @@ struct Shape {
   static constexpr int SEQS = 256;  // sequences whose bounds are kept in LDS
   // ring, masks, flags of odd tiles, sequences' bounds and positions
   static constexpr int MASK_AT = RING_B, ODD_AT = MASK_AT + (TOKENS * MASK_WORDS * 4 + 15) / 16 * 16,
-                       SEQ_AT = ODD_AT + 128, POS_AT = SEQ_AT + SEQS * 16, LDS_B = POS_AT + SEQS * 8;
+                       SEQ_AT = ODD_AT + 128, POS_AT = SEQ_AT + SEQS * 16, NEW_AT = POS_AT + SEQS * 8,
+                       LDS_B = NEW_AT + (RW == 1 ? 2 * SRC_ROWB : 0);  // (the new token's K and V rows)
   static constexpr int NKK = D / 32, NJ = D / 16;
   static_assert(COPS >= 1, "every wave copies");
 };
@@ -908,9 +915,73 @@ __device__ __forceinline__ void span_body() {
       float alpha[QS];
       if constexpr (RW == 1) {
         const Plain plain = plain_of(ta, tb);
+        // The new token: the piece that holds the sequence's last tile (or the
+        // item without tiles) stores its rows, and takes them from there for the
+        // tile, when its cache row is the one they go to: the store and the
+        // attention need no order.
+        uint8_t *const lds_new = smem + S::NEW_AT;
+        int new_row = -1;  // of the last tile
+        if (a.k_new && hi == tl.n) {
+          const int slot_of = ld_const(a.slot_mapping + q.s), have = ld_const(a.cu_k + q.s);
+          if (n > 0 && have == q.Lk) {
+            const int at = q.Lk - 1, e = small_div(at / kKeys, a.block_size / kKeys);
+            const int blk = e < a.max_blocks ? ld_const(a.block_tables + q.s * a.bt_stride + e) : -1;
+            if (blk >= 0 && blk < a.num_blocks &&
+                slot_of == static_cast<int64_t>(blk) * a.block_size + (at - e * a.block_size))
+              new_row = at % kKeys;
+          }
+          constexpr int NC = D / 8;  // lane l: elements 8 c .. of K (l < NC) or V
+          const bool is_v = lane >= NC;
+          const int c = is_v ? lane - NC : lane;
+          if (lane < 2 * NC) {
+            const uint8_t *row = is_v ? a.v_new + q.s * a.vn_rs : a.k_new + q.s * a.kn_rs;
+            uint8_t *cache = const_cast<uint8_t *>(is_v ? a.v : a.k) + slot_of * a.kv_rs + h * SRC_ROWB;
+            const bool stored = slot_of >= 0 && slot_of < static_cast<int64_t>(a.num_blocks) * a.block_size;
+            if constexpr (FP8) {
+              float x[8];
+              if (a.new_dtype == NQ_F32) {
+                const float *f = reinterpret_cast<const float *>(row) + h * D + 8 * c;
+                const f32x4 w0 = *reinterpret_cast<const f32x4 *>(f), w1 = *reinterpret_cast<const f32x4 *>(f + 4);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                  x[t] = w0[t];
+                  x[4 + t] = w1[t];
+                }
+              } else {
+                const u32x4 w = load16(row + (h * D + 8 * c) * 2);
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                  const uint16_t b = static_cast<uint16_t>(w[t >> 1] >> (16 * (t & 1)));
+                  x[t] = a.new_dtype == NQ_F16 ? F16::to_float(b) : BF16::to_float(b);
+                }
+              }
+              const float inv = 1.0f / (is_v ? a.v_scale : a.k_scale)[h];
+              const u32x2 codes{fp8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                                fp8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
+              if (stored) *reinterpret_cast<u32x2 *>(cache + 8 * c) = codes;
+              *reinterpret_cast<u32x2 *>(lds_new + (is_v ? SRC_ROWB : 0) + 8 * c) = codes;
+            } else {
+              const u32x4 w = load16(row + (h * D + 8 * c) * 2);
+              if (stored) store16(cache + 16 * c, w);
+              *reinterpret_cast<u32x4 *>(lds_new + (is_v ? SRC_ROWB : 0) + 16 * c) = w;
+            }
+          }
+          wave_lds_sync();
+        }
+        // the row over the one that was copied, a 16-byte piece per lane
+        auto patch = [&](uint32_t tile, bool is_v) {
+          if (lane < S::LPR) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(lds_new + (is_v ? SRC_ROWB : 0) + 16 * lane);
+            const int sw = FP8 ? swz8<D>(new_row) : is_v ? swz_v(new_row) : swz_k(new_row);
+            lds_store_b128(tile + (is_v ? TILE_B : 0) + new_row * SRC_ROWB + ((lane ^ sw) << 4), w);
+          }
+          wave_lds_sync();
+        };
         for (int i = lo; i < hi; ++i) {
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // K of this tile (younger: its V and the tiles after it)
           asm volatile("" ::: "memory");
+          const bool patched = new_row >= 0 && i == tl.n - 1;
+          if (patched) patch(slot, false);
           scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
           const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && !bad_seen;
@@ -922,6 +993,7 @@ __device__ __forceinline__ void span_body() {
           for (int t = 0; t < 4; ++t) pb[0][t] = p_unit(0, t);
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
           asm volatile("" ::: "memory");
+          if (patched) patch(slot, true);
           if (careful && !whole_tile && odd_values(slot)) {
             poison(slot);
             clean(slot);
@@ -1417,10 +1489,11 @@ extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_
              q_dtype, kv_dtype, workspace, workspace_bytes, need, stream);
 }
 
-extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
-                                const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, void *k_cache,
+                                void *v_cache, const int32_t *block_tables, int64_t bt_stride,
                                 int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
-                                void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
+                                const void *k_new, int64_t k_new_row_stride, const void *v_new,
+                                int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
                                 int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
                                 float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
                                 const float *v_scale, const void *gate, int64_t gate_batch_stride,
@@ -1429,6 +1502,15 @@ extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q
   const char *what = "window_decode";
   if (window <= 0 || num_sinks < 0) return fail(NQ_EINVAL, "%s: window %d, sinks %d", what, window, num_sinks);
   if (batch > 0 && !block_tables) return fail(NQ_EINVAL, "%s: null pointer", what);
+  const int64_t new_size = elem_size(new_dtype), row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (k_new) {
+    if (!v_new || !slot_mapping) return fail(NQ_EINVAL, "%s: null v_new or slot_mapping", what);
+    if (new_size == 0 || new_dtype == NQ_FP8_E4M3 || (kv_dtype != NQ_FP8_E4M3 && new_dtype != kv_dtype))
+      return fail(NQ_EUNSUPPORTED, "%s: new rows of dtype %d into a cache of dtype %d", what, new_dtype, kv_dtype);
+    if (k_new_row_stride < row || v_new_row_stride < row || (k_new_row_stride * new_size) % 16 ||
+        (v_new_row_stride * new_size) % 16 || !aligned(k_new, 16) || !aligned(v_new, 16))
+      return fail(NQ_EINVAL, "%s: k_new/v_new rows must be 16-byte aligned [Hkv, D] rows", what);
+  }
   SpanArgs a{};
   a.q = static_cast<const uint8_t *>(q);
   a.q_rs = q_batch_stride * 2;
@@ -1456,6 +1538,14 @@ extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q
   a.num_seqs = batch;
   a.window = std::min(window, 1 << 28);
   a.sinks = std::min(num_sinks, 1 << 28);
+  if (k_new) {
+    a.k_new = static_cast<const uint8_t *>(k_new);
+    a.v_new = static_cast<const uint8_t *>(v_new);
+    a.kn_rs = k_new_row_stride * new_size;
+    a.vn_rs = v_new_row_stride * new_size;
+    a.slot_mapping = slot_mapping;
+    a.new_dtype = new_dtype;
+  }
   a.scale_log2 = softmax_scale * kLog2e;
   a.k_scale = k_scale;
   a.v_scale = v_scale;

@@ -22,7 +22,8 @@ from __future__ import annotations
 import torch
 
 from .. import kernels
-from ..utils.context import get_context, reset_context, set_context
+from ..utils.context import get_context, reset_context, set_context, set_tree_context
+from .sequence import Sequence
 
 
 class ModelRunner:
@@ -53,6 +54,7 @@ class ModelRunner:
         self.graph_bs = []
         self.graph_pool = None
         self.graph_vars = None
+        self.tree = None
         # MRV2-style persistent batch: batch_idx -> request slot, and the last
         # sampled token of every slot (engine/model_runner.py:100-106).
         self.sampled_token_ids_gpu = torch.zeros(max_num_seqs, dtype=torch.int64, device=self.device)
@@ -249,6 +251,119 @@ class ModelRunner:
         block_tables = self.prepare_block_tables(seqs)
         set_context(False, slot_mapping=slot_mapping, context_lens=context_lens, block_tables=block_tables)
         return input_ids, positions
+
+    # ---------------------------------------------- trees of drafted tokens
+    # (these and the pages' moves below have no counterpart in the reference)
+    def prepare_tree(self, seqs, drafts, parents):
+        """Inputs and context of a step that verifies a tree of drafted tokens behind every sequence.
+
+        A sequence's last token (not in the cache yet, as before a decode step) is its tree's root, node 0;
+        ``drafts[i]`` are the tokens of its nodes 1, 2, ... and ``parents[i]`` their parents, indices below their
+        own.  Node j goes to position ``len(seq) - 1 + j`` of the cache, for which the block table has to have
+        room, and has the position of its depth.  Returns ``(input_ids, positions)`` of all nodes; the model then
+        runs as in a prefill, and ``commit_tree`` ends the step."""
+        input_ids, positions, slots, all_parents = [], [], [], []
+        cu_q, cu_k = [0], [0]
+        bs = self.block_size
+        for seq, tokens, up in zip(seqs, drafts, parents, strict=True):
+            if len(tokens) != len(up):
+                raise ValueError(f"prepare_tree: {len(tokens)} drafted tokens, {len(up)} parents")
+            base, n = len(seq) - 1, len(tokens) + 1
+            if base + n > len(seq.block_table) * bs:
+                raise ValueError(f"prepare_tree: {base + n} tokens in {len(seq.block_table)} blocks of {bs}")
+            depth = [0]
+            for i, p in enumerate(up, 1):
+                if not 0 <= p < i:
+                    raise ValueError(f"prepare_tree: node {i} has parent {p}")
+                depth.append(depth[p] + 1)
+            input_ids += [seq.last_token, *tokens]
+            positions += [base + x for x in depth]
+            slots += [seq.block_table[p // bs] * bs + p % bs for p in range(base, base + n)]
+            all_parents.append([-1, *up])
+            cu_q.append(cu_q[-1] + n)
+            cu_k.append(cu_k[-1] + base + n)
+        max_q = max(len(p) for p in all_parents)
+        max_k = max(b - a for a, b in zip(cu_k, cu_k[1:]))
+        mask = kernels.tree_masks(all_parents)
+        mask = (mask.pin_memory() if self._pin else mask).to(self.device, non_blocking=True)
+        input_ids = self._to_device(input_ids, torch.int64)
+        cu_q, cu_k = self._to_device(cu_q, torch.int32), self._to_device(cu_k, torch.int32)
+        tables = self.prepare_block_tables(seqs)
+        self.tree = dict(tokens=input_ids, parents=self._to_device([p for t in all_parents for p in t], torch.int32),
+                         cu_q=cu_q, cu_k=cu_k, max_q=max_q, tables=tables)
+        set_tree_context(cu_q, cu_k, max_q, max_k, self._to_device(slots, torch.int32), tables, mask)
+        return input_ids, self._to_device(positions, torch.int64)
+
+    def commit_tree(self, target_tokens):
+        """Ends the step that ``prepare_tree`` began: ``target_tokens`` (int64, one per node) is what the model
+        chose after each node.  The accepted paths' keys and values move to where the sequences go on, in every
+        layer; returns ``kernels.commit_tree``'s ``(path, num_accepted, next_tokens)``, on the device.
+        ``accept_tree`` brings the sequences up to date."""
+        t = self.tree
+        return kernels.commit_tree(self.kv_cache, t["tables"], t["cu_q"], t["cu_k"], t["max_q"], t["parents"],
+                                   t["tokens"], target_tokens)
+
+    def accept_tree(self, seqs, drafts, path, num_accepted, next_tokens):
+        """Appends what ``commit_tree`` accepted, and the token after it, to the sequences (waits for the device)."""
+        for seq, tokens, p, n, last in zip(seqs, drafts, path.tolist(), num_accepted.tolist(), next_tokens.tolist()):
+            for node in p[1:n]:
+                seq.append_token(tokens[node - 1])
+            seq.append_token(last)
+
+    # ------------------------------------------------------ pages of the pool
+    def copy_blocks(self, src, dst, num_tokens=None):
+        """Pages ``src`` to pages ``dst`` (lists of ids) in every layer, in one launch; ``num_tokens``: the first
+        tokens of each only.  A page that is written may appear in no other pair."""
+        if len(src) != len(dst) or (num_tokens is not None and len(num_tokens) != len(src)):
+            raise ValueError(f"copy_blocks: {len(src)} pages to {len(dst)}")
+        if len(set(dst)) != len(dst) or set(dst) & set(src):
+            raise ValueError("copy_blocks: a page that is written appears in another pair")
+        blocks = self.kv_cache.shape[2]
+        if any(not 0 <= b < blocks for b in (*src, *dst)):
+            raise ValueError(f"copy_blocks: a page outside the pool of {blocks}")
+        if src:
+            up = [self._to_device(x, torch.int32) for x in (src, dst)]
+            kernels.copy_kv_blocks(self.kv_cache, *up,
+                                   None if num_tokens is None else self._to_device(num_tokens, torch.int32))
+
+    def fork(self, seqs, new_blocks):
+        """A continuation of every sequence with a cache of its own: full pages are shared, the next tokens go to
+        the page ``new_blocks[i]``, to which a partly filled last page is copied.  Returns the new sequences; who
+        owns which page is the caller's to count."""
+        children, src, dst, filled = [], [], [], []
+        for seq, block in zip(seqs, new_blocks, strict=True):
+            full, rows = divmod(len(seq) - 1, self.block_size)    # the last token is not in the cache yet
+            children.append(Sequence(seq.token_ids, [*seq.block_table[:full], block], seq.num_cached_tokens,
+                                     seq.num_scheduled_tokens))
+            if rows:
+                src.append(seq.block_table[full])
+                dst.append(block)
+                filled.append(rows)
+        self.copy_blocks(src, dst, filled)
+        return children
+
+    def compact(self, seqs):
+        """Moves the pages that ``seqs`` (all sequences of the pool) use to the pool's first ids, in one launch, and
+        their block tables with them; returns how many pages are in use."""
+        used = sorted({b for seq in seqs for b in seq.block_table if b >= 0})
+        free = sorted(set(range(len(used))) - set(used))
+        moves = dict(zip([b for b in used if b >= len(used)], free, strict=True))
+        self.copy_blocks(list(moves), list(moves.values()))
+        for seq in seqs:
+            seq.block_table = [moves.get(b, b) for b in seq.block_table]
+        return len(used)
+
+    def release_window_blocks(self, seq, window, num_sinks=0):
+        """Takes the pages out of the sequence's table (-1) that no token from its last one on sees through a
+        ``window`` with ``num_sinks`` sinks, and returns their ids.  Of layers with several windows, the largest
+        counts; layers without one need every page."""
+        first = max(0, len(seq) - window)    # what the last token sees
+        freed = []
+        for i in range(-(-num_sinks // self.block_size), first // self.block_size):
+            if seq.block_table[i] >= 0:
+                freed.append(seq.block_table[i])
+                seq.block_table[i] = -1
+        return freed
 
     # ------------------------------------------------------- graph capture
     @torch.inference_mode()

@@ -816,6 +816,29 @@ def tree_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q
     return out
 
 
+def tree_masks(parents, words=None):
+    """The masks of trees whose nodes see their ancestors and themselves: int64 ``[T, words]`` on the CPU.
+
+    ``parents``: for each tree the parent of every node, an index below the node's own (the root's, node 0's, is
+    ignored).  ``words``: 64-bit words per node, by default what the largest tree needs.
+    """
+    most = max((len(p) for p in parents), default=0)
+    words = max(1, -(-most // 64)) if words is None else words
+    if most > 64 * words:
+        raise ValueError(f"tree_masks: {most} nodes in {words} words")
+    rows, full = [], (1 << 64) - 1
+    for tree in parents:
+        seen = []
+        for i, p in enumerate(tree):
+            if i and not 0 <= p < i:
+                raise ValueError(f"tree_masks: node {i} has parent {p}")
+            seen.append(1 << i | (seen[p] if i else 0))
+        for m in seen:
+            word = [m >> 64 * w & full for w in range(words)]
+            rows.append([x - (1 << 64) if x >> 63 else x for x in word])
+    return torch.tensor(rows, dtype=torch.int64).reshape(len(rows), words)
+
+
 def window_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, window,
                    num_sinks=0, block_table=None, k_scale=None, v_scale=None, out=None, gate=None):
     """``varlen_prefill`` (causal) where the token at position p sees the ``window`` tokens up to itself and the
@@ -859,7 +882,7 @@ def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale
     sequence's first ``num_sinks``.
 
     ``q [B, 1, Hq, D]`` (or ``[B, Hq, D]``); returns ``out`` shaped like ``q``.  With ``k, v [B, Hkv, D]`` and
-    ``slot_mapping [B]`` the new token is stored first, as ``store_kvcache`` stores it.
+    ``slot_mapping [B]`` the new token is stored in the same launch, on the terms of ``paged_decode``.
     """
     what = "window_decode"
     dev = _check_one_device(what, q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out, gate, k, v,
@@ -876,11 +899,20 @@ def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale
     qa, oa = _rows_of(what, "q", q, shape, q.dtype), _rows_of(what, "out", out, shape, q.dtype)
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, shape, q.dtype)
     scales = _scale_args(what, k_cache.dtype, hkv, k_scale, v_scale)
+    new = (None, 0, None, 0, None, -1)
     if k is not None:
-        store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        if v is None or slot_mapping is None or slot_mapping.dtype != torch.int32 or slot_mapping.numel() != B or \
+                not slot_mapping.is_contiguous():
+            raise RuntimeError(f"{what}: k needs v and a contiguous int32 slot_mapping [B]")
+        kv_shape = torch.Size((B, hkv, d))
+        rows = [_rows_of(what, name, t, kv_shape, k.dtype) for name, t in (("k", k), ("v", v))]
+        if any(r[2] != d for r in rows) and hkv > 1:
+            raise RuntimeError(f"{what}: k and v must be [B, Hkv, D] with contiguous heads")
+        new = (rows[0][0], rows[0][1] if B > 1 else hkv * d, rows[1][0], rows[1][1] if B > 1 else hkv * d,
+               slot_mapping.data_ptr(), dtype_code(k.dtype))
     _launch_span(what, lib().nq_window_decode, dev, (
         *qa, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], cache_seqlens.data_ptr(), int(window), int(num_sinks), *oa, B, hq, hkv, d, bs, nb,
+        block_table.shape[1], cache_seqlens.data_ptr(), int(window), int(num_sinks), *new, *oa, B, hq, hkv, d, bs, nb,
         float(softmax_scale), dtype_code(q.dtype), dtype_code(k_cache.dtype), *scales, *ga))
     return out
 
@@ -979,5 +1011,5 @@ def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
 
 __all__ = ["store_kvcache", "paged_decode", "varlen_prefill", "prepare_decode", "decode_plan", "qk_norm_rope_store",
            "output_gate", "gdn_decode", "gdn_prefill", "gated_rmsnorm", "gdn_conv1d", "tree_attention",
-           "window_prefill", "window_decode", "copy_kv_blocks", "commit_tree", "decode_workspace",
+           "tree_masks", "window_prefill", "window_decode", "copy_kv_blocks", "commit_tree", "decode_workspace",
            "prefill_workspace", "release_workspaces", "decode_schedule", "_lib"]

@@ -8,6 +8,10 @@ fp8 extension (absent from the reference): when the runner binds
 ``float8_e4m3fn`` caches it also binds ``k_scale`` / ``v_scale`` (float32
 ``[Hkv]``, one scale per kv head of this layer); the store quantizes with
 them and both attention kernels dequantize in registers.
+
+Windows and trees (absent from the reference): a layer with a ``window`` sees
+that many tokens up to the query's own, and the sequence's first ``num_sinks``;
+under a ``TreeContext`` a layer without one attends to trees of drafted tokens.
 """
 from __future__ import annotations
 
@@ -33,14 +37,20 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 
 class Attention(nn.Module):
 
-    def __init__(self, num_heads, head_dim, scale, num_kv_heads):
+    def __init__(self, num_heads, head_dim, scale, num_kv_heads, window: int | None = None, num_sinks: int = 0):
         super().__init__()
+        if window is not None and (window < 1 or num_sinks < 0):
+            raise ValueError(f"Attention: window {window}, num_sinks {num_sinks}")
+        if window is None and num_sinks:
+            raise ValueError("Attention: num_sinks without a window")
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = None
+        self.window = window
+        self.num_sinks = num_sinks
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_stored: bool = False,
                 gate: torch.Tensor | None = None):
@@ -54,6 +64,9 @@ class Attention(nn.Module):
         inside the decode kernel's store, or one in-place pass after prefill.
         """
         context = get_context()
+        tree_mask = getattr(context, "tree_mask", None)
+        if self.window is not None or tree_mask is not None:
+            return self._forward_span(context, tree_mask, q, k, v, kv_stored, gate)
         k_cache, v_cache = self.k_cache, self.v_cache
         store = k_cache.numel() and v_cache.numel() and not kv_stored
         if store and not context.is_prefill:
@@ -85,3 +98,26 @@ class Attention(nn.Module):
                                      block_table=context.block_tables, softmax_scale=self.scale,
                                      k_scale=self.k_scale, v_scale=self.v_scale, gate=gate)
         return o
+
+    def _forward_span(self, context, tree_mask, q, k, v, kv_stored, gate):
+        """``forward`` of a layer with a window, or of trees of drafted tokens."""
+        if tree_mask is not None and self.window is not None:
+            raise RuntimeError("Attention: trees of drafted tokens are not supported in layers with a window")
+        k_cache, v_cache = self.k_cache, self.v_cache
+        store = k_cache.numel() and v_cache.numel() and not kv_stored
+        if not context.is_prefill:
+            new = dict(k=k, v=v, slot_mapping=context.slot_mapping) if store else {}
+            return kernels.window_decode(q.unsqueeze(1), k_cache, v_cache, context.context_lens, context.block_tables,
+                                         self.scale, self.window, self.num_sinks, self.k_scale, self.v_scale, gate=gate,
+                                         **new)
+        if store:
+            store_kvcache(k, v, k_cache, v_cache, context.slot_mapping, self.k_scale, self.v_scale)
+        k_scale = v_scale = None
+        if context.block_tables is not None:    # prefix cache, or trees
+            k, v = k_cache, v_cache
+            k_scale, v_scale = self.k_scale, self.v_scale
+        args = (q, k, v, context.cu_seqlens_q, context.cu_seqlens_k, context.max_seqlen_q, context.max_seqlen_k, self.scale)
+        if tree_mask is not None:
+            return kernels.tree_attention(*args, context.block_tables, tree_mask, k_scale, v_scale, gate=gate)
+        return kernels.window_prefill(*args, self.window, self.num_sinks, block_table=context.block_tables,
+                                      k_scale=k_scale, v_scale=v_scale, gate=gate)
