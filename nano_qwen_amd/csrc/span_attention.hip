@@ -1198,66 +1198,87 @@ void span_attention_kernel(const SpanArgs a) {
 
 // Merge of the items that ranges cut: workgroup (range, part) takes the item
 // whose first piece lies in the range's slot 1; its other pieces are the slots
-// 0 of the next ranges, up to the one marked last.
+// 0 of the next ranges, up to the one marked last.  A wave takes J 16-dim
+// blocks of one row block, kMergeUnroll pieces in flight: the chain is two round
+// trips to memory and one per eight pieces.
+constexpr int kMergeUnroll = 8;
+template <class S>
+struct MergeShape {
+  static constexpr int J = S::NJ >= 16 ? 4 : S::RW == 1 ? 2 : 4;
+  static constexpr int WAVES = S::RW * S::QS * S::NJ / J;
+  static_assert(WAVES % 4 == 0, "workgroups of four waves");
+};
 template <class T, class S>
 __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
-  constexpr int NJ = S::NJ, M = S::M, kUnroll = 8;
+  constexpr int NJ = S::NJ, M = S::M, J = MergeShape<S>::J;
   const int w = blockIdx.x, h = w / a.n_ranges, w_end = (h + 1) * a.n_ranges;
-  const int4 d = a.part_desc[2 * w + 1];
-  if (d.z == kPieceNone) return;
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const int e = blockIdx.y * 4 + (threadIdx.x >> 6);  // (row block, 16-dim block)
-  const int unit = e / NJ, j = e % NJ;
+  const int4 d = a.part_desc[2 * w + 1];
+  auto kind = [&](int b) { return a.part_desc[2 * min(b + lane, w_end - 1)].z; };
+  int next = kind(w + 1);
+  if (d.z == kPieceNone) return;
+  const int e = blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int unit = e / (NJ / J), j0 = e % (NJ / J) * J;
+  const Seq q = seq_of(a, d.x, true);
+  const int r = d.y * M + unit * 16 + m;
   int pieces = 1;
   for (int b = w + 1;; b += 64) {
-    const uint64_t last = __builtin_amdgcn_ballot_w64(b + lane < w_end && a.part_desc[2 * min(b + lane, w_end - 1)].z == kPieceLast);
+    const uint64_t last = __builtin_amdgcn_ballot_w64(b + lane < w_end && next == kPieceLast);
     if (last != 0) {
       pieces += static_cast<int>(__builtin_ctzll(last)) + 1;
       break;
     }
     if (b + 64 >= w_end) return;  // not reached: every cut item has a last piece
     pieces += 64;
+    next = kind(b + 64);
   }
-  const Seq q = seq_of(a, d.x, true);
-  const int r = d.y * M + unit * 16 + m;
   if (r >= q.Lq * a.G) return;
   float mx = kNegInf, W = 0.f;
-  f32x4 acc{0, 0, 0, 0};
-  for (int c = 0; c < pieces; c += kUnroll) {
-    float l[kUnroll];
-    f32x4 p[kUnroll];
+  f32x4 acc[J];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+  for (int j = 0; j < J; ++j) acc[j] = f32x4{0, 0, 0, 0};
+  for (int c = 0; c < pieces; c += kMergeUnroll) {
+    float l[kMergeUnroll];
+    f32x4 p[kMergeUnroll][J];
+#pragma unroll
+    for (int u = 0; u < kMergeUnroll; ++u) {
       l[u] = kNegInf;
       if (c + u < pieces) {
         const int64_t at = static_cast<int64_t>(2 * (w + c + u) + (c + u == 0 ? 1 : 0)) * S::RW * S::QS + unit;
         l[u] = a.part_l[at * 16 + m];
-        p[u] = reinterpret_cast<const f32x4 *>(a.part_o)[(at * NJ + j) * 64 + lane];
+#pragma unroll
+        for (int j = 0; j < J; ++j) p[u][j] = reinterpret_cast<const f32x4 *>(a.part_o)[(at * NJ + j0 + j) * 64 + lane];
       }
     }
     float mc = mx;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) mc = fmaxf(mc, l[u]);
+    for (int u = 0; u < kMergeUnroll; ++u) mc = fmaxf(mc, l[u]);
     const float mu = mc == kNegInf ? 0.f : mc;
     const float f = __builtin_amdgcn_exp2f(mx - mu);
     W *= f;
-    acc *= f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] *= f;
     mx = mc;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kMergeUnroll; ++u)
       if (l[u] != kNegInf) {
         const float x = __builtin_amdgcn_exp2f(l[u] - mu);
         W += x;
-        acc += p[u] * x;
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] += p[u][j] * x;
       }
   }
-  acc *= W > 0.f ? 1.0f / W : 0.f;
+  const float inv = W > 0.f ? 1.0f / W : 0.f;
   const int t = small_div(r, a.G), head = h * a.G + r - t * a.G;
-  uint8_t *op = a.out + static_cast<int64_t>(q.q0 + t) * a.o_rs + head * a.o_hs + 32 * j + 8 * g;
-  *reinterpret_cast<u32x2 *>(op) =
-      a.gate ? gate4<T>(acc, *reinterpret_cast<const u32x2 *>(a.gate + static_cast<int64_t>(q.q0 + t) * a.g_rs +
-                                                              head * a.g_hs + 32 * j + 8 * g))
-             : u32x2{T::pack2(acc[0], acc[1]), T::pack2(acc[2], acc[3])};
+  uint8_t *op = a.out + static_cast<int64_t>(q.q0 + t) * a.o_rs + head * a.o_hs + 32 * j0 + 8 * g;
+  const uint8_t *gp = a.gate + static_cast<int64_t>(q.q0 + t) * a.g_rs + head * a.g_hs + 32 * j0 + 8 * g;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const f32x4 v = acc[j] * inv;
+    *reinterpret_cast<u32x2 *>(op + 32 * j) =
+        a.gate ? gate4<T>(v, *reinterpret_cast<const u32x2 *>(gp + 32 * j))
+               : u32x2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
+  }
 }
 
 // ---------------------------------------------------------------- launch
@@ -1297,7 +1318,7 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
     span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(W * a.Hkv)), 64 * S::RW, S::LDS_B, stream>>>(a);
     const int rc = check_launch("span attention");
     if (rc != NQ_OK || W <= 1) return rc;
-    span_merge_kernel<T, S><<<dim3(static_cast<unsigned>(W * a.Hkv), S::RW * S::QS * S::NJ / 4), 256, 0, stream>>>(a);
+    span_merge_kernel<T, S><<<dim3(static_cast<unsigned>(W * a.Hkv), MergeShape<S>::WAVES / 4), 256, 0, stream>>>(a);
     return check_launch("span attention (merge)");
   }
   // Whole items, dealt out in turn to the workgroups that the chip holds at once

@@ -715,12 +715,17 @@ def gdn_conv1d(x, weight, conv_state, state_indices, cu_seqlens=None, out=None):
 # (no counterpart in the reference, whose attention is causal over the whole
 # context and whose pages never move)
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)    # (without the shim's check)
+
+
 def _check_one_device(what, first, *others):
-    require_cuda(first, *others, what=what)
-    dev = first.get_device()
+    dev = first.get_device()    # -1: not on a device
     for t in others:
         if t is not None and t.get_device() != dev:
+            require_cuda(first, *others, what=what)
             raise RuntimeError(f"{what}: tensors on several devices")
+    if dev < 0:
+        require_cuda(first, what=what)
     return dev
 
 
@@ -761,7 +766,7 @@ def _check_cu(what, n1, *tensors):
 def _launch_span(what, fn, device, args):
     """Calls ``fn(*args, workspace, bytes, need, stream)``, which asks once for a workspace of its size: the
     stream's own, or during a capture one of the graph's (whose replays may then overlap other calls)."""
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         with torch.cuda.device(device):
             return _launch_span(what, fn, device, args)
     key = device, raw_stream(device)
@@ -948,7 +953,7 @@ def copy_kv_blocks(kv_cache, src_blocks, dst_blocks, num_tokens=None):
     n = src_blocks.numel()
     args = (_id_list(what, "src_blocks", src_blocks, n), _id_list(what, "dst_blocks", dst_blocks, n),
             None if num_tokens is None else _id_list(what, "num_tokens", num_tokens, n))
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             return copy_kv_blocks(kv_cache, src_blocks, dst_blocks, num_tokens)
     check(lib().nq_copy_kv_blocks(kv_cache.data_ptr(), slabs, nb, bs, row, *args, n, raw_stream(dev)), what)
@@ -973,7 +978,7 @@ def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
     what = "commit_tree"
     dev = _check_one_device(what, kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, parents, tokens, target_tokens,
                             path, num_accepted)
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             return commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, parents, tokens,
                                target_tokens, path, num_accepted)
