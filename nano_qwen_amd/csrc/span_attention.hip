@@ -299,7 +299,7 @@ __device__ __forceinline__ void span_body() {
     pos1 = w < W ? static_cast<int>(static_cast<int64_t>(w + 1) * total / W) : 0;
   }
   // The range's two partial pieces, written for the merge when it is done.
-  int4 desc0{0, 0, kPieceNone, 0}, desc1{0, 0, kPieceNone, 0};
+  int cuts = 0;  // which of the range's two slots have been described
   // The first item from `at` (a position or a round) on that this workgroup has
   // to do something for (live: there is one).
   struct Item {
@@ -470,6 +470,9 @@ __device__ __forceinline__ void span_body() {
       ++st_chunk;
       st_l = 0;
       st_list = list_of(*kernel_args(), describe(st_at), st_chunk);
+      // (here, where the list is needed at once: a load that the compiler cannot
+      // see waited for on every path, it waits for in the loop, with the copies)
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     }
     const int at = __builtin_amdgcn_readlane(st_list, st_l);
     src = st_base + static_cast<int64_t>(static_cast<uint32_t>(max(at, 0))) * static_cast<uint32_t>(kKeys * kv_rs);
@@ -1177,15 +1180,21 @@ __device__ __forceinline__ void span_body() {
       }
       const bool whole = lo == 0 && hi == tl.n;
       done = Done{true, whole, q.q0, r0, r_last, ((2 * w_of + (lo > 0 ? 0 : 1)) * RW + rw) * QS};
-      if (!whole) (lo > 0 ? desc0 : desc1) = int4{q.s, cur.rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
+      if (!whole) {
+        const int at = lo > 0 ? 0 : 1;
+        cuts |= 1 << at;
+        if (rw == 0 && lane == 0)
+          kernel_args()->part_desc[2 * w_of + at] = int4{q.s, cur.rt, hi == tl.n ? kPieceLast : kPieceMore, 0};
+      }
     }
     cur = describe(cur.next);
     careful = false;
   }
   if (ranges && rw == 0 && lane == 0) {
     int4 *d = kernel_args()->part_desc + 2 * w_of;
-    d[0] = desc0;
-    d[1] = desc1;
+    const int4 none{0, 0, kPieceNone, 0};
+    if (!(cuts & 1)) d[0] = none;
+    if (!(cuts & 2)) d[1] = none;
   }
   wait_vmcnt<0>();  // no copy outlives the workgroup's LDS
 }
