@@ -721,8 +721,9 @@ int nq_copy_kv_blocks(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int
  * nodes), next_tokens the last one's target (-1 without nodes).
  * Then the row of position C + path[r] goes to position C + r, C =
  * cu_seqlens_k[s+1] - cu_seqlens_k[s] - nodes; positions without a page are
- * skipped.  target_tokens == NULL: path and num_accepted are inputs (indices
- * that rise; the path ends before one that does not).  At most 256 nodes.
+ * skipped.  parents, tokens, target_tokens and next_tokens all NULL: path and
+ * num_accepted are inputs (indices that rise; the path ends before one that
+ * does not).  At most 256 nodes.
  */
 int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int block_size, int64_t row_bytes,
                    const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,

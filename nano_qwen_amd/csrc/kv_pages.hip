@@ -239,8 +239,8 @@ extern "C" int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blo
   if (!block_tables || !cu_seqlens_q || !cu_seqlens_k || (max_seqlen_q > 0 && !path) || !num_accepted ||
       (num_slabs > 0 && num_blocks > 0 && !kv_cache))
     return fail(NQ_EINVAL, "commit_tree: null pointer");
-  if (target_tokens && (!next_tokens || (total_q > 0 && (!parents || !tokens))))
-    return fail(NQ_EINVAL, "commit_tree: null parents, tokens or next_tokens");
+  if (next_tokens ? total_q > 0 && (!parents || !tokens || !target_tokens) : parents || tokens || target_tokens)
+    return fail(NQ_EINVAL, "commit_tree: null parents, tokens, target_tokens or next_tokens");
   if (max_blocks_per_seq < 0 || bt_stride < max_blocks_per_seq) return fail(NQ_EINVAL, "commit_tree: block table width");
   if (row_bytes % 16 || !aligned(kv_cache, 16))
     return fail(NQ_EINVAL, "commit_tree: cache rows of %lld bytes must be 16-byte aligned", (long long)row_bytes);
@@ -263,7 +263,7 @@ extern "C" int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blo
   a.path = path;
   a.count = num_accepted;
   a.next = next_tokens;
-  a.given = target_tokens == nullptr;
+  a.given = next_tokens == nullptr;
   const int64_t units = std::max<int64_t>(1, (row_bytes / 16 * a.slabs + kCommitThreads - 1) / kCommitThreads);
   if (units > 0x7fffffff) return fail(NQ_EINVAL, "commit_tree: %lld columns", (long long)units);
   commit_tree_kernel<<<dim3(static_cast<unsigned>(units), num_seqs), kCommitThreads, 0,

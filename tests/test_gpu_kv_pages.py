@@ -124,3 +124,61 @@ def test_commit_given_paths_end_where_they_do_not_rise(cuda):
     assert same_bytes(dev, ref)
     kernels.commit_tree(dev, table, cu_q, cu_k, 6, path=i32([[0, 9, 4, 4, 5, 2]]), num_accepted=i32([99]))
     assert same_bytes(dev, ref)
+
+
+@pytest.mark.parametrize("most", [0, 7])
+def test_commit_without_nodes(cuda, most):
+    """A step in which no sequence has a node still answers for each of them."""
+    p = pool((2, 2, 4, 32, 1, 64), torch.bfloat16)
+    dev = p.to(cuda)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)    # noqa: E731
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    held = [torch.full((4096,), 77, dtype=torch.int32, device=cuda) for _ in range(8)]    # what new tensors then find
+    del held
+    path, count, nxt = kernels.commit_tree(dev, i32([[0], [1], [2]]), i32([0, 0, 0, 0]), i32([0, 9, 9, 30]), most,
+                                           i32([]), none, none)
+    assert path.tolist() == [[-1] * most] * 3 and count.tolist() == [0] * 3 and nxt.tolist() == [-1] * 3
+    assert same_bytes(dev, p)
+
+
+def test_captured_commit_and_copy(cuda):
+    """One graph that accepts a tree, moves its rows and copies its page, replayed over new drafts and pools."""
+    r = random.Random(4)
+    shape, pre, n = (2, 2, 6, 32, 2, 64), 40, 20
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)    # noqa: E731
+    dev = pool(shape, torch.float16).to(cuda)
+    table, cu_q, cu_k, src, dst = i32([[3, 1]]), i32([0, n]), i32([0, pre + n]), i32([1]), i32([4])
+    parents, tokens, targets = (torch.zeros(n, dtype=t, device=cuda) for t in (torch.int32, torch.int64, torch.int64))
+
+    def step():
+        got = kernels.commit_tree(dev, table, cu_q, cu_k, n, parents, tokens, targets)
+        kernels.copy_kv_blocks(dev, src, dst)
+        return got
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        tree = random_tree(r, n)
+        tok = [r.randrange(3) for _ in tree]
+        tgt = [r.randrange(3) for _ in tree]
+        for v in range(n):
+            kids = [j for j, q in enumerate(tree) if q == v]
+            if kids:
+                tgt[v] = tok[r.choice(kids)]
+        p = pool(shape, torch.float16, seed=turn)
+        ref = p.clone()
+        for x, y in ((parents, tree), (tokens, tok), (targets, tgt)):
+            x.copy_(torch.tensor(y))
+        dev.copy_(p)
+        graph.replay()
+        path, nxt = spans.accepted_path(tree, tok, tgt)
+        spans.move_rows(ref.view(torch.uint8), table[0].tolist(), pre, path)
+        ref[:, :, 4] = ref[:, :, 1]
+        assert out[0].tolist() == [path + [-1] * (n - len(path))] and out[1].tolist() == [len(path)]
+        assert out[2].tolist() == [nxt] and same_bytes(dev, ref), turn

@@ -417,3 +417,34 @@ def test_decode_stores_the_new_token(cuda, d, dtype, fp8, new_dtype):
         assert torch.equal(got, want)
         for x, y in ((a.k_dev, b.k_dev), (a.v_dev, b.v_dev)):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_captured_decode_stores_the_new_token(cuda):
+    """The fused store in a graph: new rows, slots and lengths at every replay, against the separate store."""
+    a, b = (Case([1] * 3, [255, 31, 90], 8, 2, 128, BF, block=32, seed=9).to(cuda) for _ in range(2))
+    k, v = (torch.zeros(3, 2, 128, dtype=BF, device=cuda) for _ in range(2))
+    slots, lens = (torch.zeros(3, dtype=torch.int32, device=cuda) for _ in range(2))
+
+    def step(c, **new):
+        return kernels.window_decode(c.q_dev, c.k_dev, c.v_dev, lens, c.table_dev, c.scale, 50, 2, **new)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    slots.fill_(-1)
+    with torch.cuda.stream(side):
+        step(a, k=k, v=v, slot_mapping=slots)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(a, k=k, v=v, slot_mapping=slots)
+    for turn, pos in enumerate([[255, 31, 90], [0, 32, 64], [254, 0, 63], [31, 31, 31]]):
+        k.normal_()
+        v.normal_()
+        lens.copy_(torch.tensor([p + 1 for p in pos]))
+        slots.copy_(torch.tensor([int(a.table[i, p // 32]) * 32 + p % 32 for i, p in enumerate(pos)]))
+        graph.replay()
+        kernels.store_kvcache(k, v, b.k_dev, b.v_dev, slots)
+        want = step(b)
+        assert torch.equal(out, want), turn
+        for x, y in ((a.k_dev, b.k_dev), (a.v_dev, b.v_dev)):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), turn
