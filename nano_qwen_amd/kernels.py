@@ -763,6 +763,11 @@ def _check_cu(what, n1, *tensors):
             raise RuntimeError(f"{what}: cu_seqlens must be contiguous int32 [sequences + 1]")
 
 
+def _int32(x):
+    """A window or number of sinks as the C int that means the same: beyond every sequence is beyond."""
+    return min(int(x), 0x7fffffff)
+
+
 def _launch_span(what, fn, device, args):
     """Calls ``fn(*args, workspace, bytes, need, stream)``, which asks once for a workspace of its size: the
     stream's own, or during a capture one of the graph's (whose replays may then overlap other calls)."""
@@ -875,7 +880,7 @@ def window_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
     _launch_span(what, lib().nq_window_prefill, dev, (
         *qa, k.data_ptr(), v.data_ptr(), kv_rs, tk, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-        int(max_seqlen_q), int(max_seqlen_k), *pa, int(window), int(num_sinks), *oa, n, tq, hq, hkv, d, bs,
+        int(max_seqlen_q), int(max_seqlen_k), *pa, _int32(window), _int32(num_sinks), *oa, n, tq, hq, hkv, d, bs,
         float(softmax_scale), dtype_code(q.dtype), dtype_code(k.dtype),
         *_scale_args(what, k.dtype, hkv, k_scale, v_scale), *ga))
     return out
@@ -917,7 +922,7 @@ def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale
                slot_mapping.data_ptr(), dtype_code(k.dtype))
     _launch_span(what, lib().nq_window_decode, dev, (
         *qa, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], cache_seqlens.data_ptr(), int(window), int(num_sinks), *new, *oa, B, hq, hkv, d, bs, nb,
+        block_table.shape[1], cache_seqlens.data_ptr(), _int32(window), _int32(num_sinks), *new, *oa, B, hq, hkv, d, bs, nb,
         float(softmax_scale), dtype_code(q.dtype), dtype_code(k_cache.dtype), *scales, *ga))
     return out
 

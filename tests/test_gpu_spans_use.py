@@ -448,3 +448,12 @@ def test_captured_decode_stores_the_new_token(cuda):
         assert torch.equal(out, want), turn
         for x, y in ((a.k_dev, b.k_dev), (a.v_dev, b.v_dev)):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), turn
+
+
+def test_windows_beyond_32_bits(cuda):
+    """A window (or sinks) that no int holds is one that every token sees through."""
+    c = Case([1, 1], [300, 40], 8, 2, 128, BF, block=32).to(cuda)
+    p = Case([40, 3], [0, 90], 8, 2, 128, BF, block=32).to(cuda)
+    for case, call in ((c, c.window_decode), (p, p.window_prefill)):
+        want = call(4096, 0)
+        assert torch.equal(call(2 ** 32 + 3, 0), want) and torch.equal(call(1, 2 ** 32 + 3), want)
