@@ -87,7 +87,7 @@ struct SpanArgs {
   // Equal ranges: n_ranges per kv head (0: one item per workgroup), the partial
   // outputs of range w's slots 2 w and 2 w + 1 (fp32, normalised, as the lanes
   // hold them), their rows' log2-sum-exp, and what they are.
-  int n_ranges;
+  int n_ranges, min_range;
   int stride;  // whole items: from a workgroup's item to its next
   float *part_o;
   float *part_l;
@@ -199,7 +199,14 @@ struct Cost {
   // one wave: Q and first-tile latency, in the time of a tile; more waves: the
   // same in their faster tiles
   static constexpr int kItem = S::RW == 1 ? 1 : 4;
-  static constexpr int kMinRange = 2;
+  // A range has at least kMinRange tiles, and enough that the longest item is cut
+  // into about kPieces.  Fewer pieces leave compute units idle, more are a longer
+  // merge: one tree of 16 rows behind 8192 tokens 58 us in ranges of 2 tiles (128
+  // pieces), 21 in ranges of 8; one of 64 rows 54 in ranges of 2, 34 of 8, 26 of
+  // 16; a decode of 1028 tokens 14.4 in ranges of 2, 15.3 of 4.
+  static constexpr int kMinRange = S::RW == 1 ? 2 : 8, kPieces = S::RW == 1 ? 32 : 16;
+  // What cutting costs, in the time of a tile: partials written, a second launch.
+  static constexpr int kCut = 20;
 };
 template <class S, class A>
 __device__ __forceinline__ int row_tiles(const A &a, const Seq &q) {
@@ -294,7 +301,7 @@ __device__ __forceinline__ void span_body() {
   int w_of = 0;  // the range's partials
   if (ranges) {
     w_of = h * n_ranges + w;
-    const int W = min(n_ranges, max(1, total / Cost<S>::kMinRange));
+    const int W = min(n_ranges, max(1, total / a0.min_range));
     pos0 = w < W ? static_cast<int>(static_cast<int64_t>(w) * total / W) : 0;
     pos1 = w < W ? static_cast<int>(static_cast<int64_t>(w + 1) * total / W) : 0;
   }
@@ -1209,7 +1216,9 @@ void span_attention_kernel(const SpanArgs a) {
 // whose first piece lies in the range's slot 1; its other pieces are the slots
 // 0 of the next ranges, up to the one marked last.  A wave takes J 16-dim
 // blocks of one row block, kMergeUnroll pieces in flight: the chain is two round
-// trips to memory and one per eight pieces.
+// trips to memory and one per eight pieces, or per 32 where SPREAD = 4 waves
+// share them and join through LDS.  Latency bounds it (5-7 us, half of that the
+// launch), or reading the partials: 11 us for trees of 32 nodes, 16 sequences.
 constexpr int kMergeUnroll = 8;
 template <class S>
 struct MergeShape {
@@ -1217,7 +1226,7 @@ struct MergeShape {
   static constexpr int WAVES = S::RW * S::QS * S::NJ / J;
   static_assert(WAVES % 4 == 0, "workgroups of four waves");
 };
-template <class T, class S>
+template <class T, class S, int SPREAD>
 __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
   constexpr int NJ = S::NJ, M = S::M, J = MergeShape<S>::J;
   const int w = blockIdx.x, h = w / a.n_ranges, w_end = (h + 1) * a.n_ranges;
@@ -1226,7 +1235,7 @@ __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
   auto kind = [&](int b) { return a.part_desc[2 * min(b + lane, w_end - 1)].z; };
   int next = kind(w + 1);
   if (d.z == kPieceNone) return;
-  const int e = blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6, e = SPREAD > 1 ? blockIdx.y : blockIdx.y * 4 + wave;
   const int unit = e / (NJ / J), j0 = e % (NJ / J) * J;
   const Seq q = seq_of(a, d.x, true);
   const int r = d.y * M + unit * 16 + m;
@@ -1241,18 +1250,18 @@ __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
     pieces += 64;
     next = kind(b + 64);
   }
-  if (r >= q.Lq * a.G) return;
+  const bool live = r < q.Lq * a.G;
   float mx = kNegInf, W = 0.f;
   f32x4 acc[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) acc[j] = f32x4{0, 0, 0, 0};
-  for (int c = 0; c < pieces; c += kMergeUnroll) {
+  for (int c = (SPREAD > 1 ? wave * kMergeUnroll : 0); c < pieces; c += SPREAD * kMergeUnroll) {
     float l[kMergeUnroll];
     f32x4 p[kMergeUnroll][J];
 #pragma unroll
     for (int u = 0; u < kMergeUnroll; ++u) {
       l[u] = kNegInf;
-      if (c + u < pieces) {
+      if (live && c + u < pieces) {
         const int64_t at = static_cast<int64_t>(2 * (w + c + u) + (c + u == 0 ? 1 : 0)) * S::RW * S::QS + unit;
         l[u] = a.part_l[at * 16 + m];
 #pragma unroll
@@ -1277,6 +1286,32 @@ __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
         for (int j = 0; j < J; ++j) acc[j] += p[u][j] * x;
       }
   }
+  if constexpr (SPREAD > 1) {
+    if (pieces > kMergeUnroll) {
+      __shared__ float states[SPREAD - 1][J * 4 + 2][64];
+      if (wave > 0) {
+        float(*const st)[64] = states[wave - 1];
+#pragma unroll
+        for (int i = 0; i < 4 * J; ++i) st[i][lane] = acc[i >> 2][i & 3];
+        st[4 * J][lane] = mx;
+        st[4 * J + 1][lane] = W;
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int u = 0; u < SPREAD - 1; ++u) {
+          const float mo = states[u][4 * J][lane], mn = fmaxf(mx, mo), mu = mn == kNegInf ? 0.f : mn;
+          const float f0 = __builtin_amdgcn_exp2f(mx - mu), f1 = __builtin_amdgcn_exp2f(mo - mu);
+          W = W * f0 + states[u][4 * J + 1][lane] * f1;
+#pragma unroll
+          for (int i = 0; i < 4 * J; ++i) acc[i >> 2][i & 3] = acc[i >> 2][i & 3] * f0 + states[u][i][lane] * f1;
+          mx = mn;
+        }
+      }
+    }
+    if (wave > 0) return;
+  }
+  if (!live) return;
   const float inv = W > 0.f ? 1.0f / W : 0.f;
   const int t = small_div(r, a.G), head = h * a.G + r - t * a.G;
   uint8_t *op = a.out + static_cast<int64_t>(q.q0 + t) * a.o_rs + head * a.o_hs + 32 * j0 + 8 * g;
@@ -1300,17 +1335,29 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
   const int64_t by_total = static_cast<int64_t>(a.total_q) * a.G / S::M + a.num_seqs;
   const int64_t items = std::min(by_total, a.num_seqs * ((max_rows + S::M - 1) / S::M));
   const int64_t slots = static_cast<int64_t>(device_cus()) * per_cu;
-  const int64_t max_cost = (static_cast<int64_t>(a.max_k) + kKeys - 1) / kKeys + Cost<S>::kItem;
+  const int64_t max_tiles = (static_cast<int64_t>(a.max_k) + kKeys - 1) / kKeys, max_cost = max_tiles + Cost<S>::kItem;
   a.n_ranges = 0;
-  // Equal ranges while whole items would leave the chip uneven.
-  if (items * a.Hkv < 4 * slots && by_total * max_cost < (int64_t{1} << 31)) {
+  // the tiles that an item can have: all, or those of its tokens' windows and the sinks'
+  int64_t item_tiles = max_tiles;
+  if (a.window > 0)
+    item_tiles = std::min(item_tiles, (static_cast<int64_t>(a.window) + a.sinks + std::min<int64_t>(S::M, max_rows)) / kKeys + 2);
+  // Equal ranges where they beat whole items, whose last round may be nearly empty
+  // (both as if every item were as large as it can be).  Measured, whole items
+  // against ranges, D = 128, 8 kv heads, window 1024: one prompt of 512 tokens 24
+  // against 27 us, 1024 37 - 42, 2048 51 - 55, 8192 176 - 177; decode of 64 rows
+  // 49 - 54, of 256 206 - 211.  The other way round: trees of 32 nodes for 16
+  // sequences of 4096 111 - 77, decode of one row 31 - 14.
+  const int64_t n = items * a.Hkv, c = item_tiles + Cost<S>::kItem, rounds = (n + slots - 1) / slots;
+  const bool cut = rounds * c * slots > n * c + Cost<S>::kCut * slots;
+  if (cut && by_total * max_cost < (int64_t{1} << 31)) {
     const int per = a.Hkv < 8 && 8 % a.Hkv == 0 ? 8 / a.Hkv : 1;
-    const int64_t most = by_total * max_cost / Cost<S>::kMinRange + 1;  // ranges that can have work
+    a.min_range = static_cast<int>(std::max<int64_t>(Cost<S>::kMinRange, item_tiles / Cost<S>::kPieces));
+    const int64_t most = by_total * max_cost / a.min_range + 1;  // ranges that can have work
     int64_t W = std::max<int64_t>(1, std::min(slots / a.Hkv, most));
     W = (W + per - 1) / per * per;
-    const int64_t n = W * a.Hkv * 2;
-    const int64_t o_bytes = align256(n * S::M * S::D * 4), l_bytes = align256(n * S::M * 4);
-    const int64_t bytes = o_bytes + l_bytes + align256(n * 16);
+    const int64_t parts = W * a.Hkv * 2;
+    const int64_t o_bytes = align256(parts * S::M * S::D * 4), l_bytes = align256(parts * S::M * 4);
+    const int64_t bytes = o_bytes + l_bytes + align256(parts * 16);
     if (!workspace || workspace_bytes < bytes) {
       if (!need)
         return fail(NQ_EINVAL, "span attention: workspace %lld bytes < %lld", (long long)workspace_bytes,
@@ -1327,7 +1374,16 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
     span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(W * a.Hkv)), 64 * S::RW, S::LDS_B, stream>>>(a);
     const int rc = check_launch("span attention");
     if (rc != NQ_OK || W <= 1) return rc;
-    span_merge_kernel<T, S><<<dim3(static_cast<unsigned>(W * a.Hkv), MergeShape<S>::WAVES / 4), 256, 0, stream>>>(a);
+    const unsigned n_wg = static_cast<unsigned>(W * a.Hkv);
+    // Four waves to an element where items have many pieces, unless that is many
+    // workgroups: decode of one row 14.4 us against 15.4 with one wave, a tree of 4
+    // nodes behind 8192 tokens 21 against 26 (2080 workgroups); of 32 rows of 4096 fp8
+    // tokens (4 pieces each) 67 against 61, and trees of 4 nodes for 16 sequences at
+    // D = 256, fp8 (16 pieces each, 4096 workgroups) 59 against 52.
+    if (W > kMergeUnroll * items && n_wg * MergeShape<S>::WAVES < 16u * static_cast<unsigned>(device_cus()))
+      span_merge_kernel<T, S, 4><<<dim3(n_wg, MergeShape<S>::WAVES), 256, 0, stream>>>(a);
+    else
+      span_merge_kernel<T, S, 1><<<dim3(n_wg, MergeShape<S>::WAVES / 4), 256, 0, stream>>>(a);
     return check_launch("span attention (merge)");
   }
   // Whole items, dealt out in turn to the workgroups that the chip holds at once

@@ -151,3 +151,17 @@ def test_masked_nan_and_infinity(cuda, hq, hkv, d, dtype, fp8):
         c = Case(new, [0] * len(new), hq, hkv, d, dtype, block=32, fp8=fp8, seed=seed)
         _odd(c, torch.Generator().manual_seed(seed), 0.06).to(cuda)
         _check_odd(c.tree_attention(mask), tree_reference(c, mask), c, dtype)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype,fp8,block", [
+    (8, 2, 128, BF, False, 64), (8, 8, 128, HF, True, 32), (12, 3, 128, BF, True, 256), (16, 1, 128, BF, False, 32),
+    (8, 2, 256, BF, False, 32), (4, 4, 256, HF, True, 64), (8, 1, 256, HF, False, 64), (8, 2, 256, BF, True, 32)])
+@pytest.mark.parametrize("new,pre", [([3], [4100]), ([14], [2600]), ([40, 1, 33], [2000, 900, 70])])
+def test_items_cut_into_pieces(cuda, new, pre, hq, hkv, d, dtype, fp8, block):
+    """Few long items: each cut into many pieces, for every launch shape; trees, windows and decode."""
+    c = Case(new, pre, hq, hkv, d, dtype, block=block, fp8=fp8, seed=sum(new)).to(cuda)
+    trees, mask = tree_masks(new, seed=sum(pre))
+    check(c.tree_attention(mask), *tree_reference(c, mask), dtype)
+    check(c.window_prefill(1500, 40), *c.window_reference(1500, 40), dtype)
+    one = Case([1] * len(pre), pre, hq, hkv, d, dtype, block=block, fp8=fp8, seed=1).to(cuda)
+    check(one.window_decode(1900, 3), *one.window_reference(1900, 3), dtype)
