@@ -27,9 +27,24 @@
 // rounding P to 16 bits loses no more than it does at P <= 1).
 //
 // NaN and infinities in keys or values that a row does not see do not reach
-// it: masked scores are replaced before use, and a masked tile whose values
-// are not all finite takes them out of the product and gives them back to the
-// rows that see them (odd_values, poison, clean).
+// it: masked scores are replaced before use, and an item whose outputs are not
+// all finite is done again with the values that are not finite taken out of the
+// products and given back to the rows that see them (odd_values, poison, clean).
+// Checking every masked tile's values in the first pass cost more than the rare
+// second one: a prompt pair of 8000 tokens, window 2048, 757 us against 570.
+//
+// Work.  Few long items are cut into equal ranges of the tiles laid end to end,
+// one per workgroup, and joined by a second kernel; many are dealt out whole
+// (launch).  A workgroup's copies run on from an item into the next, kAhead
+// tiles before the tile at work.
+//
+// What bounds it, measured: prefill, the matrix cores and the exponentials
+// beside them: two prompts of 8016 and 8089 tokens, 32 query heads of 8 kv heads
+// at D = 128, window 2048, 570 us, 830 TFLOP/s; full causal of 8192 980.  Trees
+// of 64 nodes and 64 query heads over 16000-32768 fp8 tokens 256 us, 750 TFLOP/s
+// (the conversions share the vector unit with the exponentials).  Batched
+// decode, HBM: 96 rows through a window of 4096, 258-266 us, 5.5 TB/s.  Single
+// requests, a chain of round trips to memory: 11 us, and 7 for the second kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -99,8 +114,9 @@ constexpr int kPieceNone = -1, kPieceMore = 0, kPieceLast = 1;
 // a ring of SLOTS tiles.
 //  * one wave (M = 16): decode and the smallest trees.  Its ring is its own:
 //    no barriers, and K and V of SLOTS tiles are in flight at all times.
-//  * four waves of 16 or 32 rows (eight of 16 at head_dim 256).  A barrier per
-//    tile; copies run SLOTS - 1 tiles ahead.
+//  * four waves of 16 or 32 rows (eight of 16 at head_dim 256, where four of 32,
+//    with 400 registers and so one per SIMD, ran 147 us for the prompts that take
+//    124).  A barrier per tile; copies run SLOTS - 1 tiles ahead.
 template <int D_, bool FP8, int RW_, int QS_, int SLOTS_>
 struct Shape {
   static constexpr int D = D_, RW = RW_, QS = QS_, SLOTS = SLOTS_;
@@ -203,8 +219,11 @@ struct Cost {
   // into about kPieces.  Fewer pieces leave compute units idle, more are a longer
   // merge: one tree of 16 rows behind 8192 tokens 58 us in ranges of 2 tiles (128
   // pieces), 21 in ranges of 8; one of 64 rows 54 in ranges of 2, 34 of 8, 26 of
-  // 16; a decode of 1028 tokens 14.4 in ranges of 2, 15.3 of 4.
-  static constexpr int kMinRange = S::RW == 1 ? 2 : 8, kPieces = S::RW == 1 ? 32 : 16;
+  // 16; a decode of 1028 tokens 14.4 in ranges of 2, 15.3 of 4.  The larger a
+  // piece's partials, the longer its range: trees of 8 nodes (64 rows) behind 800
+  // tokens 17.8 in ranges of 4, 18.9 of 8 (D = 256: 19.5 and 22.3); a prefill of
+  // 100 tokens (128 rows) behind 2000 49 and 34.
+  static constexpr int kMinRange = S::RW == 1 ? 2 : S::M <= 64 ? 4 : 8, kPieces = S::RW == 1 ? 32 : 16;
   // What cutting costs, in the time of a tile: partials written, a second launch.
   static constexpr int kCut = 20;
 };
@@ -1398,6 +1417,10 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
 
 template <class T, bool FP8>
 int launch_shape(const SpanArgs &a, int D, int64_t max_rows, void *ws, int64_t ws_bytes, int64_t *need, hipStream_t s) {
+  // The smallest shape that holds the longest sequence's rows.  One row block in
+  // the four waves' shape: decode of 32 rows of 4096 tokens 110 us against 107, of
+  // fp8 80 against 58.  Up to 64 rows in the largest: trees of 8 nodes for 16
+  // sequences of 4096 61 against 59, fp8 64 against 50 (D = 256: 67 against 59).
   if (D == 256) {
     if (max_rows <= 16)
       return launch<T, FP8, Shape<256, FP8, 1, 1, 2>>(a, max_rows, FP8 ? 4 : 2, ws, ws_bytes, need, s);

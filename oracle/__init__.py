@@ -23,6 +23,8 @@ Modules
 ``output_gate`` the ``attn_output * sigmoid(gate)`` gate of Qwen3.5.
 ``gdn``        the gated delta rule (decode step, packed prefill) in float64
                and the gated RMS norm of its output.
+``spans``      attention over windows with sinks and over trees of drafted
+               tokens in float64, accepted paths and page moves.
 
 Parity pinning (what checks each function; see ``tests/test_oracle.py``):
 
