@@ -324,8 +324,7 @@ __device__ __forceinline__ void span_body() {
     pos0 = w < W ? static_cast<int>(static_cast<int64_t>(w) * total / W) : 0;
     pos1 = w < W ? static_cast<int>(static_cast<int64_t>(w + 1) * total / W) : 0;
   }
-  // The range's two partial pieces, written for the merge when it is done.
-  int cuts = 0;  // which of the range's two slots have been described
+  int cuts = 0;  // which of the range's two partial pieces have been described to the merge
   // The first item from `at` (a position or a round) on that this workgroup has
   // to do something for (live: there is one).
   struct Item {
