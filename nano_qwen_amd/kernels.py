@@ -730,22 +730,24 @@ def _check_one_device(what, first, *others):
 
 
 def _rows_of(what, name, t, shape, dtype):
-    """(pointer, row stride, head stride) of a ``[rows, heads, dim]`` tensor of ``shape``."""
-    t3 = t.squeeze(1) if t.dim() == 4 and t.shape[1] == 1 else t
-    if t3.shape != shape or t3.stride(-1) != 1 or t3.dtype != dtype:
+    """(pointer, row stride, head stride) of a ``[rows, heads, dim]`` (or ``[rows, 1, heads, dim]``) tensor of ``shape``."""
+    have, strides = tuple(t.shape), t.stride()
+    if len(have) == 4 and have[1] == 1:
+        have, strides = (have[0], have[2], have[3]), (strides[0], strides[2], strides[3])
+    if have != tuple(shape) or strides[2] != 1 or t.dtype != dtype:
         raise RuntimeError(f"{what}: {name} must be {list(shape)} of {dtype} with a contiguous last dim")
-    return t3.data_ptr(), t3.stride(0), t3.stride(1)
+    return t.data_ptr(), strides[0], strides[1]
 
 
 def _paged_args(what, d, k_cache, v_cache, block_table, n):
     """(blocks, block_size, kv heads) of paged K/V and their table, checked."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != d or \
+    pool, table = k_cache.shape, block_table.shape
+    if len(pool) != 4 or v_cache.shape != pool or pool[3] != d or \
             not (k_cache.is_contiguous() and v_cache.is_contiguous()) or v_cache.dtype != k_cache.dtype:
         raise RuntimeError(f"{what}: caches must be contiguous [num_blocks, block_size, Hkv, {d}] of one dtype")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n or \
-            block_table.shape[1] == 0 or block_table.stride(1) != 1:
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] < n or table[1] == 0 or block_table.stride(1) != 1:
         raise RuntimeError(f"{what}: block_table must be int32 [sequences, width] with contiguous rows")
-    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[2]
+    return pool[0], pool[1], pool[2]
 
 
 def _scale_args(what, kv_dtype, hkv, k_scale, v_scale):
