@@ -44,7 +44,7 @@
 // of 64 nodes and 64 query heads over 16000-32768 fp8 tokens 256 us, 750 TFLOP/s
 // (the conversions share the vector unit with the exponentials).  Batched
 // decode, HBM: 96 rows through a window of 4096, 258-266 us, 5.5 TB/s.  Single
-// requests, a chain of round trips to memory: 11 us, and 7 for the second kernel.
+// requests, a chain of round trips to memory: 12 us, and 4-6 for the second kernel.
 #include <algorithm>
 #include <type_traits>
 
