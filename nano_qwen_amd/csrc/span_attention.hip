@@ -225,7 +225,7 @@ struct Cost {
   // 100 tokens (128 rows) behind 2000 49 and 34.
   static constexpr int kMinRange = S::RW == 1 ? 2 : S::M <= 64 ? 4 : 8, kPieces = S::RW == 1 ? 32 : 16;
   // What cutting costs, in the time of a tile: partials written, a second launch.
-  static constexpr int kCut = 20;
+  static constexpr int kCut = S::RW == 1 ? 20 : 28;
 };
 template <class S, class A>
 __device__ __forceinline__ int row_tiles(const A &a, const Seq &q) {
@@ -1362,7 +1362,8 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
   // Equal ranges where they beat whole items, whose last round may be nearly empty
   // (both as if every item were as large as it can be).  Measured, whole items
   // against ranges, D = 128, 8 kv heads, window 1024: one prompt of 512 tokens 24
-  // against 27 us, 1024 37 - 42, 2048 51 - 55, 8192 176 - 177; decode of 64 rows
+  // against 27 us, 1024 37 - 42, 2048 51 - 55, 8192 176 - 177; chats of 81-333
+  // tokens behind 4000-8000 fp8 ones, four of them, 43 - 47; decode of 64 rows
   // 49 - 54, of 256 206 - 211.  The other way round: trees of 32 nodes for 16
   // sequences of 4096 111 - 77, decode of one row 31 - 14.
   const int64_t n = items * a.Hkv, c = item_tiles + Cost<S>::kItem, rounds = (n + slots - 1) / slots;
