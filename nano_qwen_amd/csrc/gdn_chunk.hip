@@ -382,12 +382,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     const u32x4 rv = rsrc_words(a.v + static_cast<int64_t>(c0) * a.v_rs + hv * kD * 2,
                                 static_cast<uint32_t>((rows - 1) * a.v_rs + kD * 2));
     const int l = tid & 63;
+    uint32_t src[4];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) {
-      const int row0 = 16 * wave + 4 * q4, row = row0 + (l >> 4);  // row0 uniform: M0
+      const int row = 16 * wave + 4 * q4 + (l >> 4);
       const int chunk = (l & 15) ^ swz_c(row);
-      dma16_opaque(LV + row0 * 256, rv, static_cast<uint32_t>(row * static_cast<int>(a.v_rs) + 16 * chunk));
+      src[q4] = static_cast<uint32_t>(row * static_cast<int>(a.v_rs) + 16 * chunk);
     }
+    dma16_group(LV + 16 * wave * 256, rv, src);
   };
   // The next chunk's q and k rows into L2 ahead of their fetch: one dword
   // of each 128-byte line, by LDS DMA into a scratch area nobody reads

@@ -506,14 +506,10 @@ __device__ __forceinline__ void span_body() {
     --st_left;
   };
   auto copy_k = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
-    const u32x4 r = rsrc_words(src, nrec);
-#pragma unroll
-    for (int c = 0; c < COPS; ++c) dma16_opaque(dst + (rw * COPS + c) * 1024, r, src_k[c]);
+    dma16_group(dst + rw * COPS * 1024, rsrc_words(src, nrec), src_k);
   };
   auto copy_v = [&](uint32_t dst, const uint8_t *src, uint32_t nrec) {
-    const u32x4 r = rsrc_words(src + v_minus_k, nrec);
-#pragma unroll
-    for (int c = 0; c < COPS; ++c) dma16_opaque(dst + TILE_B + (rw * COPS + c) * 1024, r, src_v[c]);
+    dma16_group(dst + TILE_B + rw * COPS * 1024, rsrc_words(src + v_minus_k, nrec), src_v);
   };
 
   // ---------------------------------------------------------------- operands

@@ -790,13 +790,8 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   auto issue = [&]() {
     if (run_left == 0) next_run();
     const uint32_t dst = st_dst + wave * (CR * SRC_ROWB);
-    const u32x4 rk = rsrc_words(st_src, st_nrec);
-    const u32x4 rv = rsrc_words(st_src + v_minus_k, st_nrec);
-#pragma unroll
-    for (int c = 0; c < COPS; ++c) {
-      dma16_opaque(dst + 1024 * c, rk, src_k[c]);
-      dma16_opaque(dst + DT::TILE_B + 1024 * c, rv, src_v[c]);
-    }
+    dma16_group(dst, rsrc_words(st_src, st_nrec), src_k);
+    dma16_group(dst + DT::TILE_B, rsrc_words(st_src + v_minus_k, st_nrec), src_v);
     st_src += tile_bytes;
     st_dst = st_dst == lds_last ? lds0 : st_dst + DT::SLOT_B;
     --run_left;

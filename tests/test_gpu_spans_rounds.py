@@ -1,0 +1,42 @@
+"""Windowed and tree attention where a workgroup has many items, one after the other: the entries of its stream of
+tiles full, partly filled, empty and missing by turns, lists of more than 64 tiles, items dealt out over several rounds."""
+import pytest
+import torch
+
+from oracle import spans
+from tests.spans import Case, check, tree_masks, tree_reference
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _lose_pages(case, every=3):
+    """Some visible pages are missing: one in the middle, the last, or all of a sequence's."""
+    pages = [(case.table[i] >= 0).nonzero()[:, 0].tolist() for i in range(len(case.have))]
+    for i in range(0, len(pages), every):
+        if pages[i]:
+            lost = (pages[i][len(pages[i]) // 2:][:1], pages[i][-1:], pages[i])[(i // every) % 3]
+            for j in lost:
+                case.table[i, j] = (-1, 10 ** 6)[i % 2]
+    return case
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("dtype,fp8", [(BF, False), (HF, False), (BF, True), (HF, True)])
+def test_one_wave_entries(cuda, d, dtype, fp8):
+    """Rows of one wave (decode, the smallest trees and prefills): long items behind items of one tile or none, last
+    tiles of one key, missing pages; whole items and equal ranges (a window of 65, of all)."""
+    pre = [0, 330, 31, 32, 33, 400, -1, 64, 5, 250, 95, 1, 160] * 10
+    c = _lose_pages(Case([1] * len(pre), pre, 8, 8, d, dtype, block=32, fp8=fp8, seed=d)).to(cuda)
+    for window, sinks in ((65, 3), (1, 0), (5000, 0)):
+        check(c.window_decode(window, sinks), *c.window_reference(window, sinks), dtype, f"decode {window}")
+    new, pre = [2, 1, 3, 0, 1, 2, 3] * 8, [max(p, 0) for p in pre[:56]]
+    t = _lose_pages(Case(new, pre, 8, 2, d, dtype, block=32, fp8=fp8, seed=d + 1)).to(cuda)
+    trees, mask = tree_masks([n for n in new if n], seed=d)
+    check(t.tree_attention(mask), *tree_reference(t, mask), dtype, "trees")
+    check(t.window_prefill(40, 5), *t.window_reference(40, 5), dtype, "paged prefill")
+    if not fp8:    # packed, the last sequence's last tile at the tensor's end
+        for seed, last in enumerate((1, 31, 32, 33, 70)):
+            p = Case(new + [2], [k % 90 for k in pre] + [last - 2 if last > 2 else 0], 8, 2, d, dtype, paged=False,
+                     seed=seed).to(cuda)
+            check(p.window_prefill(50, 1), *p.window_reference(50, 1), dtype, f"packed prefill {last}")
