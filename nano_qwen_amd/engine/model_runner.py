@@ -231,12 +231,13 @@ class ModelRunner:
         return input_ids, positions
 
     def prepare_decode(self, seqs):
-        """engine/model_runner.py:285-306 with the HIP metadata kernel."""
+        """engine/model_runner.py:285-306 with the HIP metadata kernel.  The last token's page is the one of its
+        position: a table may have pages to spare behind it (the reference's last one, after a tree step)."""
         bs = len(seqs)
         cpu = self.decode_cpu
         for i, seq in enumerate(seqs):
             cpu["seq_lens"][i] = len(seq)
-            cpu["last_block_ids"][i] = seq.block_table[-1]
+            cpu["last_block_ids"][i] = seq.block_table[(len(seq) - 1) // self.block_size]
         for name, tensor in cpu.items():
             self.decode_gpu[name][:bs].copy_(tensor[:bs], non_blocking=True)
         gpu = self.decode_gpu
@@ -304,7 +305,9 @@ class ModelRunner:
                                    t["tokens"], target_tokens)
 
     def accept_tree(self, seqs, drafts, path, num_accepted, next_tokens):
-        """Appends what ``commit_tree`` accepted, and the token after it, to the sequences (waits for the device)."""
+        """Appends what ``commit_tree`` accepted, and the token after it, to the sequences (waits for the device).
+        Their tables keep the pages that the other drafts needed; a decode step that follows takes its input ids from
+        ``sampled_token_ids_gpu``, where the caller puts ``next_tokens`` as after any step."""
         for seq, tokens, p, n, last in zip(seqs, drafts, path.tolist(), num_accepted.tolist(), next_tokens.tolist()):
             for node in p[1:n]:
                 seq.append_token(tokens[node - 1])
