@@ -204,6 +204,7 @@ class ModelRunner:
             seqlen_q = seq.num_scheduled_tokens
             end = start + seqlen_q
             seqlen_k = end
+            seq.num_prepared_tokens = end
             input_ids.extend(seq[start:end])
             positions.extend(range(start, end))
             cu_seqlens_q.append(cu_seqlens_q[-1] + seqlen_q)
@@ -236,6 +237,7 @@ class ModelRunner:
         bs = len(seqs)
         cpu = self.decode_cpu
         for i, seq in enumerate(seqs):
+            seq.num_prepared_tokens = len(seq)
             cpu["seq_lens"][i] = len(seq)
             cpu["last_block_ids"][i] = seq.block_table[(len(seq) - 1) // self.block_size]
         for name, tensor in cpu.items():
@@ -283,6 +285,7 @@ class ModelRunner:
             all_parents.append([-1, *up])
             cu_q.append(cu_q[-1] + n)
             cu_k.append(cu_k[-1] + base + n)
+            seq.num_prepared_tokens = base + n
         max_q = max(len(p) for p in all_parents)
         max_k = max(b - a for a, b in zip(cu_k, cu_k[1:]))
         mask = kernels.tree_masks(all_parents)
@@ -338,6 +341,7 @@ class ModelRunner:
             full, rows = divmod(len(seq) - 1, self.block_size)    # the last token is not in the cache yet
             children.append(Sequence(seq.token_ids, [*seq.block_table[:full], block], seq.num_cached_tokens,
                                      seq.num_scheduled_tokens))
+            children[-1].num_prepared_tokens = getattr(seq, "num_prepared_tokens", 0)
             if rows:
                 src.append(seq.block_table[full])
                 dst.append(block)
@@ -356,13 +360,17 @@ class ModelRunner:
             seq.block_table = [moves.get(b, b) for b in seq.block_table]
         return len(used)
 
-    def release_window_blocks(self, seq, window, num_sinks=0):
-        """Takes the pages out of the sequence's table (-1) that no token from its last one on sees through a
-        ``window`` with ``num_sinks`` sinks, and returns their ids.  Of layers with several windows, the largest
-        counts; layers without one need every page."""
-        first = max(0, len(seq) - window)    # what the last token sees
+    def release_window_blocks(self, seq, window, num_sinks=0, position=None):
+        """Takes the pages out of the sequence's table (-1) that no token from ``position`` on sees through a
+        ``window`` with ``num_sinks`` sinks, and returns their ids.  ``position``: of the first token still to be
+        computed; by default the last one's or, while a prompt is prefilled in chunks, the one behind the last chunk
+        that ``prepare_prefill`` was given.  Of layers with several windows, the largest counts; layers without one
+        need every page."""
+        if position is None:
+            position = min(len(seq) - 1, getattr(seq, "num_prepared_tokens", 0) or len(seq))
+        first = max(0, position - window + 1)    # what that token sees
         freed = []
-        for i in range(-(-num_sinks // self.block_size), first // self.block_size):
+        for i in range(-(-num_sinks // self.block_size), min(first // self.block_size, len(seq.block_table))):
             if seq.block_table[i] >= 0:
                 freed.append(seq.block_table[i])
                 seq.block_table[i] = -1

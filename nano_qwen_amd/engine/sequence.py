@@ -19,6 +19,7 @@ class Sequence:
         self.num_cached_tokens = num_cached_tokens
         self.num_scheduled_tokens = num_scheduled_tokens
         self.block_table = list(block_table or [])
+        self.num_prepared_tokens = 0    # of the last step that the runner prepared: what is in the cache after it
 
     def __len__(self):
         return self.num_tokens

@@ -1,11 +1,12 @@
-"""Tree steps followed by other steps of the runner, on the GPU."""
+"""Tree steps followed by other steps of the runner, and pages released in the middle of a prompt, on the GPU."""
 import pytest
 import torch
 
 import nano_qwen_amd.utils.context as C
 from nano_qwen_amd.engine import Sequence
-from tests.spans import half_step
-from tests.test_gpu_spans_use import BF, _engine, _run
+from oracle import spans
+from tests.spans import check, half_step
+from tests.test_gpu_spans_use import BF, _engine, _run, _token_rows
 
 pytestmark = pytest.mark.gpu
 # two outputs of the same token: rounding of P and of the output in both, values of |v| <= 5
@@ -49,4 +50,29 @@ def test_decode_after_partial_acceptance(cuda, accepted):
     for p in range(len(a) - 1):
         x, y = (raw[:, :, s.block_table[p // 32], p % 32] for s in (a, twin))
         assert torch.equal(x, y), p
+    C.reset_context()
+
+
+def test_pages_released_between_chunks(cuda):
+    """A long prompt through windowed layers in chunks, pages given back after each and overwritten by their takers."""
+    window, sinks, n = 40, 3, 190
+    runner, attns = _engine(cuda, 2, window=window, num_sinks=sinks)
+    tokens = list(range(300, 300 + n))
+    s = Sequence(tokens, [9, 3, 14, 1, 22, 6])
+    rows = [_token_rows(tokens, range(n), i, "cpu") for i in range(2)]
+    see = spans.window_visible(torch.arange(n), n, window, sinks)
+    want = [spans.attend(q, k.double(), v.double(), see, 128 ** -0.5) for q, k, v in rows]
+    done, freed = 0, []
+    for chunk in (32, 40, 1, 77, 39):
+        s.num_cached_tokens, s.num_scheduled_tokens = done, chunk
+        ids, pos = runner.prepare_prefill([s])
+        outs = _run(attns, ids, pos, cuda)
+        done += chunk
+        for out, (ref, mag) in zip(outs, want):
+            check(out, ref[done - chunk:done], mag[done - chunk:done], BF, f"to {done}")
+        taken = runner.release_window_blocks(s, window, sinks)
+        runner.kv_cache[:, :, taken] = float("nan")
+        freed += taken
+    assert done == n - 1 and freed == [3, 14, 1]    # 150 .. 189 are seen by the last token
+    s.append_token(1000)
     C.reset_context()

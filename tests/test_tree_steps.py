@@ -1,4 +1,5 @@
 """The runner's host side around tree steps, releases and compaction (CPU)."""
+import pytest
 import torch
 
 import nano_qwen_amd.utils.context as C
@@ -31,3 +32,35 @@ def test_decode_goes_to_the_page_of_its_position(monkeypatch):
     runner.prepare_decode([a, b])
     assert seen == dict(lens=[33, 34], last=[2, 5])
     C.reset_context()
+
+
+@pytest.mark.parametrize("window,sinks", [(40, 3), (1, 0), (33, 40), (300, 1)])
+def test_pages_released_between_chunks(window, sinks):
+    """While a prompt is prefilled in chunks, every page that a later token sees stays in the table."""
+    runner = make_runner()
+    n = 150
+    s = Sequence(list(range(n)), [9, 3, 14, 1, 22])
+    done = 0
+    for chunk in (32, 32, 20, 60, 6):
+        s.num_cached_tokens, s.num_scheduled_tokens = done, chunk
+        runner.prepare_prefill([s])
+        assert min(C.get_context().slot_mapping.tolist()) >= 0
+        done += chunk
+        runner.release_window_blocks(s, window, sinks)
+        for i, page in enumerate(s.block_table):    # seen by a later token, or to be written
+            needed = any(j >= done or j < sinks or j > min(done, n - 1) - window for j in range(32 * i, 32 * i + 32))
+            assert (page >= 0) == needed, (done, i)
+    s.append_token(7)
+    runner.release_window_blocks(s, window, sinks)
+    assert [x >= 0 for x in s.block_table] == [32 * i < sinks or 32 * i + 31 > 150 - window for i in range(5)]
+    C.reset_context()
+
+
+def test_release_from_a_position():
+    runner = make_runner()
+    s = Sequence(list(range(200)), list(range(10, 17)))
+    assert runner.release_window_blocks(s, 40, 3, position=64) == []
+    assert runner.release_window_blocks(s, 40, 3, position=103) == [11]    # 64 .. 103 are seen
+    assert runner.release_window_blocks(s, 40, 3) == [12, 13, 14]          # 160 .. 199
+    t = Sequence(list(range(200)), [1])
+    assert runner.release_window_blocks(t, 10) == [1]                      # no pages behind the first
