@@ -293,7 +293,7 @@ class ModelRunner:
         input_ids = self._to_device(input_ids, torch.int64)
         cu_q, cu_k = self._to_device(cu_q, torch.int32), self._to_device(cu_k, torch.int32)
         tables = self.prepare_block_tables(seqs)
-        self.tree = dict(tokens=input_ids, parents=self._to_device([p for t in all_parents for p in t], torch.int32),
+        self.tree = dict(seqs=list(seqs), tokens=input_ids, parents=self._to_device([p for t in all_parents for p in t], torch.int32),
                          cu_q=cu_q, cu_k=cu_k, max_q=max_q, tables=tables)
         set_tree_context(cu_q, cu_k, max_q, max_k, self._to_device(slots, torch.int32), tables, mask)
         return input_ids, self._to_device(positions, torch.int64)
@@ -302,10 +302,14 @@ class ModelRunner:
         """Ends the step that ``prepare_tree`` began: ``target_tokens`` (int64, one per node) is what the model
         chose after each node.  The accepted paths' keys and values move to where the sequences go on, in every
         layer; returns ``kernels.commit_tree``'s ``(path, num_accepted, next_tokens)``, on the device.
-        ``accept_tree`` brings the sequences up to date."""
+        ``accept_tree`` brings the sequences up to date.  A step is committed once: its rows move."""
         t = self.tree
-        return kernels.commit_tree(self.kv_cache, t["tables"], t["cu_q"], t["cu_k"], t["max_q"], t["parents"],
+        if t is None:
+            raise RuntimeError("commit_tree: no tree step is open")
+        done = kernels.commit_tree(self.kv_cache, t["tables"], t["cu_q"], t["cu_k"], t["max_q"], t["parents"],
                                    t["tokens"], target_tokens)
+        self.tree = None
+        return done
 
     def accept_tree(self, seqs, drafts, path, num_accepted, next_tokens):
         """Appends what ``commit_tree`` accepted, and the token after it, to the sequences (waits for the device).
@@ -315,6 +319,8 @@ class ModelRunner:
             for node in p[1:n]:
                 seq.append_token(tokens[node - 1])
             seq.append_token(last)
+        if self.tree is not None and self.tree["seqs"] == list(seqs):    # committed by the caller's own rule
+            self.tree = None
 
     # ------------------------------------------------------ pages of the pool
     def copy_blocks(self, src, dst, num_tokens=None):
@@ -351,7 +357,10 @@ class ModelRunner:
 
     def compact(self, seqs):
         """Moves the pages that ``seqs`` (all sequences of the pool) use to the pool's first ids, in one launch, and
-        their block tables with them; returns how many pages are in use."""
+        their block tables with them; returns how many pages are in use.  Not while a tree step is open, whose tables
+        are on the device (``commit_tree`` ends it; ``runner.tree = None`` gives it up)."""
+        if self.tree is not None:
+            raise RuntimeError("compact: a tree step is open")
         used = sorted({b for seq in seqs for b in seq.block_table if b >= 0})
         free = sorted(set(range(len(used))) - set(used))
         moves = dict(zip([b for b in used if b >= len(used)], free, strict=True))

@@ -64,3 +64,38 @@ def test_release_from_a_position():
     assert runner.release_window_blocks(s, 40, 3) == [12, 13, 14]          # 160 .. 199
     t = Sequence(list(range(200)), [1])
     assert runner.release_window_blocks(t, 10) == [1]                      # no pages behind the first
+
+
+def test_tree_steps_end_once(monkeypatch):
+    """A step is committed once, and the pool is not compacted under it."""
+    runner = make_runner()
+    calls = []
+    monkeypatch.setattr(kernels, "commit_tree", lambda *a, **kw: calls.append(a) or "done")
+    monkeypatch.setattr(kernels, "copy_kv_blocks", lambda *a: None)
+    with pytest.raises(RuntimeError, match="no tree step"):
+        runner.commit_tree(torch.zeros(3, dtype=torch.int64))
+    a, b = Sequence(list(range(30)), [7, 2]), Sequence([1, 2], [9])
+    runner.prepare_tree([a], [[5, 6]], [[0, 1]])
+    with pytest.raises(RuntimeError, match="open"):
+        runner.compact([a, b])
+    assert a.block_table == [7, 2]
+    assert runner.commit_tree(torch.zeros(3, dtype=torch.int64)) == "done" and len(calls) == 1
+    with pytest.raises(RuntimeError, match="no tree step"):
+        runner.commit_tree(torch.zeros(3, dtype=torch.int64))
+    # the next sequences' step is prepared before this one's are brought up to date
+    runner.prepare_tree([b], [[5]], [[0]])
+    result = torch.tensor([[0, 1]]), torch.tensor([2]), torch.tensor([8])
+    runner.accept_tree([a], [[5, 6]], *result)
+    runner.commit_tree(torch.zeros(2, dtype=torch.int64))
+    assert len(calls) == 2
+    # a caller that commits through kernels.commit_tree
+    runner.prepare_tree([b], [[5]], [[0]])
+    runner.accept_tree([b], [[5]], *result)
+    assert runner.compact([a, b]) == 3 and runner.tree is None
+    # a call that is refused leaves the step open
+    runner.prepare_tree([a], [[5, 6]], [[0, 1]])
+    monkeypatch.undo()
+    with pytest.raises(RuntimeError, match="device"):
+        runner.commit_tree(torch.zeros(3, dtype=torch.int64))
+    assert runner.tree is not None
+    C.reset_context()
