@@ -285,9 +285,10 @@ class ModelRunner:
             all_parents.append([-1, *up])
             cu_q.append(cu_q[-1] + n)
             cu_k.append(cu_k[-1] + base + n)
-            seq.num_prepared_tokens = base + n
         max_q = max(len(p) for p in all_parents)
         max_k = max(b - a for a, b in zip(cu_k, cu_k[1:]))
+        for seq, a, b in zip(seqs, cu_k, cu_k[1:]):
+            seq.num_prepared_tokens = b - a
         mask = kernels.tree_masks(all_parents)
         mask = (mask.pin_memory() if self._pin else mask).to(self.device, non_blocking=True)
         input_ids = self._to_device(input_ids, torch.int64)

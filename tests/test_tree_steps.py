@@ -62,6 +62,10 @@ def test_release_from_a_position():
     assert runner.release_window_blocks(s, 40, 3, position=64) == []
     assert runner.release_window_blocks(s, 40, 3, position=103) == [11]    # 64 .. 103 are seen
     assert runner.release_window_blocks(s, 40, 3) == [12, 13, 14]          # 160 .. 199
+    s.num_prepared_tokens = 200
+    with pytest.raises(ValueError):    # refused: nothing is prepared
+        runner.prepare_tree([s, Sequence([1], [2])], [[1], [2]], [[0], [1]])
+    assert s.num_prepared_tokens == 200
     t = Sequence(list(range(200)), [1])
     assert runner.release_window_blocks(t, 10) == [1]                      # no pages behind the first
 
