@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from .. import kernels
+from ..utils.context import get_context
 
 
 def _float32(p: torch.Tensor) -> torch.Tensor:
@@ -34,7 +35,11 @@ def gdn_core(layer, qkv_raw: torch.Tensor, z: torch.Tensor, a: torch.Tensor, b: 
     ``a, b [T, HV]``; ``state_indices [N]`` int32 (decode: N = T, one token
     per sequence; prefill: ``cu_seqlens [N + 1]`` int32 packs the sequences).
     Returns the normalized output ``[T, value_dim]`` (the ``out_proj`` input).
+    Refuses a step of trees of drafted tokens (``TreeContext``): the state would
+    run through every node, in their order.
     """
+    if getattr(get_context(), "tree_mask", None) is not None:
+        raise RuntimeError("gdn_core: trees of drafted tokens are not supported by layers with a recurrent state")
     T = qkv_raw.shape[0]
     H, HV = layer.num_k_heads, layer.num_v_heads
     Dk, Dv = layer.head_k_dim, layer.head_v_dim

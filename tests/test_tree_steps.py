@@ -5,7 +5,7 @@ import torch
 import nano_qwen_amd.utils.context as C
 from nano_qwen_amd import kernels
 from nano_qwen_amd.engine import ModelRunner, Sequence
-from nano_qwen_amd.layers import Attention
+from nano_qwen_amd.layers import Attention, gdn_core
 
 
 def make_runner(block=32, blocks=40, layers=2):
@@ -103,3 +103,15 @@ def test_tree_steps_end_once(monkeypatch):
         runner.commit_tree(torch.zeros(3, dtype=torch.int64))
     assert runner.tree is not None
     C.reset_context()
+
+
+def test_recurrent_layers_refuse_trees():
+    """A tree step looks like a prefill, but its nodes are no sequence."""
+    runner = make_runner()
+    x = torch.zeros(3, 8)
+    runner.prepare_tree([Sequence([1], [0])], [[5, 6]], [[0, 0]])
+    with pytest.raises(RuntimeError, match="trees"):
+        gdn_core(None, x, x, x, x, torch.zeros(1, dtype=torch.int32), cu_seqlens=C.get_context().cu_seqlens_q)
+    C.reset_context()
+    with pytest.raises(AttributeError):    # past the check
+        gdn_core(None, x, x, x, x, torch.zeros(1, dtype=torch.int32))
