@@ -766,8 +766,9 @@ def _check_cu(what, n1, *tensors):
 
 
 def _int32(x):
-    """A window or number of sinks as the C int that means the same: beyond every sequence is beyond."""
-    return min(int(x), 0x7fffffff)
+    """A window, number of sinks or length as the C int that means the same: beyond every sequence is beyond, and
+    below zero is refused."""
+    return max(-1, min(int(x), 0x7fffffff))
 
 
 def _launch_span(what, fn, device, args):
@@ -822,7 +823,7 @@ def tree_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q
     words = mask.shape[1]
     _launch_span(what, lib().nq_tree_attention, dev, (
         *qa, k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-        int(max_seqlen_q), int(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb,
+        _int32(max_seqlen_q), _int32(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb,
         mask.data_ptr(), mask.stride(0) if tq > 1 else words, words, *oa, n, tq, hq, hkv, d, bs, float(softmax_scale),
         dtype_code(q.dtype), dtype_code(k_cache.dtype), *_scale_args(what, k_cache.dtype, hkv, k_scale, v_scale), *ga))
     return out
@@ -882,7 +883,7 @@ def window_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
     _launch_span(what, lib().nq_window_prefill, dev, (
         *qa, k.data_ptr(), v.data_ptr(), kv_rs, tk, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-        int(max_seqlen_q), int(max_seqlen_k), *pa, _int32(window), _int32(num_sinks), *oa, n, tq, hq, hkv, d, bs,
+        _int32(max_seqlen_q), _int32(max_seqlen_k), *pa, _int32(window), _int32(num_sinks), *oa, n, tq, hq, hkv, d, bs,
         float(softmax_scale), dtype_code(q.dtype), dtype_code(k.dtype),
         *_scale_args(what, k.dtype, hkv, k_scale, v_scale), *ga))
     return out

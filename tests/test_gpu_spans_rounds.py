@@ -40,3 +40,26 @@ def test_one_wave_entries(cuda, d, dtype, fp8):
             p = Case(new + [2], [k % 90 for k in pre] + [last - 2 if last > 2 else 0], 8, 2, d, dtype, paged=False,
                      seed=seed).to(cuda)
             check(p.window_prefill(50, 1), *p.window_reference(50, 1), dtype, f"packed prefill {last}")
+
+
+def test_lengths_beyond_32_bits(cuda):
+    """Largest lengths that no int holds mean no bound; windows and sinks far below zero are refused."""
+    c = Case([3, 2], [100, 40], 8, 2, 128, BF, block=32).to(cuda)
+    p = Case([40, 3], [0, 0], 8, 2, 128, BF, paged=False).to(cuda)
+    trees, mask = tree_masks([3, 2])
+    want = c.tree_attention(mask), c.window_prefill(50, 2)
+    for far in (2 ** 31, 2 ** 32, 2 ** 40 + 7):
+        c.max_k = far
+        assert torch.equal(c.tree_attention(mask), want[0]) and torch.equal(c.window_prefill(50, 2), want[1])
+        for case, window, sinks in ((c, -far + 5, 0), (c, 5, -far + 1), (p, -far + 5, 0)):
+            with pytest.raises(RuntimeError):
+                case.window_prefill(window, sinks)
+        with pytest.raises(RuntimeError):
+            Case([1], [9], 8, 2, 128, BF, block=32).to(cuda).window_decode(-far + 5, 0)
+        p.max_k = far    # packed keys of a length that no tensor has
+        with pytest.raises(RuntimeError):
+            p.window_prefill(50, 2)
+        p.max_k = 40
+    c.max_q = -2 ** 32 + 3
+    with pytest.raises(RuntimeError):
+        c.tree_attention(mask)
