@@ -567,7 +567,8 @@ __device__ __forceinline__ void span_body() {
   // register per operand
   auto unhoist = [&]() { asm volatile("" : "+v"(kx_l), "+v"(vx_l)); };
 
-  const float sl2 = a0.scale_log2 * (FP8 ? ld_const(a0.k_scale + h) : 1.f);
+  // (never 0: a masked score, -inf, must stay that under a scale of 0)
+  const float sl2 = FP8 ? fmaxf(a0.scale_log2 * ld_const(a0.k_scale + h), 0x1p-126f) : a0.scale_log2;
 
   constexpr int kAhead = RW == 1 ? SLOTS : SLOTS - 1;
   const uint8_t *src;

@@ -63,3 +63,17 @@ def test_lengths_beyond_32_bits(cuda):
     c.max_q = -2 ** 32 + 3
     with pytest.raises(RuntimeError):
         c.tree_attention(mask)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_scales_of_zero(cuda, d):
+    """Keys of a head whose scale is 0 are all 0: the mean of the visible values."""
+    for new, pre in (([1, 1, 1], [70, 0, 300]), ([2, 9, 40], [33, 0, 90])):
+        c = Case(new, pre, 8, 2, d, BF, block=32, fp8=True, seed=d)
+        c.k_scale[1] = 0.0
+        c.to(cuda)
+        trees, mask = tree_masks(new, seed=1)
+        check(c.tree_attention(mask), *tree_reference(c, mask), BF, "tree")
+        check(c.window_prefill(40, 3), *c.window_reference(40, 3), BF, "prefill")
+        if max(new) == 1:
+            check(c.window_decode(40, 3), *c.window_reference(40, 3), BF, "decode")
