@@ -344,16 +344,18 @@ __device__ inline float sum32(float v) {
   return u2f(a) + u2f(b);
 }
 
+// The largest of three scores as they leave the matrix core: instructions that
+// the compiler knows, so that it keeps the wait states between a product and its
+// readers (inline assembly has none).  A NaN among them is the result.
+__device__ inline float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
 // The same maxima with a plain v_max_f32 after the swap: no NaN quieting of
-// the swapped value (the inputs are finite or -inf).
+// the swapped value (the inputs are finite or -inf).  Not for a matrix product's
+// results (see max3).
 __device__ inline float vmax_raw(float a, float b) {
   float r;
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
-__device__ inline float max3_raw(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 __device__ inline float max16_raw(float v) {

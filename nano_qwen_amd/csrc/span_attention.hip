@@ -183,12 +183,6 @@ __device__ __forceinline__ int small_div(int n, int d) {
 // A value that every lane has, in a scalar register (small_div leaves it in a
 // vector one).
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// Of scores as they leave the matrix core: instructions that the compiler knows,
-// so that it keeps the wait states between a product and its readers (inline
-// assembly has none).  A NaN among them is the result.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
-}
 // The tiles of a row tile whose tokens are ta .. tb.
 struct Tiles {
   int ts, tlo, n;  // tiles 0 .. ts - 1, then tlo, tlo + 1, ...: n in all

@@ -1206,8 +1206,8 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
               xt[qs][4 * ks + rr] = v;
             }
           // this lane's maximum over its 8 keys of row m (scaled)
-          mnew[qs] = max3_raw(max3_raw(xt[qs][0], xt[qs][1], xt[qs][2]),
-                              max3_raw(xt[qs][3], xt[qs][4], xt[qs][5]), vmax_raw(xt[qs][6], xt[qs][7])) * sl2;
+          mnew[qs] = max3(max3(xt[qs][0], xt[qs][1], xt[qs][2]), max3(xt[qs][3], xt[qs][4], xt[qs][5]),
+                          __builtin_elementwise_maximum(xt[qs][6], xt[qs][7])) * sl2;
           grow |= mnew[qs] > m_use[qs] + kRescale;
         }
         bool moved = false;
