@@ -23,8 +23,7 @@ constexpr int kChunk = kCopyThreads * kCopyUnroll * 16;
 
 __global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(uint8_t *pool, const int32_t *src, const int32_t *dst,
                                                                    const int32_t *tokens, int64_t num_blocks,
-                                                                   int block_size, int64_t row_bytes, int chunks,
-                                                                   int n) {
+                                                                   int block_size, int64_t row_bytes, int chunks) {
   // chunk fastest, then slab, then pair
   const int64_t unit = blockIdx.x;
   const int chunk = static_cast<int>(unit % chunks);
@@ -224,7 +223,7 @@ extern "C" int nq_copy_kv_blocks(void *kv_cache, int64_t num_slabs, int64_t num_
   copy_blocks_kernel<<<dim3(static_cast<unsigned>(chunks * num_pairs), static_cast<unsigned>(num_slabs)), kCopyThreads,
                        0, static_cast<hipStream_t>(stream)>>>(
       static_cast<uint8_t *>(kv_cache), src_blocks, dst_blocks, num_tokens, num_blocks, block_size, row_bytes,
-      static_cast<int>(chunks), static_cast<int>(num_pairs));
+      static_cast<int>(chunks));
   return check_launch("copy_kv_blocks");
 }
 
