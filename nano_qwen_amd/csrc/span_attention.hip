@@ -40,11 +40,13 @@
 //
 // What bounds it, measured: prefill, the matrix cores and the exponentials
 // beside them: two prompts of 8016 and 8089 tokens, 32 query heads of 8 kv heads
-// at D = 128, window 2048, 570 us, 830 TFLOP/s; full causal of 8192 980.  Trees
-// of 64 nodes and 64 query heads over 16000-32768 fp8 tokens 256 us, 750 TFLOP/s
-// (the conversions share the vector unit with the exponentials).  Batched
-// decode, HBM: 96 rows through a window of 4096, 258-266 us, 5.5 TB/s.  Single
-// requests, a chain of round trips to memory: 12 us, and 4-6 for the second kernel.
+// at D = 128, window 2048, 574-592 us, 800-820 TFLOP/s (products busy 38 % of the
+// time, other vector instructions 41 %); full causal of 8192 980.  Trees of 64
+// nodes and 64 query heads over 16000-32768 fp8 tokens 254-262 us, 740-760
+// TFLOP/s (35 % and 52 %: the conversions share the vector unit with the
+// exponentials).  Batched decode, HBM: 96 rows through a window of 4096, 265 us,
+// 5.5 TB/s.  Single requests, a chain of round trips to memory: 12 us, and 4-6
+// for the second kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -114,9 +116,11 @@ constexpr int kPieceNone = -1, kPieceMore = 0, kPieceLast = 1;
 // a ring of SLOTS tiles.
 //  * one wave (M = 16): decode and the smallest trees.  Its ring is its own:
 //    no barriers, and K and V of SLOTS tiles are in flight at all times.
-//  * four waves of 16 or 32 rows (eight of 16 at head_dim 256, where four of 32,
-//    with 400 registers and so one per SIMD, ran 147 us for the prompts that take
-//    124).  A barrier per tile; copies run SLOTS - 1 tiles ahead.
+//  * four waves of 16 or 32 rows (eight of 16 at head_dim 256; four of 32, with
+//    400 registers and so one per SIMD, ran 147 us for six prompts of 200-2567
+//    tokens where these took 124, before the rules of launch() brought them to
+//    113).  A barrier per tile; copies run SLOTS - 1 tiles ahead.  (The 16-bit
+//    shapes at head_dim 256 spill one and five registers, in the items' set-up.)
 template <int D_, bool FP8, int RW_, int QS_, int SLOTS_>
 struct Shape {
   static constexpr int D = D_, RW = RW_, QS = QS_, SLOTS = SLOTS_;
@@ -1226,8 +1230,8 @@ void span_attention_kernel(const SpanArgs a) {
 // 0 of the next ranges, up to the one marked last.  A wave takes J 16-dim
 // blocks of one row block, kMergeUnroll pieces in flight: the chain is two round
 // trips to memory and one per eight pieces, or per 32 where SPREAD = 4 waves
-// share them and join through LDS.  Latency bounds it (5-7 us, half of that the
-// launch), or reading the partials: 11 us for trees of 32 nodes, 16 sequences.
+// share them and join through LDS.  Latency bounds it (4-6 us, half of that the
+// launch), or reading the partials: 13 us for trees of 16-32 nodes, 16 sequences.
 constexpr int kMergeUnroll = 8;
 template <class S>
 struct MergeShape {
