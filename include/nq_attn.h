@@ -626,7 +626,8 @@ int nq_gdn_conv1d(const void *x, int64_t x_row_stride, const void *weight, int k
  *
  * All three: head_dim 128 or 256, groups of up to 16 query heads, q and out
  * F16/BF16 (q 16-byte aligned, out 8-byte), K/V of the type of q or
- * NQ_FP8_E4M3 with k_scale/v_scale float[num_kv_heads]; softmax_scale > 0.
+ * NQ_FP8_E4M3 with k_scale (not negative) and v_scale float[num_kv_heads];
+ * softmax_scale > 0.
  * Paged K/V: block_tables [num_seqs, >= max_blocks_per_seq] int32 with row
  * stride bt_stride, block_size a multiple of 32; entries of pages that hold no
  * visible key of the sequence's queries are not used, and keys of pages outside
@@ -688,8 +689,8 @@ int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_strid
                      void *v_cache, const int32_t *block_tables, int64_t bt_stride,
                      int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
                      const void *k_new, int64_t k_new_row_stride, const void *v_new,
-                     int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
-                     int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                     int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out,
+                     int64_t out_batch_stride, int64_t out_head_stride, int batch, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
                      float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
                      const float *v_scale, const void *gate, int64_t gate_batch_stride,
                      int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,

@@ -1597,8 +1597,8 @@ extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q
                                 void *v_cache, const int32_t *block_tables, int64_t bt_stride,
                                 int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
                                 const void *k_new, int64_t k_new_row_stride, const void *v_new,
-                                int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
-                                int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                                int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out,
+                                int64_t out_batch_stride, int64_t out_head_stride, int batch, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
                                 float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
                                 const float *v_scale, const void *gate, int64_t gate_batch_stride,
                                 int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,

@@ -86,8 +86,8 @@ def _grow(table, key, nbytes, dtype, device, zero=False):
 def release_workspaces(device=None) -> int:
     """Drop the kernels' per-stream buffers (decode split-K workspaces and
     arrival counters, prefill queue counters and partial outputs, GDN segment
-    states, windowed and tree attention's partial outputs) and every retired buffer, of ``device`` or of all devices; returns
-    how many were dropped.  Only safe once no HIP graph captured with them will
+    states, windowed and tree attention's partial outputs) and every retired
+    buffer, of ``device`` or of all devices; returns how many were dropped.  Only safe once no HIP graph captured with them will
     be replayed again (a replay would write freed memory) and while no other
     thread calls the kernels.  Later calls allocate fresh buffers (the counters
     start at zero again)."""
