@@ -733,6 +733,41 @@ int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int bl
                    const int64_t *target_tokens, int32_t *path, int32_t *num_accepted, int64_t *next_tokens,
                    void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A scale for each block of tokens and head (no counterpart in the reference):
+ * a cache of e4m3 codes whose pages are cut into blocks of scale_block tokens
+ * (32, 64, 128 or 256; a divisor of block_size).  k_scale / v_scale are float32
+ * [num_blocks, block_size / scale_block, num_kv_heads]: the code c of cache row
+ * `slot`, head h, stands for c * scale[slot / scale_block, h].
+ */
+
+/*
+ * Appends num_tokens rows of keys and values (16-bit [N, Hkv, D], contiguous
+ * heads) to cache rows slot_mapping[i], and the rotary embedding with them:
+ * the rows of q (null: none) and k are normed (q_weight, k_weight: both or
+ * neither; x / rms(x) * (w + weight_offset)), their first rotary_dim dims
+ * rotated by cos_sin_cache[positions[i]] (float32: rotary_dim / 2 cosines, then
+ * the sines), in fp32, and rounded once to q_out and k_out (null: keys are
+ * stored as they are given out, and not given out; must not overlap k).  A
+ * position outside [0, max_position) makes its row NaN.
+ *
+ * The scale of a block and head becomes the smallest power of two, from 2^-60
+ * to 2^60, whose 448-fold no finite value of the call's rows in it exceeds, or,
+ * unless those hold the block's first token, the old one if that is larger; the
+ * codes of the block's tokens before them are coded again where it grew.  What
+ * lies behind them in the block is not kept.  The rows of one block must be
+ * neighbours with rising slots, and no slot may occur twice.  Rows with a slot
+ * outside [0, num_slots) are not stored.
+ */
+int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                      int64_t k_row_stride, const void *v, int64_t v_row_stride, const int64_t *positions,
+                      const float *cos_sin_cache, int64_t max_position, int rotary_dim, const void *q_weight,
+                      const void *k_weight, float eps, float weight_offset, void *q_out, int64_t q_out_row_stride,
+                      int64_t q_out_head_stride, void *k_out, int64_t k_out_row_stride, void *k_cache, void *v_cache,
+                      float *k_scale, float *v_scale, const int32_t *slot_mapping, int64_t num_slots,
+                      int scale_block, int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1022,7 +1022,115 @@ def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
     return path, num_accepted, next_tokens
 
 
+# ------------------------------------- a scale for each block of tokens and head
+# (no counterpart in the reference, whose cache holds the model's own type)
+
+SCALE_BLOCKS = (32, 64, 128, 256)    # tokens of a block
+
+
+def _block_scales(what, k_cache, k_scale, v_scale):
+    """Tokens per block of scales ``[num_blocks, block_size / tokens, Hkv]``, checked against their e4m3 cache."""
+    nb, bs, hkv, _ = k_cache.shape
+    for t in (k_scale, v_scale):
+        if t is None or t.dtype != torch.float32 or t.dim() != 3 or t.shape != k_scale.shape or not t.is_contiguous():
+            raise RuntimeError(f"{what}: k_scale and v_scale must be contiguous float32 [num_blocks, block_size / tokens, Hkv]")
+    units = k_scale.shape[1]
+    if k_scale.shape[0] != nb or k_scale.shape[2] != hkv or units == 0 or bs % units or bs // units not in SCALE_BLOCKS:
+        raise RuntimeError(f"{what}: scales {list(k_scale.shape)} of a cache {list(k_cache.shape)}: blocks of "
+                           f"{', '.join(map(str, SCALE_BLOCKS))} tokens")
+    if k_cache.dtype != torch.float8_e4m3fn:
+        raise RuntimeError(f"{what}: a scale for each block needs a float8_e4m3fn cache")
+    return bs // units
+
+
+def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query=None, positions=None,
+                   cos_sin_cache=None, rotary_dim=0, q_weight=None, k_weight=None, eps=1e-6, weight_offset=1.0,
+                   q_out=None, k_out=None):
+    """Appends ``key/value [N, Hkv, D]`` to cache rows ``slot_mapping [N]`` (int32) of a paged ``float8_e4m3fn`` cache
+    whose blocks of 32, 64, 128 or 256 tokens have a scale for each head: ``k_scale/v_scale`` float32 ``[num_blocks,
+    block_size / tokens, Hkv]``, updated here.  One launch, with the rotary embedding (and the RMS norm) on the way.
+
+    With ``q_weight, k_weight [D]`` queries ``[N, Hq, D]`` and keys are normed (``x / rms * (w + weight_offset)``, 1.0
+    for a Gemma norm); with ``rotary_dim > 0`` their first dims are rotated by ``cos_sin_cache [max_position,
+    (1,) rotary_dim]`` (float32: cosines, then sines) at ``positions [N]`` (int64); all in fp32, rounded once.  Returns
+    ``(q_out, k_out)``: what is not transformed comes back as it is, and ``None`` for no query.
+
+    A block's scale is the smallest power of two, from 2^-60 to 2^60, whose 448-fold is no smaller than any finite
+    value; the block's first token sets it anew, later ones can only raise it, and then the block's earlier codes are
+    coded again.  A block's tokens are appended in order: those of one call are neighbouring rows with rising slots, no
+    slot occurs twice, and nothing is kept of what lies behind them in the block.  Rows with a slot outside the pool
+    are transformed and not stored.
+    """
+    what = "append_kvcache"
+    dev = _check_one_device(what, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query, positions,
+                            cos_sin_cache, q_weight, k_weight, q_out, k_out)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query, positions,
+                                  cos_sin_cache, rotary_dim, q_weight, k_weight, eps, weight_offset, q_out, k_out)
+    if key.dim() != 3:
+        raise RuntimeError(f"{what}: key and value must be [N, Hkv, D]")
+    n, hkv, d = key.shape
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[2:] != (hkv, d) or \
+            v_cache.dtype != k_cache.dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise RuntimeError(f"{what}: caches must be contiguous [num_blocks, block_size, {hkv}, {d}] of one dtype")
+    unit = _block_scales(what, k_cache, k_scale, v_scale)
+    for name, t in (("key", key), ("value", value)):
+        if t.shape != key.shape or t.dtype != key.dtype or t.stride(2) != 1 or (t.stride(1) != d and hkv > 1):
+            raise RuntimeError(f"{what}: {name} must be [N, Hkv, D] of key's dtype with contiguous heads")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous():
+        raise RuntimeError(f"{what}: slot_mapping must be contiguous int32 [{n}]")
+    norm = q_weight is not None or k_weight is not None
+    for t in (q_weight, k_weight) if norm else ():
+        if t is None or t.dtype != key.dtype or t.shape != (d,) or not t.is_contiguous():
+            raise RuntimeError(f"{what}: q_weight and k_weight must be contiguous [{d}] of key's dtype, both or neither")
+    max_pos = 0
+    if rotary_dim > 0:
+        if positions is None or positions.dtype != torch.int64 or positions.shape != (n,) or not positions.is_contiguous():
+            raise RuntimeError(f"{what}: positions must be contiguous int64 [{n}]")
+        if cos_sin_cache is None or cos_sin_cache.dtype != torch.float32 or not cos_sin_cache.is_contiguous() or \
+                cos_sin_cache.numel() != cos_sin_cache.shape[0] * rotary_dim:
+            raise RuntimeError(f"{what}: cos_sin_cache must be contiguous float32 [max_position, rotary_dim]")
+        max_pos = cos_sin_cache.shape[0]
+    transforms = norm or rotary_dim > 0
+    qa = qo = (None, 0, 0)
+    if query is None:
+        if q_out is not None:
+            raise RuntimeError(f"{what}: q_out without a query")
+    elif not transforms:
+        if q_out is not None:
+            raise RuntimeError(f"{what}: q_out without a norm or a rotation")
+        q_out = query
+    else:
+        shape = (n, query.shape[-2], d)
+        qa = _rows_of(what, "query", query, shape, key.dtype)
+        if q_out is None:
+            q_out = torch.empty(shape, dtype=key.dtype, device=key.device)
+        qo = _rows_of(what, "q_out", q_out, shape, key.dtype)
+    ko = (None, 0)
+    if not transforms:
+        if k_out is not None:
+            raise RuntimeError(f"{what}: k_out without a norm or a rotation")
+        k_out = key
+    else:
+        if k_out is None:
+            k_out = torch.empty(n, hkv, d, dtype=key.dtype, device=key.device)
+        elif _overlaps(k_out, key):    # a long run's keys are read twice
+            raise RuntimeError(f"{what}: k_out must not overlap key")
+        ko = _rows_of(what, "k_out", k_out, key.shape, key.dtype)
+        if ko[2] != d and hkv > 1:
+            raise RuntimeError(f"{what}: k_out must have contiguous heads")
+    one = hkv * d    # (row strides of single rows mean nothing)
+    check(lib().nq_append_kvcache(
+        *qa, ptr(key), key.stride(0) if n > 1 else one, ptr(value), value.stride(0) if n > 1 else one, ptr(positions),
+        ptr(cos_sin_cache), max_pos, int(rotary_dim), ptr(q_weight), ptr(k_weight), float(eps), float(weight_offset), *qo,
+        ko[0], ko[1] if n > 1 else one, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(slot_mapping),
+        k_cache.shape[0] * k_cache.shape[1], unit, n, 0 if qa[0] is None else query.shape[-2], hkv, d,
+        dtype_code(key.dtype), raw_stream(dev)), what)
+    return q_out, k_out
+
+
 __all__ = ["store_kvcache", "paged_decode", "varlen_prefill", "prepare_decode", "decode_plan", "qk_norm_rope_store",
            "output_gate", "gdn_decode", "gdn_prefill", "gated_rmsnorm", "gdn_conv1d", "tree_attention",
            "tree_masks", "window_prefill", "window_decode", "copy_kv_blocks", "commit_tree", "decode_workspace",
-           "prefill_workspace", "release_workspaces", "decode_schedule", "_lib"]
+           "prefill_workspace", "release_workspaces", "decode_schedule", "append_kvcache", "_lib"]
