@@ -768,6 +768,41 @@ int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride
                       int scale_block, int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                       void *stream);
 
+/*
+ * Attention over such a cache; any positive scales.  nq_paged_decode_auto without
+ * new rows, nq_varlen_prefill over the paged cache (causal; with window > 0 as
+ * nq_window_prefill, with 0 without one) and nq_window_decode without new rows:
+ * their arguments, with scale_block, and the same terms for `workspace`, `need`
+ * and `counters` (nq_decode_config and nq_decode_workspace_bytes with NQ_FP8_E4M3).
+ */
+int nq_paged_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                           const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                           int max_blocks_per_seq, const int32_t *context_lens, void *out, int64_t out_batch_stride,
+                           int64_t out_head_stride, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                           int block_size, int64_t num_blocks, float softmax_scale, int q_dtype, const float *k_scale,
+                           const float *v_scale, int scale_block, const void *gate, int64_t gate_batch_stride,
+                           int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, void *counters,
+                           int64_t counter_bytes, int64_t *need, void *stream);
+
+int nq_varlen_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+                             const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                             int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables, int64_t bt_stride,
+                             int max_blocks_per_seq, int64_t num_blocks, int window, int num_sinks, void *out,
+                             int64_t out_row_stride, int64_t out_head_stride, int num_seqs, int64_t total_q,
+                             int num_q_heads, int num_kv_heads, int head_dim, int block_size, float softmax_scale,
+                             int q_dtype, const float *k_scale, const float *v_scale, int scale_block,
+                             const void *gate, int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                             int64_t workspace_bytes, int64_t *need, void *stream);
+
+int nq_window_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                            const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                            int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks, void *out,
+                            int64_t out_batch_stride, int64_t out_head_stride, int batch, int num_q_heads,
+                            int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, float softmax_scale,
+                            int q_dtype, const float *k_scale, const float *v_scale, int scale_block,
+                            const void *gate, int64_t gate_batch_stride, int64_t gate_head_stride, void *workspace,
+                            int64_t workspace_bytes, int64_t *need, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

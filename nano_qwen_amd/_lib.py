@@ -124,6 +124,18 @@ _SIGS = {
     "nq_commit_tree": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p,
                                c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_void_p]),
+    "nq_paged_decode_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                       c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, c_float,
+                                       c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                       c_void_p, c_int64, POINTER(c_int64), c_void_p]),
+    "nq_varlen_prefill_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                         c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_int64,
+                                         c_int, c_int64, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p,
+                                         c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64), c_void_p]),
+    "nq_window_decode_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                        c_int, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int,
+                                        c_int64, c_float, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_int64, POINTER(c_int64), c_void_p]),
     "nq_append_kvcache": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                   c_int64, c_int, c_void_p, c_void_p, c_float, c_float, c_void_p, c_int64, c_int64,
                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,

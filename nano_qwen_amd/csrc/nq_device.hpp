@@ -407,6 +407,12 @@ inline int elem_size(int dtype) {
   }
 }
 
+// Tokens per scale that the kernels of caches with a scale for each block of
+// tokens and head are built for: a tile of 32 tokens lies in one block.
+inline bool block_scales_built(int tokens, int block_size) {
+  return (tokens == 32 || tokens == 64 || tokens == 128 || tokens == 256) && block_size > 0 && block_size % tokens == 0;
+}
+
 inline bool aligned(const void *p, int a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 }  // namespace nq

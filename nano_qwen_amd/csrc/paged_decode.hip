@@ -63,8 +63,9 @@ struct DecodeArgs {
   int64_t num_blocks;
   int split_tokens, num_splits;
   float scale_log2;
-  const float *k_scale;
+  const float *k_scale;  // per kv head; BLK: [num_blocks * block_size >> scale_shift, Hkv]
   const float *v_scale;
+  int scale_shift;  // BLK: log2 of the tokens of a block with one scale per head (32 or more)
   // Fused store of the new token (nq_paged_decode_store); k_new == null: none.
   const uint8_t *k_new;
   const uint8_t *v_new;
@@ -300,7 +301,13 @@ __device__ __forceinline__ float piece_lse(float m, float L) { return L == 0.f ?
 // for a merge pass.  STRIDE > 1: the wave takes steps first, first + STRIDE, ...
 // of a piece shared with other waves, and leaves its heads' maxima (log2
 // domain) and row sums in wm and wl and its O [head][dim] in its tile.
-template <class T, bool FP8, int D, int DEPTH, int STRIDE = 1>
+// BLK: a scale for each block of tokens and head; a step lies in one block.  With
+// w_j = 2^(sl2 k_scale s_j + log2 v_scale - m) the outputs are sum w_j c_j over
+// sum w_j / v_scale: V's scale costs an addend of the exponent's and a factor of
+// the sum's, and w_j, at most 1 whatever the scales, is rounded to 16 bits as p_j
+// is without them.  A step's two scales are loaded with its K and V, those
+// DEPTH steps ahead.
+template <class T, bool FP8, int D, int DEPTH, int STRIDE = 1, bool BLK = false>
 __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile, int b, int kvh, int t_begin,
                                              int t_end, bool single, int64_t ws_row, int64_t ws_head_stride,
                                              int first = 0, float *wm = nullptr, float *wl = nullptr) {
@@ -310,9 +317,9 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
   const int lane = threadIdx.x & 63;
   const int m = lane & 15, g = lane >> 4;  // m: token row / head column, g: lane group
   const int G = a.G;
-  const float kscale = FP8 ? a.k_scale[kvh] : 1.0f;
-  const float vscale = FP8 ? a.v_scale[kvh] : 1.0f;
-  const float sl2 = a.scale_log2 * kscale;
+  const float kscale = FP8 && !BLK ? a.k_scale[kvh] : 1.0f;
+  const float vscale = FP8 && !BLK ? a.v_scale[kvh] : 1.0f;
+  const float sl2_head = a.scale_log2 * kscale;
   const int32_t *bt_row = a.block_tables + b * a.bt_stride;
 
   // Q^T operand: lane (m, g) = head column m, dims 8(g + 4kk) .. +8.
@@ -355,10 +362,21 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
   }
   u32x4 kraw[DEPTH][Gm::RAW], vraw[DEPTH][Gm::RAW];
   int64_t rows[DEPTH];
+  // BLK: K's scale of a set's step in lanes 0 .. 31, V's in the others.  Loaded
+  // whatever the row, as K and V are: of the pool's first block where there is none.
+  float scales[DEPTH];
+  const float *const scale_of = BLK ? (lane < 32 ? a.k_scale : a.v_scale) + kvh : nullptr;
+  auto load_scales = [&](int64_t row) -> float {
+    if constexpr (BLK)
+      return scale_of[(max(row, int64_t{0}) >> a.scale_shift) * a.Hkv];
+    else
+      return 1.0f;
+  };
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) {
     const int td = t_begin + first * kStep + d * kNext;
     rows[d] = td < t_end ? W::step_row(a, bt_lane, first_blk, td) : -1;
+    scales[d] = load_scales(rows[d]);
     W::load(a.k_cache, a, rows[d], td, t_end, voff0, kraw[d]);
     W::load(a.v_cache, a, rows[d], td, t_end, voff0, vraw[d]);
   }
@@ -370,9 +388,18 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
 
   // One 32-token step on register set (kr, vr) holding tokens t0..t0+31 of
   // cache row `row`; returns the row of the step that refilled the set.
-  auto step = [&](int t0, int64_t row, u32x4 (&kr)[Gm::RAW], u32x4 (&vr)[Gm::RAW]) -> int64_t {
+  auto step = [&](int t0, int64_t row, u32x4 (&kr)[Gm::RAW], u32x4 (&vr)[Gm::RAW], float &sc) -> int64_t {
     const int tn = t0 + DEPTH * kNext;
     const int64_t rown = (tn < t_end) ? W::step_row(a, bt_lane, first_blk, tn) : -1;
+    float sl2 = sl2_head, lsv = 0.f, inv_sv = 1.f;
+    if constexpr (BLK) {
+      sl2 = a.scale_log2 * u2f(__builtin_amdgcn_readlane(f2u(sc), 0));
+      // (a scale of 0, of a block of zeros, would make 0 * inf of w / v_scale)
+      const float sv = fminf(fmaxf(u2f(__builtin_amdgcn_readlane(f2u(sc), 32)), 0x1p-100f), 0x1p100f);
+      lsv = __builtin_amdgcn_logf(sv);
+      inv_sv = __builtin_amdgcn_rcpf(sv);
+      sc = load_scales(rown);
+    }
     wave_lds_sync();  // the previous step's V^T reads are issued before the tile is overwritten
     W::stage(tile, kr, lane);
     if (t0 == sub_t0) W::patch_row(tile, nbuf, sub_row, lane);
@@ -396,7 +423,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
 #pragma unroll
       for (int rr = 0; rr < 4; ++rr) {
         const bool valid = row >= 0 && t0 + 16 * i + 4 * g + rr < t_end;
-        const float v = valid ? s[i][rr] * sl2 : kNegInf;
+        const float v = valid ? (BLK ? __builtin_fmaf(s[i][rr], sl2, lsv) : s[i][rr] * sl2) : kNegInf;
         x[4 * i + rr] = v;
         mloc = fmaxf(mloc, v);
       }
@@ -413,7 +440,7 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
       psum += p0 + p1;
       pw[t] = T::pack2(p0, p1);
     }
-    l_run = l_run * alpha + psum;
+    l_run = BLK ? __builtin_fmaf(psum, inv_sv, l_run * alpha) : l_run * alpha + psum;
     m_run = m_new;
     const u32x4 pb{pw[0], pw[1], pw[2], pw[3]};
     wave_lds_sync();  // V tile visible to every lane of the wave
@@ -426,10 +453,10 @@ __device__ __forceinline__ void decode_piece(const DecodeArgs &a, uint8_t *tile,
   };
 
   for (int t0 = t_begin + first * kStep; t0 < t_end; t0 += DEPTH * kNext) {
-    rows[0] = step(t0, rows[0], kraw[0], vraw[0]);
+    rows[0] = step(t0, rows[0], kraw[0], vraw[0], scales[0]);
     if constexpr (DEPTH > 1) {
       if (t0 + kNext >= t_end) break;
-      rows[1] = step(t0 + kNext, rows[1], kraw[1], vraw[1]);
+      rows[1] = step(t0 + kNext, rows[1], kraw[1], vraw[1], scales[1]);
     }
   }
 
@@ -493,7 +520,7 @@ __device__ __forceinline__ void decode_zero_row(const DecodeArgs &a, int b, int 
 // each wave owns its heads' softmax state.  The split index is the fastest
 // grid dimension: dispatching a sequence's splits together measured 6%
 // faster on cfg5 than all first splits first.
-template <class T, bool FP8, int D, int HPW, int DEPTH, int WPE>
+template <class T, bool FP8, int D, int HPW, int DEPTH, int WPE, bool BLK = false>
 __global__ __launch_bounds__(64 * HPW) __attribute__((amdgpu_waves_per_eu(WPE)))
 void paged_decode_kernel(const DecodeArgs a) {
   static_assert(DEPTH == 1 || DEPTH == 2, "prefetch depth");
@@ -515,9 +542,9 @@ void paged_decode_kernel(const DecodeArgs a) {
     return;
   }
   const int t_end = min(t_begin + a.split_tokens, ctx);
-  decode_piece<T, FP8, D, DEPTH>(a, smem + wave * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B, b, kvh, t_begin, t_end,
-                                 ctx <= a.split_tokens,
-                                 static_cast<int64_t>(b) * a.Hq * a.num_splits + split, a.num_splits);
+  decode_piece<T, FP8, D, DEPTH, 1, BLK>(a, smem + wave * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B, b, kvh, t_begin,
+                                         t_end, ctx <= a.split_tokens,
+                                         static_cast<int64_t>(b) * a.Hq * a.num_splits + split, a.num_splits);
 }
 
 // Partials of one (sequence, head) -- pieces 0 .. n - 1 -- merged by GR groups
@@ -672,7 +699,7 @@ __device__ __forceinline__ void store_merged(const DecodeArgs &a, int b, int hea
 // line one row of 4000 tokens took 224 against 207.)
 constexpr int kFusedWaves = 4;
 constexpr int kCounterBytes = 64;  // a counter per cache line: increments of one line are served one by one
-template <class T, bool FP8, int D, int DEPTH, int WPE>
+template <class T, bool FP8, int D, int DEPTH, int WPE, bool BLK = false>
 __global__ __launch_bounds__(64 * kFusedWaves) __attribute__((amdgpu_waves_per_eu(WPE)))
 void paged_decode_fused_kernel(const DecodeArgs a) {
   using Gm = Geo<D, FP8>;
@@ -693,9 +720,9 @@ void paged_decode_fused_kernel(const DecodeArgs a) {
   }
   const int t_end = min(t_begin + a.split_tokens, ctx);
   uint8_t *tile = smem + wave * Wv::LDS_PER_WAVE_B;
-  decode_piece<T, FP8, D, DEPTH, NW>(a, tile, b, kvh, t_begin, t_end, false, 0, 0, wave, wm[wave], wl[wave]);
+  decode_piece<T, FP8, D, DEPTH, NW, BLK>(a, tile, b, kvh, t_begin, t_end, false, 0, 0, wave, wm[wave], wl[wave]);
   __syncthreads();
-  const float vscale = FP8 ? a.v_scale[kvh] : 1.0f;
+  const float vscale = FP8 && !BLK ? a.v_scale[kvh] : 1.0f;
   const int n_split = (ctx + a.split_tokens - 1) / a.split_tokens;
   for (int e = threadIdx.x; e < a.G * kPer; e += 64 * NW) {
     const int h = e / kPer, d4 = e % kPer, head = kvh * a.G + h;
@@ -823,7 +850,7 @@ __device__ __forceinline__ int2 sk_boundary(const DecodeArgs &a, int batch, int 
 
 // At most two waves per SIMD: the piece loop's state does not fit the
 // register share of three (168 VGPRs) without spills.
-template <class T, bool FP8, int D, int HPW, int DEPTH, int WPE>
+template <class T, bool FP8, int D, int HPW, int DEPTH, int WPE, bool BLK = false>
 __global__ __launch_bounds__(64 * HPW) __attribute__((amdgpu_waves_per_eu(WPE)))
 void paged_decode_sk_kernel(const DecodeArgs a, int batch, int grid_w, int w_min) {
   static_assert(DEPTH == 1 || DEPTH == 2, "prefetch depth");
@@ -857,8 +884,8 @@ void paged_decode_sk_kernel(const DecodeArgs a, int batch, int grid_w, int w_min
     const int t1 = b == hi.x ? hi.y : ctx;
     if (t1 <= t0) continue;
     const int slot = t0 > 0 ? 0 : 1;
-    decode_piece<T, FP8, D, DEPTH>(a, tile, b, kvh, t0, t1, t0 == 0 && t1 == ctx,
-                                   (static_cast<int64_t>(w) * 2 + slot) * a.Hq, 1);
+    decode_piece<T, FP8, D, DEPTH, 1, BLK>(a, tile, b, kvh, t0, t1, t0 == 0 && t1 == ctx,
+                                           (static_cast<int64_t>(w) * 2 + slot) * a.Hq, 1);
   }
   store_rows();
 }
@@ -1047,17 +1074,17 @@ int sk_workgroups(int occ, int groups, int batch, int64_t max_tokens, int block_
 // kernel <T, FP8, D, H, DP, WP>, or 0 when it runs split-K: multi-split
 // plans that sk_eligible accepts, on a kernel with one resident workgroup per
 // CU, whose workspace holds the stream-K partials.
-template <class T, bool FP8, int D, int H, int DP, int WP>
+template <class T, bool FP8, int D, int H, int DP, int WP, bool BLK = false>
 int sk_ranges(int batch, int hq, int hkv, int64_t max_tokens, int block_size, int num_splits, int64_t ws_bytes) {
   if (num_splits <= 1 || !sk_eligible(batch, max_tokens, block_size)) return 0;
   const size_t lds = static_cast<size_t>(H) * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B;
-  auto *kern = paged_decode_sk_kernel<T, FP8, D, H, DP, (WP > 2 ? 2 : WP)>;
+  auto *kern = paged_decode_sk_kernel<T, FP8, D, H, DP, (WP > 2 ? 2 : WP), BLK>;
   if (kernel_occupancy(reinterpret_cast<const void *>(kern), 64 * H, lds) != 1) return 0;
   const int W = sk_workgroups(1, (hkv + H - 1) / H, batch, max_tokens, block_size);
   return sk_workspace_bytes(W, hq, D) <= ws_bytes ? W : 0;
 }
 
-template <class T, bool FP8, int D>
+template <class T, bool FP8, int D, bool BLK = false>
 struct DecodeLaunch {
   const DecodeArgs &a;
   int batch;
@@ -1067,16 +1094,16 @@ struct DecodeLaunch {
     if (a.counters) {
       constexpr size_t flds = static_cast<size_t>(kFusedWaves) * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B;
       const int64_t covers = (static_cast<int64_t>(a.max_tokens) + a.split_tokens - 1) / a.split_tokens;
-      paged_decode_fused_kernel<T, FP8, D, DP, (D == 256 ? 1 : 2)>
+      paged_decode_fused_kernel<T, FP8, D, DP, (D == 256 ? 1 : 2), BLK>
           <<<dim3(a.Hkv, static_cast<int>(covers), batch), 64 * kFusedWaves, flds, s>>>(a);
       return check_launch("paged_decode(one launch)");
     }
     const int groups = (a.Hkv + H - 1) / H;
     const size_t lds = static_cast<size_t>(H) * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B;
-    auto *kern = paged_decode_sk_kernel<T, FP8, D, H, DP, (WP > 2 ? 2 : WP)>;
+    auto *kern = paged_decode_sk_kernel<T, FP8, D, H, DP, (WP > 2 ? 2 : WP), BLK>;
     {
-      const int W = sk_ranges<T, FP8, D, H, DP, WP>(batch, a.Hq, a.Hkv, a.max_tokens, a.block_size, a.num_splits,
-                                                    a.ws_raw ? a.ws_bytes : 0);
+      const int W = sk_ranges<T, FP8, D, H, DP, WP, BLK>(batch, a.Hq, a.Hkv, a.max_tokens, a.block_size, a.num_splits,
+                                                         a.ws_raw ? a.ws_bytes : 0);
       if (W > 0) {
         DecodeArgs k = a;
         k.ws_o = reinterpret_cast<float *>(a.ws_raw);
@@ -1097,7 +1124,7 @@ struct DecodeLaunch {
     // stream-K partials of another head_dim): no workgroups for them.
     const int64_t cover = (static_cast<int64_t>(a.max_tokens) + a.split_tokens - 1) / a.split_tokens;
     const int nsplit = static_cast<int>(std::min<int64_t>(a.num_splits, cover));
-    paged_decode_kernel<T, FP8, D, H, DP, WP><<<dim3(nsplit, groups, batch), 64 * H, lds, s>>>(a);
+    paged_decode_kernel<T, FP8, D, H, DP, WP, BLK><<<dim3(nsplit, groups, batch), 64 * H, lds, s>>>(a);
     const int rc = check_launch("paged_decode");
     if (rc != NQ_OK || a.num_splits <= 1) return rc;
     if (nsplit <= kMergeUnroll)
@@ -1132,9 +1159,9 @@ struct DecodeSchedule {
   }
 };
 
-template <class T, bool FP8, int D>
+template <class T, bool FP8, int D, bool BLK = false>
 int launch_decode(const DecodeArgs &a, int batch, hipStream_t s) {
-  return with_decode_shape<FP8, D>(decode_hpw<FP8, D>(a.Hkv), DecodeLaunch<T, FP8, D>{a, batch, s});
+  return with_decode_shape<FP8, D>(decode_hpw<FP8, D>(a.Hkv), DecodeLaunch<T, FP8, D, BLK>{a, batch, s});
 }
 
 // Stream-K workgroups per group the head_dim-D kernel would launch for
@@ -1268,7 +1295,7 @@ static int paged_decode_impl(const void *q, int64_t q_batch_stride, int64_t q_he
                              int64_t gate_batch_stride, int64_t gate_head_stride, void *stream,
                              const void *k_new = nullptr, int64_t k_new_row_stride = 0, const void *v_new = nullptr,
                              int64_t v_new_row_stride = 0, const int32_t *slot_mapping = nullptr,
-                             int new_dtype = -1, void *counters = nullptr) {
+                             int new_dtype = -1, void *counters = nullptr, int scale_block = 0) {
   if (batch == 0) return NQ_OK;
   if (batch < 0 || batch > 65535 || num_q_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535)
     return fail(NQ_EINVAL, "paged_decode: bad batch/head counts");
@@ -1287,6 +1314,9 @@ static int paged_decode_impl(const void *q, int64_t q_batch_stride, int64_t q_he
   if (!fp8 && kv_dtype != q_dtype)
     return fail(NQ_EUNSUPPORTED, "paged_decode: kv dtype %d with q dtype %d", kv_dtype, q_dtype);
   if (fp8 && (!k_scale || !v_scale)) return fail(NQ_EINVAL, "paged_decode: fp8 cache needs scales");
+  if (scale_block != 0 && (!fp8 || num_blocks <= 0 || !block_scales_built(scale_block, block_size)))
+    return fail(NQ_EUNSUPPORTED, "paged_decode: a scale per %d tokens in pages of %d, kv dtype %d", scale_block, block_size,
+                kv_dtype);
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out)
     return fail(NQ_EINVAL, "paged_decode: null pointer");
   if (max_blocks_per_seq <= 0 || bt_stride < max_blocks_per_seq)
@@ -1363,6 +1393,12 @@ static int paged_decode_impl(const void *q, int64_t q_batch_stride, int64_t q_he
   }
   a.counters = static_cast<unsigned *>(counters);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (scale_block != 0) {
+    a.scale_shift = __builtin_ctz(static_cast<unsigned>(scale_block));
+    if (q_dtype == NQ_BF16)
+      return head_dim == 256 ? launch_decode<BF16, true, 256, true>(a, batch, s) : launch_decode<BF16, true, 128, true>(a, batch, s);
+    return head_dim == 256 ? launch_decode<F16, true, 256, true>(a, batch, s) : launch_decode<F16, true, 128, true>(a, batch, s);
+  }
   if (q_dtype == NQ_BF16)
     return head_dim == 256
                ? (fp8 ? launch_decode<BF16, true, 256>(a, batch, s) : launch_decode<BF16, false, 256>(a, batch, s))
@@ -1498,7 +1534,7 @@ extern "C" int nq_paged_decode_fused(const void *q, int64_t q_batch_stride, int6
                            v_new, v_new_row_stride, slot_mapping, new_dtype, counters);
 }
 
-extern "C" int nq_paged_decode_auto(const void *q, int64_t q_batch_stride, int64_t q_head_stride,
+static int decode_auto(const void *q, int64_t q_batch_stride, int64_t q_head_stride,
                                     void *k_cache, void *v_cache, const int32_t *block_tables, int64_t bt_stride,
                                     int max_blocks_per_seq, const int32_t *context_lens, const void *k_new,
                                     int64_t k_new_row_stride, const void *v_new, int64_t v_new_row_stride,
@@ -1508,7 +1544,7 @@ extern "C" int nq_paged_decode_auto(const void *q, int64_t q_batch_stride, int64
                                     int64_t num_blocks, float softmax_scale, void *workspace,
                                     int64_t workspace_bytes, int q_dtype, int kv_dtype, const float *k_scale,
                                     const float *v_scale, const void *gate, int64_t gate_batch_stride,
-                                    int64_t gate_head_stride, void *counters, int64_t counter_bytes, int64_t *need,
+                                    int64_t gate_head_stride, int scale_block, void *counters, int64_t counter_bytes, int64_t *need,
                                     void *stream) {
   int64_t config[4];
   int rc = nq_decode_config(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq, block_size, kv_dtype, config);
@@ -1531,7 +1567,44 @@ extern "C" int nq_paged_decode_auto(const void *q, int64_t q_batch_stride, int64
                            num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, softmax_scale,
                            ns, st, workspace, workspace_bytes, q_dtype, kv_dtype, k_scale,
                            v_scale, gate, gate_batch_stride, gate_head_stride, stream, k_new, k_new_row_stride,
-                           v_new, v_new_row_stride, slot_mapping, new_dtype, fused ? counters : nullptr);
+                           v_new, v_new_row_stride, slot_mapping, new_dtype, fused ? counters : nullptr, scale_block);
+}
+
+extern "C" int nq_paged_decode_auto(const void *q, int64_t q_batch_stride, int64_t q_head_stride,
+                                    void *k_cache, void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                                    int max_blocks_per_seq, const int32_t *context_lens, const void *k_new,
+                                    int64_t k_new_row_stride, const void *v_new, int64_t v_new_row_stride,
+                                    const int32_t *slot_mapping, int new_dtype, void *out,
+                                    int64_t out_batch_stride, int64_t out_head_stride, int batch,
+                                    int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                    int64_t num_blocks, float softmax_scale, void *workspace,
+                                    int64_t workspace_bytes, int q_dtype, int kv_dtype, const float *k_scale,
+                                    const float *v_scale, const void *gate, int64_t gate_batch_stride,
+                                    int64_t gate_head_stride, void *counters, int64_t counter_bytes, int64_t *need,
+                                    void *stream) {
+  return decode_auto(q, q_batch_stride, q_head_stride, k_cache, v_cache, block_tables, bt_stride, max_blocks_per_seq,
+                     context_lens, k_new, k_new_row_stride, v_new, v_new_row_stride, slot_mapping, new_dtype, out,
+                     out_batch_stride, out_head_stride, batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+                     softmax_scale, workspace, workspace_bytes, q_dtype, kv_dtype, k_scale, v_scale, gate,
+                     gate_batch_stride, gate_head_stride, 0, counters, counter_bytes, need, stream);
+}
+
+extern "C" int nq_paged_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                                      const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                                      int max_blocks_per_seq, const int32_t *context_lens, void *out,
+                                      int64_t out_batch_stride, int64_t out_head_stride, int batch, int num_q_heads,
+                                      int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                                      float softmax_scale, int q_dtype, const float *k_scale, const float *v_scale,
+                                      int scale_block, const void *gate, int64_t gate_batch_stride,
+                                      int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, void *counters,
+                                      int64_t counter_bytes, int64_t *need, void *stream) {
+  if (scale_block <= 0) return fail(NQ_EUNSUPPORTED, "paged_decode_blocks: blocks of %d tokens", scale_block);
+  if (batch == 0) return NQ_OK;
+  return decode_auto(q, q_batch_stride, q_head_stride, const_cast<void *>(k_cache), const_cast<void *>(v_cache),
+                     block_tables, bt_stride, max_blocks_per_seq, context_lens, nullptr, 0, nullptr, 0, nullptr, -1, out,
+                     out_batch_stride, out_head_stride, batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+                     softmax_scale, workspace, workspace_bytes, q_dtype, NQ_FP8_E4M3, k_scale, v_scale, gate,
+                     gate_batch_stride, gate_head_stride, scale_block, counters, counter_bytes, need, stream);
 }
 
 // ---------------------------------------------------------------------------

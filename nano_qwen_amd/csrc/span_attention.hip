@@ -93,7 +93,7 @@ struct SpanArgs {
   int64_t mask_rs;
   int words;
   float scale_log2;
-  const float *k_scale;
+  const float *k_scale;  // per kv head; BLK: [num_blocks * tiles of a page >> scale_shift, Hkv]
   const float *v_scale;
   // Decode: the new token's rows to store [num_seqs, Hkv, D] (null: none), of type new_dtype.
   const uint8_t *k_new;
@@ -109,6 +109,7 @@ struct SpanArgs {
   float *part_o;
   float *part_l;
   int4 *part_desc;  // (sequence, row tile, kind, 0)
+  int scale_shift;  // BLK: log2 of the tiles of a block with one scale per head
 };
 constexpr int kPieceNone = -1, kPieceMore = 0, kPieceLast = 1;
 
@@ -244,7 +245,13 @@ __device__ __forceinline__ int item_cost(const A &a, const Seq &q) {
 }
 
 // ---------------------------------------------------------------- the kernel
-template <class T, bool FP8, class S>
+// BLK: fp8 K/V with a scale for each block of tokens and head, paged, no trees.  A
+// tile lies in one block.  With w_j = 2^(sl2 k_scale s_j + log2 v_scale - m) the
+// outputs are sum w_j c_j over sum w_j / v_scale, so that P is w: V's scale costs
+// an addend of the exponent's fma and a factor of the sum's, and w <= 2^kRescale
+// whatever the scales.  The scales of a tile go with its copies: 64 tiles' with
+// the list of where they lie, then, per ring slot, to a lane of ring_k and ring_v.
+template <class T, bool FP8, class S, bool BLK>
 __device__ __forceinline__ void span_body() {
   constexpr int D = S::D, RW = S::RW, QS = S::QS, M = S::M, SLOTS = S::SLOTS, COPS = S::COPS;
   constexpr int NKK = S::NKK, NJ = S::NJ, TILE_B = S::TILE_B, SLOT_B = S::SLOT_B, SRC_ROWB = S::SRC_ROWB;
@@ -445,6 +452,8 @@ __device__ __forceinline__ void span_body() {
   int nx_list = 0, nx_left = 0, nx_at = 0, nx_first = 0;
   const uint8_t *nx_base = a0.k;
   uint32_t nx_last = 0;
+  float st_ks = 1.f, st_vs = 1.f, nx_ks = 1.f, nx_vs = 1.f;  // BLK: the lists' tiles' scales
+  float ring_k = 1.f, ring_v = 1.f;                          // BLK: lane e % SLOTS: of entry e
   bool bad_seen = false;  // some tile lay in a missing page: from then on every tile is looked up
   auto list_of = [&](KernArgs &a, const Item &it, int chunk) -> int {
     const int i = it.lo + 64 * chunk + lane;
@@ -461,11 +470,19 @@ __device__ __forceinline__ void span_body() {
     bad_seen = uni(bad_seen | (__builtin_amdgcn_ballot_w64(at < 0) != 0)) != 0;
     return at;
   };
+  auto scales_of = [&](KernArgs &a, int at, float &ks, float &vs) {
+    if constexpr (BLK) {
+      const int64_t i = static_cast<int64_t>(max(at, 0) >> a.scale_shift) * a.Hkv + h;
+      ks = a.k_scale[i];
+      vs = a.v_scale[i];
+    }
+  };
   auto queue = [&](const Item &it) {
     nx_queued = it.live && it.hi > it.lo;
     if (!nx_queued) return;
     KernArgs &a = *kernel_args();
     nx_list = list_of(a, it, 0);
+    scales_of(a, nx_list, nx_ks, nx_vs);
     nx_at = it.at;
     nx_left = uni(it.hi - it.lo);
     nx_base = a.k + (paged ? 0 : static_cast<int64_t>(it.q.k0) * kv_rs) + h * SRC_ROWB;
@@ -480,6 +497,8 @@ __device__ __forceinline__ void span_body() {
       nx_queued = false;
       nx_first = st_pos;
       st_list = nx_list;
+      st_ks = nx_ks;
+      st_vs = nx_vs;
       st_l = 0;
       st_left = nx_left;
       st_at = nx_at;
@@ -493,11 +512,17 @@ __device__ __forceinline__ void span_body() {
       ++st_chunk;
       st_l = 0;
       st_list = list_of(*kernel_args(), describe(st_at), st_chunk);
+      scales_of(*kernel_args(), st_list, st_ks, st_vs);
       // (here, where the list is needed at once: a load that the compiler cannot
       // see waited for on every path, it waits for in the loop, with the copies)
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     }
     const int at = __builtin_amdgcn_readlane(st_list, st_l);
+    if constexpr (BLK) {
+      const bool here = lane == ((st_pos - 1) & (SLOTS - 1));
+      ring_k = here ? u2f(__builtin_amdgcn_readlane(f2u(st_ks), st_l)) : ring_k;
+      ring_v = here ? u2f(__builtin_amdgcn_readlane(f2u(st_vs), st_l)) : ring_v;
+    }
     src = st_base + static_cast<int64_t>(static_cast<uint32_t>(max(at, 0))) * static_cast<uint32_t>(kKeys * kv_rs);
     nrec = at < 0 ? 0u : st_left == 1 ? st_last : static_cast<uint32_t>(kKeys * kv_rs);
     ++st_l;
@@ -566,7 +591,19 @@ __device__ __forceinline__ void span_body() {
   auto unhoist = [&]() { asm volatile("" : "+v"(kx_l), "+v"(vx_l)); };
 
   // (never 0: a masked score, -inf, must stay that under a scale of 0)
-  const float sl2 = FP8 ? fmaxf(a0.scale_log2 * ld_const(a0.k_scale + h), 0x1p-126f) : a0.scale_log2;
+  const float sl2_head = FP8 && !BLK ? fmaxf(a0.scale_log2 * ld_const(a0.k_scale + h), 0x1p-126f) : a0.scale_log2;
+  float sl2 = sl2_head, lsv = 0.f, inv_sv = 1.f;  // BLK: of the tile whose P is formed
+  auto tile_scales = [&](int entry) {
+    if constexpr (BLK) {
+      static_assert((SLOTS & (SLOTS - 1)) == 0, "ring slots by mask");
+      const int e = entry & (SLOTS - 1);
+      sl2 = fmaxf(sl2_head * u2f(__builtin_amdgcn_readlane(f2u(ring_k), e)), 0x1p-126f);
+      // (a scale of 0, of a block of zeros, would make 0 * inf of w / v_scale)
+      const float sv = fminf(fmaxf(u2f(__builtin_amdgcn_readlane(f2u(ring_v), e)), 0x1p-100f), 0x1p100f);
+      lsv = __builtin_amdgcn_logf(sv);
+      inv_sv = __builtin_amdgcn_rcpf(sv);
+    }
+  };
 
   constexpr int kAhead = RW == 1 ? SLOTS : SLOTS - 1;
   const uint8_t *src;
@@ -628,7 +665,7 @@ __device__ __forceinline__ void span_body() {
     }
     if (cur.live) queue(describe(cur.next));
     if (done.live) {
-      const float vscale = FP8 ? ld_const(a.v_scale + h) : 1.f;
+      const float vscale = FP8 && !BLK ? ld_const(a.v_scale + h) : 1.f;
       // lane (m, g) holds dims 16 j + 4 g .. +3 of row 16 qs + m
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
@@ -690,6 +727,7 @@ __device__ __forceinline__ void span_body() {
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
       asm volatile("" : "+v"(nx_list));
+      if constexpr (BLK) asm volatile("" : "+v"(nx_ks), "+v"(nx_vs));
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
         m_use[qs] = kNegInf;
@@ -798,7 +836,8 @@ __device__ __forceinline__ void span_body() {
         for (int qs = 0; qs < QS; ++qs) {
           mloc[qs] = max3(max3(sc[qs][0][0], sc[qs][0][1], sc[qs][0][2]),
                           max3(sc[qs][0][3], sc[qs][1][0], sc[qs][1][1]),
-                          __builtin_elementwise_maximum(sc[qs][1][2], sc[qs][1][3])) * sl2;
+                          __builtin_elementwise_maximum(sc[qs][1][2], sc[qs][1][3]));
+          mloc[qs] = BLK ? __builtin_fmaf(mloc[qs], sl2, lsv) : mloc[qs] * sl2;
           grow |= mloc[qs] > m_use[qs] + kRescale;
         }
         if (__builtin_amdgcn_ballot_w64(grow) == 0) return false;
@@ -820,9 +859,10 @@ __device__ __forceinline__ void span_body() {
       };
       // Elements 2 t, 2 t + 1 of a row block: P, its sum, packed.
       auto p_unit = [&](int qs, int t) -> uint32_t {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -mref[qs]));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -mref[qs]));
-        lsum[qs] += e0 + e1;
+        const float at0 = BLK ? lsv - mref[qs] : -mref[qs];
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, at0));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, at0));
+        lsum[qs] = BLK ? __builtin_fmaf(e0 + e1, inv_sv, lsum[qs]) : lsum[qs] + (e0 + e1);
         return T::pack2(e0, e1);
       };
       auto scores = [&](uint32_t kt) {
@@ -944,7 +984,7 @@ __device__ __forceinline__ void span_body() {
         // attention need no order.
         uint8_t *const lds_new = smem + S::NEW_AT;
         int new_row = -1;  // of the last tile
-        if (a.k_new && hi == tl.n) {
+        if (!BLK && a.k_new && hi == tl.n) {
           const int slot_of = ld_const(a.slot_mapping + q.s), have = ld_const(a.cu_k + q.s);
           if (n > 0 && have == q.Lk) {
             const int at = q.Lk - 1, e = small_div(at / kKeys, a.block_size / kKeys);
@@ -1007,6 +1047,7 @@ __device__ __forceinline__ void span_body() {
           if (patched) patch(slot, false);
           scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
+          tile_scales(p0 + i - lo);
           const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && !bad_seen;
           if (!whole_tile) mask_tile(i, true);
           next_tile(src, nrec);
@@ -1044,6 +1085,7 @@ __device__ __forceinline__ void span_body() {
         auto step = [&](auto first_tag, int i) {
           constexpr bool FIRST = decltype(first_tag)::value;
           unhoist();
+          tile_scales(p0 + i - lo);
           if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
           const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && !bad_seen;
           if (!whole_tile) mask_tile(i, wave_live);
@@ -1219,10 +1261,10 @@ __device__ __forceinline__ void span_body() {
   wait_vmcnt<0>();  // no copy outlives the workgroup's LDS
 }
 
-template <class T, bool FP8, class S>
+template <class T, bool FP8, class S, bool BLK>
 __global__ __launch_bounds__(64 * S::RW) __attribute__((amdgpu_waves_per_eu(S::RW == 1 ? 1 : 2)))
 void span_attention_kernel(const SpanArgs a) {
-  span_body<T, FP8, S>();
+  span_body<T, FP8, S, BLK>();
 }
 
 // Merge of the items that ranges cut: workgroup (range, part) takes the item
@@ -1341,7 +1383,7 @@ __global__ __launch_bounds__(256) void span_merge_kernel(const SpanArgs a) {
 // ---------------------------------------------------------------- launch
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
-template <class T, bool FP8, class S>
+template <class T, bool FP8, bool BLK, class S>
 int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t workspace_bytes, int64_t *need,
            hipStream_t stream) {
   // row tiles of the batch, at most: every sequence's last one may be partial
@@ -1385,7 +1427,7 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
     a.part_o = reinterpret_cast<float *>(ws);
     a.part_l = reinterpret_cast<float *>(ws + o_bytes);
     a.part_desc = reinterpret_cast<int4 *>(ws + o_bytes + l_bytes);
-    span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(W * a.Hkv)), 64 * S::RW, S::LDS_B, stream>>>(a);
+    span_attention_kernel<T, FP8, S, BLK><<<dim3(static_cast<unsigned>(W * a.Hkv)), 64 * S::RW, S::LDS_B, stream>>>(a);
     const int rc = check_launch("span attention");
     if (rc != NQ_OK || W <= 1) return rc;
     const unsigned n_wg = static_cast<unsigned>(W * a.Hkv);
@@ -1406,11 +1448,11 @@ int launch(SpanArgs a, int64_t max_rows, int per_cu, void *workspace, int64_t wo
   const int64_t unit = static_cast<int64_t>(a.Hkv) * per;
   const int64_t grid = unit * std::max<int64_t>(1, std::min((items + per - 1) / per, slots / unit));
   a.stride = static_cast<int>(grid / a.Hkv);
-  span_attention_kernel<T, FP8, S><<<dim3(static_cast<unsigned>(grid)), 64 * S::RW, S::LDS_B, stream>>>(a);
+  span_attention_kernel<T, FP8, S, BLK><<<dim3(static_cast<unsigned>(grid)), 64 * S::RW, S::LDS_B, stream>>>(a);
   return check_launch("span attention");
 }
 
-template <class T, bool FP8>
+template <class T, bool FP8, bool BLK = false>
 int launch_shape(const SpanArgs &a, int D, int64_t max_rows, void *ws, int64_t ws_bytes, int64_t *need, hipStream_t s) {
   // The smallest shape that holds the longest sequence's rows.  One row block in
   // the four waves' shape: decode of 32 rows of 4096 tokens 110 us against 107, of
@@ -1418,21 +1460,21 @@ int launch_shape(const SpanArgs &a, int D, int64_t max_rows, void *ws, int64_t w
   // sequences of 4096 61 against 59, fp8 64 against 50 (D = 256: 67 against 59).
   if (D == 256) {
     if (max_rows <= 16)
-      return launch<T, FP8, Shape<256, FP8, 1, 1, 2>>(a, max_rows, FP8 ? 4 : 2, ws, ws_bytes, need, s);
+      return launch<T, FP8, BLK, Shape<256, FP8, 1, 1, 2>>(a, max_rows, FP8 ? 4 : 2, ws, ws_bytes, need, s);
     if (max_rows <= 64)
-      return launch<T, FP8, Shape<256, FP8, 4, 1, 4>>(a, max_rows, FP8 ? 2 : 1, ws, ws_bytes, need, s);
-    return launch<T, FP8, Shape<256, FP8, 8, 1, 4>>(a, max_rows, 1, ws, ws_bytes, need, s);
+      return launch<T, FP8, BLK, Shape<256, FP8, 4, 1, 4>>(a, max_rows, FP8 ? 2 : 1, ws, ws_bytes, need, s);
+    return launch<T, FP8, BLK, Shape<256, FP8, 8, 1, 4>>(a, max_rows, 1, ws, ws_bytes, need, s);
   }
   if (max_rows <= 16)
-    return launch<T, FP8, Shape<128, FP8, 1, 1, FP8 ? 4 : 2>>(a, max_rows, 4, ws, ws_bytes, need, s);
-  if (max_rows <= 64) return launch<T, FP8, Shape<128, FP8, 4, 1, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
-  return launch<T, FP8, Shape<128, FP8, 4, 2, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
+    return launch<T, FP8, BLK, Shape<128, FP8, 1, 1, FP8 ? 4 : 2>>(a, max_rows, 4, ws, ws_bytes, need, s);
+  if (max_rows <= 64) return launch<T, FP8, BLK, Shape<128, FP8, 4, 1, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
+  return launch<T, FP8, BLK, Shape<128, FP8, 4, 2, 4>>(a, max_rows, 2, ws, ws_bytes, need, s);
 }
 
 // What the three entry points share: checks and the launch of `a`, whose
 // pointers, byte strides and mode are set.
 int run(const char *what, SpanArgs a, int head_dim, int64_t max_rows, int q_dtype, int kv_dtype, void *workspace,
-        int64_t workspace_bytes, int64_t *need, void *stream) {
+        int64_t workspace_bytes, int64_t *need, void *stream, int scale_block = 0) {
   const bool fp8 = kv_dtype == NQ_FP8_E4M3;
   if (a.num_seqs < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hkv > 65535 || a.total_q < 0)
     return fail(NQ_EINVAL, "%s: bad sequence or head counts", what);
@@ -1447,9 +1489,15 @@ int run(const char *what, SpanArgs a, int head_dim, int64_t max_rows, int q_dtyp
   if (!fp8 && kv_dtype != q_dtype)
     return fail(NQ_EUNSUPPORTED, "%s: kv dtype %d with q dtype %d", what, kv_dtype, q_dtype);
   if (fp8 && (!a.k_scale || !a.v_scale)) return fail(NQ_EINVAL, "%s: fp8 K/V needs scales", what);
+  if (scale_block != 0) {  // the caller's mode is a window over paged fp8 K/V without new rows
+    if (!block_scales_built(scale_block, a.block_size))
+      return fail(NQ_EUNSUPPORTED, "%s: a scale per %d tokens in pages of %d", what, scale_block, a.block_size);
+    a.scale_shift = __builtin_ctz(static_cast<unsigned>(scale_block / kKeys));
+  }
   if (!(a.scale_log2 > 0.f)) return fail(NQ_EINVAL, "%s: softmax_scale must be positive", what);
   if (a.num_seqs == 0 || a.total_q == 0) return NQ_OK;
-  if (!a.q || !a.k || !a.v || !a.cu_k || !a.out) return fail(NQ_EINVAL, "%s: null pointer", what);
+  if (!a.q || !a.k || !a.v || !a.cu_k || !a.out || (scale_block != 0 && (!a.block_tables || a.num_blocks <= 0)))
+    return fail(NQ_EINVAL, "%s: null pointer", what);
   if (a.block_tables) {
     if (a.block_size <= 0 || a.block_size % kKeys != 0 || a.block_size > 1 << 26)
       return fail(NQ_EUNSUPPORTED, "%s: block_size %d must be a multiple of 32", what, a.block_size);
@@ -1469,6 +1517,9 @@ int run(const char *what, SpanArgs a, int head_dim, int64_t max_rows, int q_dtyp
     return fail(NQ_EINVAL, "%s: %lld rows per kv head", what, (long long)max_rows);
   if (a.max_k < 0 || a.max_k >= 1 << 26) return fail(NQ_EINVAL, "%s: %d tokens in a sequence", what, a.max_k);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (scale_block != 0)
+    return q_dtype == NQ_BF16 ? launch_shape<BF16, true, true>(a, head_dim, max_rows, workspace, workspace_bytes, need, s)
+                              : launch_shape<F16, true, true>(a, head_dim, max_rows, workspace, workspace_bytes, need, s);
   if (q_dtype == NQ_BF16)
     return fp8 ? launch_shape<BF16, true>(a, head_dim, max_rows, workspace, workspace_bytes, need, s)
                : launch_shape<BF16, false>(a, head_dim, max_rows, workspace, workspace_bytes, need, s);
@@ -1536,7 +1587,7 @@ extern "C" int nq_tree_attention(const void *q, int64_t q_row_stride, int64_t q_
              q_dtype, kv_dtype, workspace, workspace_bytes, need, stream);
 }
 
-extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+static int window_prefill(const char *what, int scale_block, const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
                                  const void *v, int64_t kv_row_stride, int64_t total_k, const int32_t *cu_seqlens_q,
                                  const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
                                  const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,
@@ -1546,7 +1597,6 @@ extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_
                                  int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
                                  int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
                                  int64_t workspace_bytes, int64_t *need, void *stream) {
-  const char *what = "window_prefill";
   if (window <= 0 || num_sinks < 0) return fail(NQ_EINVAL, "%s: window %d, sinks %d", what, window, num_sinks);
   if (num_seqs > 0 && total_q > 0 && !cu_seqlens_q) return fail(NQ_EINVAL, "%s: null pointer", what);
   if (total_q > 0x7fffffff || total_k > 0x7fffffff || max_seqlen_q < 0)
@@ -1590,10 +1640,47 @@ extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   return run(what, a, head_dim, static_cast<int64_t>(max_seqlen_q) * (num_kv_heads > 0 ? num_q_heads / num_kv_heads : 1),
-             q_dtype, kv_dtype, workspace, workspace_bytes, need, stream);
+             q_dtype, kv_dtype, workspace, workspace_bytes, need, stream, scale_block);
 }
 
-extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, void *k_cache,
+extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
+                                 const void *v, int64_t kv_row_stride, int64_t total_k, const int32_t *cu_seqlens_q,
+                                 const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
+                                 const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                                 int64_t num_blocks, int window, int num_sinks, void *out, int64_t out_row_stride,
+                                 int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                                 int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                                 int kv_dtype, const float *k_scale, const float *v_scale, const void *gate,
+                                 int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                                 int64_t workspace_bytes, int64_t *need, void *stream) {
+  return window_prefill("window_prefill", 0, q, q_row_stride, q_head_stride, k, v, kv_row_stride, total_k, cu_seqlens_q,
+                        cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables, bt_stride, max_blocks_per_seq, num_blocks,
+                        window, num_sinks, out, out_row_stride, out_head_stride, num_seqs, total_q, num_q_heads,
+                        num_kv_heads, head_dim, block_size, softmax_scale, q_dtype, kv_dtype, k_scale, v_scale, gate,
+                        gate_row_stride, gate_head_stride, workspace, workspace_bytes, need, stream);
+}
+
+extern "C" int nq_varlen_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+                                        const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                        int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables,
+                                        int64_t bt_stride, int max_blocks_per_seq, int64_t num_blocks, int window,
+                                        int num_sinks, void *out, int64_t out_row_stride, int64_t out_head_stride,
+                                        int num_seqs, int64_t total_q, int num_q_heads, int num_kv_heads, int head_dim,
+                                        int block_size, float softmax_scale, int q_dtype, const float *k_scale,
+                                        const float *v_scale, int scale_block, const void *gate, int64_t gate_row_stride,
+                                        int64_t gate_head_stride, void *workspace, int64_t workspace_bytes,
+                                        int64_t *need, void *stream) {
+  const char *what = "varlen_prefill_blocks";
+  if (scale_block <= 0) return fail(NQ_EUNSUPPORTED, "%s: blocks of %d tokens", what, scale_block);
+  return window_prefill(what, scale_block, q, q_row_stride, q_head_stride, k_cache, v_cache, 0, 0, cu_seqlens_q,
+                        cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables, bt_stride, max_blocks_per_seq, num_blocks,
+                        window == 0 ? INT32_MAX : window, num_sinks, out, out_row_stride, out_head_stride, num_seqs,
+                        total_q, num_q_heads, num_kv_heads, head_dim, block_size, softmax_scale, q_dtype, NQ_FP8_E4M3,
+                        k_scale, v_scale, gate, gate_row_stride, gate_head_stride, workspace, workspace_bytes, need,
+                        stream);
+}
+
+static int window_decode(const char *what, int scale_block, const void *q, int64_t q_batch_stride, int64_t q_head_stride, void *k_cache,
                                 void *v_cache, const int32_t *block_tables, int64_t bt_stride,
                                 int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
                                 const void *k_new, int64_t k_new_row_stride, const void *v_new,
@@ -1603,7 +1690,6 @@ extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q
                                 const float *v_scale, const void *gate, int64_t gate_batch_stride,
                                 int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,
                                 void *stream) {
-  const char *what = "window_decode";
   if (window <= 0 || num_sinks < 0) return fail(NQ_EINVAL, "%s: window %d, sinks %d", what, window, num_sinks);
   if (batch > 0 && !block_tables) return fail(NQ_EINVAL, "%s: null pointer", what);
   const int64_t new_size = elem_size(new_dtype), row = static_cast<int64_t>(num_kv_heads) * head_dim;
@@ -1654,5 +1740,42 @@ extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   return run(what, a, head_dim, num_kv_heads > 0 ? num_q_heads / num_kv_heads : 1, q_dtype, kv_dtype, workspace,
-             workspace_bytes, need, stream);
+             workspace_bytes, need, stream, scale_block);
+}
+
+extern "C" int nq_window_decode(const void *q, int64_t q_batch_stride, int64_t q_head_stride, void *k_cache,
+                                void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                                int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
+                                const void *k_new, int64_t k_new_row_stride, const void *v_new,
+                                int64_t v_new_row_stride, const int32_t *slot_mapping, int new_dtype, void *out,
+                                int64_t out_batch_stride, int64_t out_head_stride, int batch, int num_q_heads, int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+                                float softmax_scale, int q_dtype, int kv_dtype, const float *k_scale,
+                                const float *v_scale, const void *gate, int64_t gate_batch_stride,
+                                int64_t gate_head_stride, void *workspace, int64_t workspace_bytes, int64_t *need,
+                                void *stream) {
+  return window_decode("window_decode", 0, q, q_batch_stride, q_head_stride, k_cache, v_cache, block_tables, bt_stride,
+                       max_blocks_per_seq, context_lens, window, num_sinks, k_new, k_new_row_stride, v_new,
+                       v_new_row_stride, slot_mapping, new_dtype, out, out_batch_stride, out_head_stride, batch,
+                       num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, softmax_scale, q_dtype, kv_dtype,
+                       k_scale, v_scale, gate, gate_batch_stride, gate_head_stride, workspace, workspace_bytes, need,
+                       stream);
+}
+
+extern "C" int nq_window_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
+                                       const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
+                                       int max_blocks_per_seq, const int32_t *context_lens, int window, int num_sinks,
+                                       void *out, int64_t out_batch_stride, int64_t out_head_stride, int batch,
+                                       int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                       int64_t num_blocks, float softmax_scale, int q_dtype, const float *k_scale,
+                                       const float *v_scale, int scale_block, const void *gate,
+                                       int64_t gate_batch_stride, int64_t gate_head_stride, void *workspace,
+                                       int64_t workspace_bytes, int64_t *need, void *stream) {
+  const char *what = "window_decode_blocks";
+  if (scale_block <= 0) return fail(NQ_EUNSUPPORTED, "%s: blocks of %d tokens", what, scale_block);
+  return window_decode(what, scale_block, q, q_batch_stride, q_head_stride, const_cast<void *>(k_cache),
+                       const_cast<void *>(v_cache), block_tables, bt_stride, max_blocks_per_seq, context_lens, window,
+                       num_sinks, nullptr, 0, nullptr, 0, nullptr, -1, out, out_batch_stride, out_head_stride, batch,
+                       num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, softmax_scale, q_dtype, NQ_FP8_E4M3,
+                       k_scale, v_scale, gate, gate_batch_stride, gate_head_stride, workspace, workspace_bytes, need,
+                       stream);
 }

@@ -300,7 +300,11 @@ def paged_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale,
     cache equal ``store_kvcache`` followed by this call when each
     ``slot_mapping[b]`` is -1 or the slot of token ``cache_seqlens[b] - 1``
     of ``block_table[b]`` (what prepare_decode writes).
+    With ``k_scale, v_scale [num_blocks, block_size / tokens, Hkv]`` the fp8 cache has a scale for each block of
+    tokens and head (``append_kvcache``, which stores the new token beforehand).
     """
+    if k_scale is not None and k_scale.dim() == 3:
+        return _decode_blocks(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale, out, gate, k)
     require_cuda(q, k_cache, v_cache, cache_seqlens, block_table, what="paged_decode")
     q3 = q.squeeze(1) if q.dim() == 4 else q
     if q3.dim() != 3 or q3.stride(-1) != 1:
@@ -391,7 +395,14 @@ def varlen_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen
     With it: ``k, v`` are the paged caches ``[num_blocks, block_size, Hkv, D]``.
     With ``gate [Tq, Hq, D]`` the output is ``out * sigmoid(gate)``
     (models/qwen3_5.py:142), applied in the kernel's output store.
+    With ``k_scale, v_scale [num_blocks, block_size / tokens, Hkv]`` the paged fp8 caches have a scale for each block
+    of tokens and head (``append_kvcache``); causal only.
     """
+    if k_scale is not None and k_scale.dim() == 3:
+        if not causal:
+            raise RuntimeError("varlen_prefill: caches with a scale for each block are attended to causally")
+        return _prefill_blocks("varlen_prefill", q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                               softmax_scale, 0, 0, block_table, k_scale, v_scale, out, gate)
     require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k, block_table, what="varlen_prefill")
     tq, hq, d = q.shape
     if q.stride(-1) != 1:
@@ -858,8 +869,14 @@ def window_prefill(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen
     sequence's first ``num_sinks``: keys ``j <= p`` with ``j > p - window`` or ``j < num_sinks``.
 
     Table entries of pages that no token of the call sees are not used (``ModelRunner.release_window_blocks``).
+    Scales for each block of tokens and head as for ``varlen_prefill``.
     """
     what = "window_prefill"
+    if k_scale is not None and k_scale.dim() == 3:
+        if window < 1:
+            raise RuntimeError(f"{what}: window {window}")
+        return _prefill_blocks(what, q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                               window, num_sinks, block_table, k_scale, v_scale, out, gate)
     dev = _check_one_device(what, q, k, v, cu_seqlens_q, cu_seqlens_k, block_table, k_scale, v_scale, out, gate)
     if q.dim() != 3:
         raise RuntimeError(f"{what}: q must be [T, Hq, D]")
@@ -895,9 +912,13 @@ def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale
     sequence's first ``num_sinks``.
 
     ``q [B, 1, Hq, D]`` (or ``[B, Hq, D]``); returns ``out`` shaped like ``q``.  With ``k, v [B, Hkv, D]`` and
-    ``slot_mapping [B]`` the new token is stored in the same launch, on the terms of ``paged_decode``.
+    ``slot_mapping [B]`` the new token is stored in the same launch, on the terms of ``paged_decode``, which also
+    says what scales for each block of tokens and head are.
     """
     what = "window_decode"
+    blocks = k_scale is not None and k_scale.dim() == 3
+    if blocks and k is not None:
+        raise RuntimeError(f"{what}: {_APPEND_FIRST}")
     dev = _check_one_device(what, q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out, gate, k, v,
                             slot_mapping)
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1):
@@ -911,6 +932,13 @@ def window_decode(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale
     shape = torch.Size((B, hq, d))
     qa, oa = _rows_of(what, "q", q, shape, q.dtype), _rows_of(what, "out", out, shape, q.dtype)
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, shape, q.dtype)
+    if blocks:
+        unit = _block_scales(what, k_cache, k_scale, v_scale)
+        _launch_span(what, lib().nq_window_decode_blocks, dev, (
+            *qa, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], cache_seqlens.data_ptr(), _int32(window), _int32(num_sinks), *oa, B, hq, hkv, d, bs, nb,
+            float(softmax_scale), dtype_code(q.dtype), k_scale.data_ptr(), v_scale.data_ptr(), unit, *ga))
+        return out
     scales = _scale_args(what, k_cache.dtype, hkv, k_scale, v_scale)
     new = (None, 0, None, 0, None, -1)
     if k is not None:
@@ -1026,6 +1054,7 @@ def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
 # (no counterpart in the reference, whose cache holds the model's own type)
 
 SCALE_BLOCKS = (32, 64, 128, 256)    # tokens of a block
+_APPEND_FIRST = "append_kvcache stores the new token of a cache with a scale for each block"
 
 
 def _block_scales(what, k_cache, k_scale, v_scale):
@@ -1128,6 +1157,82 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
         k_cache.shape[0] * k_cache.shape[1], unit, n, 0 if qa[0] is None else query.shape[-2], hkv, d,
         dtype_code(key.dtype), raw_stream(dev)), what)
     return q_out, k_out
+
+
+def _decode_counters_and_workspace(key, bytes_of):
+    """What a decode's launch takes besides its tensors, with the stream's lock held: its counters (``bytes_of``: as many
+    as it needs during a capture) and workspace, or ``None``."""
+    if key[1] != 0 and _capturing(key):    # the null stream cannot be captured
+        nbytes = bytes_of()
+        counters = _captured_counter_slot(key, nbytes) if 0 < nbytes <= _COUNTER_SLOT_BYTES else None
+    else:
+        counters = _decode_counters.get(key)
+        if counters is None:
+            counters = _decode_counter_slot(key)
+    return counters, _workspaces.get(key)
+
+
+def _decode_blocks(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale, out, gate, k):
+    """``paged_decode`` over a cache with a scale for each block of tokens and head."""
+    what = "paged_decode"
+    if k is not None:
+        raise RuntimeError(f"{what}: {_APPEND_FIRST}")
+    dev = _check_one_device(what, q, k_cache, v_cache, cache_seqlens, block_table, k_scale, v_scale, out, gate)
+    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] != 1):
+        raise RuntimeError(f"{what}: q must be [B, 1, Hq, D] or [B, Hq, D]")
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _decode_blocks(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale, out,
+                                  gate, k)
+    B, hq, d = q.shape[0], q.shape[-2], q.shape[-1]
+    nb, bs, hkv = _paged_args(what, d, k_cache, v_cache, block_table, B)
+    unit = _block_scales(what, k_cache, k_scale, v_scale)
+    if cache_seqlens.dtype != torch.int32 or cache_seqlens.numel() != B or not cache_seqlens.is_contiguous():
+        raise RuntimeError(f"{what}: cache_seqlens must be contiguous int32 [B]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    shape = (B, hq, d)
+    qa, oa = _rows_of(what, "q", q, shape, q.dtype), _rows_of(what, "out", out, shape, q.dtype)
+    ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, shape, q.dtype)
+    key, need = (dev, raw_stream(dev)), ctypes.c_int64()
+    width = block_table.shape[1]
+    with _launch_locks[hash(key) & 63]:
+        counters, ws = _decode_counters_and_workspace(
+            key, lambda: _decode_config(B, hq, hkv, d, width, bs, k_cache.dtype)[0] if B else 0)
+        while True:
+            rc = lib().nq_paged_decode_blocks(
+                *qa, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.stride(0), width,
+                cache_seqlens.data_ptr(), *oa, B, hq, hkv, d, bs, nb, float(softmax_scale), dtype_code(q.dtype),
+                k_scale.data_ptr(), v_scale.data_ptr(), unit, *ga, ptr(ws), 0 if ws is None else ws.numel(),
+                ptr(counters), 0 if counters is None else counters.numel() * 4, need, key[1])
+            if rc != 1:
+                break
+            ws = decode_workspace(q.device, need.value)
+    check(rc, what)
+    return out
+
+
+def _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale,
+                    window, num_sinks, block_table, k_scale, v_scale, out, gate):
+    """``varlen_prefill`` (``window`` 0) and ``window_prefill`` over a cache with a scale for each block of tokens and head."""
+    dev = _check_one_device(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, k_scale, v_scale, out, gate)
+    if q.dim() != 3 or block_table is None:
+        raise RuntimeError(f"{what}: q must be [T, Hq, D], and a cache with a scale for each block has a block_table")
+    tq, hq, d = q.shape
+    n = cu_seqlens_q.numel() - 1
+    _check_cu(what, n + 1, cu_seqlens_q, cu_seqlens_k)
+    nb, bs, hkv = _paged_args(what, d, k_cache, v_cache, block_table, n)
+    unit = _block_scales(what, k_cache, k_scale, v_scale)
+    if out is None:
+        out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
+    qa, oa = _rows_of(what, "q", q, q.shape, q.dtype), _rows_of(what, "out", out, q.shape, q.dtype)
+    ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
+    _launch_span(what, lib().nq_varlen_prefill_blocks, dev, (
+        *qa, k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+        _int32(max_seqlen_q), _int32(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb,
+        _int32(window), _int32(num_sinks), *oa, n, tq, hq, hkv, d, bs, float(softmax_scale), dtype_code(q.dtype),
+        k_scale.data_ptr(), v_scale.data_ptr(), unit, *ga))
+    return out
 
 
 __all__ = ["store_kvcache", "paged_decode", "varlen_prefill", "prepare_decode", "decode_plan", "qk_norm_rope_store",

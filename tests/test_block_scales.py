@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from nano_qwen_amd import kernels
+from tests import test_gpu_blocks
 from tests.test_gpu_append import refusals
 
 
@@ -14,6 +15,8 @@ def host(monkeypatch):
     monkeypatch.setattr(kernels, "_check_one_device", lambda *a: 0)
     monkeypatch.setattr(kernels, "_current_device", lambda: 0)
     monkeypatch.setattr(kernels, "raw_stream", lambda i: 0)
+    monkeypatch.setattr(kernels, "_decode_counters_and_workspace", lambda *a: (None, torch.empty(1 << 26, dtype=torch.uint8)))
+    monkeypatch.setitem(kernels._span_parts, (0, 0), torch.empty(1 << 27, dtype=torch.uint8))
 
 
 def test_append_refusals(host):
@@ -30,3 +33,16 @@ def test_append_refuses_tensors_on_the_host():
     good, _ = refusals("cpu")
     with pytest.raises(RuntimeError, match="HIP device"):
         kernels.append_kvcache(**good)
+
+
+def test_attention_refusals(host):
+    for call, c, args, kw in test_gpu_blocks.refusals("cpu"):
+        with pytest.raises(RuntimeError) as e:
+            getattr(c, call)(*args, **kw)
+        assert "status -3" not in str(e.value), (call, args, list(kw), str(e.value))
+    for new in ([2, 3], [1, 1]):
+        c = test_gpu_blocks.Case(new, [40, 5], 8, 2, 128, torch.bfloat16, 64, 32).to("cpu")
+        for call in (c.prefill, c.decode)[:1 if new[0] > 1 else 2]:
+            for args in ((), (40, 1)):
+                with pytest.raises(RuntimeError, match="status -3"):
+                    call(*args)
