@@ -770,10 +770,10 @@ int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride
 
 /*
  * Attention over such a cache; any positive scales.  nq_paged_decode_auto without
- * new rows, nq_varlen_prefill over the paged cache (causal; with window > 0 as
- * nq_window_prefill, with 0 without one) and nq_window_decode without new rows:
- * their arguments, with scale_block, and the same terms for `workspace`, `need`
- * and `counters` (nq_decode_config and nq_decode_workspace_bytes with NQ_FP8_E4M3).
+ * new rows, nq_varlen_prefill_split over the paged cache (causal), nq_window_prefill
+ * over it and nq_window_decode without new rows: their arguments, with scale_block,
+ * and the same terms for workspaces, `need` and `counters` (nq_decode_config,
+ * nq_decode_workspace_bytes and the like with NQ_FP8_E4M3).
  */
 int nq_paged_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
                            const void *v_cache, const int32_t *block_tables, int64_t bt_stride,
@@ -785,6 +785,17 @@ int nq_paged_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head
                            int64_t counter_bytes, int64_t *need, void *stream);
 
 int nq_varlen_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+                             const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                             int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables, int64_t bt_stride,
+                             int max_blocks_per_seq, int64_t num_blocks, void *out, int64_t out_row_stride,
+                             int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads,
+                             int num_kv_heads, int head_dim, int block_size, float softmax_scale, int q_dtype,
+                             const float *k_scale, const float *v_scale, int scale_block, const void *gate,
+                             int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+                             int64_t workspace_bytes, void *split_workspace, int64_t split_workspace_bytes,
+                             int64_t *need, void *stream);
+
+int nq_window_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
                              const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
                              int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables, int64_t bt_stride,
                              int max_blocks_per_seq, int64_t num_blocks, int window, int num_sinks, void *out,

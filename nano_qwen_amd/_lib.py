@@ -129,6 +129,11 @@ _SIGS = {
                                        c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                        c_void_p, c_int64, POINTER(c_int64), c_void_p]),
     "nq_varlen_prefill_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                         c_void_p, c_int64, c_int, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64,
+                                         c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                                         c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, POINTER(c_int64),
+                                         c_void_p]),
+    "nq_window_prefill_blocks": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                          c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_void_p, c_int64, c_int64,
                                          c_int, c_int64, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p,
                                          c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, POINTER(c_int64), c_void_p]),

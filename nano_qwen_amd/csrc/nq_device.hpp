@@ -254,6 +254,13 @@ __device__ inline void dma4_opaque(uint32_t lds_addr, const u32x4 &rsrc, uint32_
                : "s"(lds_addr), "v"(voff), "s"(rsrc)
                : "m0");
 }
+// The four bytes at offset soff of `rsrc`, to 64 dwords from lds_addr.
+__device__ inline void dma4_spread(uint32_t lds_addr, const u32x4 &rsrc, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword off, %1, %2 lds"
+               :
+               : "s"(lds_addr), "s"(rsrc), "s"(soff)
+               : "m0");
+}
 #pragma clang diagnostic pop
 // LDS reads the compiler schedules and waits for itself, at LDS byte address
 // `addr` + OFF (the constant folds into the instruction's offset).  Only for

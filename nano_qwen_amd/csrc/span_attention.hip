@@ -249,8 +249,10 @@ __device__ __forceinline__ int item_cost(const A &a, const Seq &q) {
 // tile lies in one block.  With w_j = 2^(sl2 k_scale s_j + log2 v_scale - m) the
 // outputs are sum w_j c_j over sum w_j / v_scale, so that P is w: V's scale costs
 // an addend of the exponent's fma and a factor of the sum's, and w <= 2^kRescale
-// whatever the scales.  The scales of a tile go with its copies: 64 tiles' with
-// the list of where they lie, then, per ring slot, to a lane of ring_k and ring_v.
+// whatever the scales.  The scales of 64 tiles are loaded with the list of where
+// they lie; what a tile needs of them is formed for all 64 at once, a tile per
+// lane, and read from there (formed tile by tile, with a select per ring slot on
+// top: a chunk of 2048 tokens behind 14336 662 us, against XXX).
 template <class T, bool FP8, class S, bool BLK>
 __device__ __forceinline__ void span_body() {
   constexpr int D = S::D, RW = S::RW, QS = S::QS, M = S::M, SLOTS = S::SLOTS, COPS = S::COPS;
@@ -260,7 +262,7 @@ __device__ __forceinline__ void span_body() {
   const int rw = RW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, g = lane >> 4;
   KernArgs &a0 = *kernel_args();  // (of the prologue)
-  const bool paged = a0.block_tables != nullptr;
+  const bool paged = BLK || a0.block_tables != nullptr;
   const int n_ranges = a0.n_ranges;
   const bool ranges = n_ranges > 0;
 
@@ -452,9 +454,11 @@ __device__ __forceinline__ void span_body() {
   int nx_list = 0, nx_left = 0, nx_at = 0, nx_first = 0;
   const uint8_t *nx_base = a0.k;
   uint32_t nx_last = 0;
-  float st_ks = 1.f, st_vs = 1.f, nx_ks = 1.f, nx_vs = 1.f;  // BLK: the lists' tiles' scales
-  float ring_k = 1.f, ring_v = 1.f;                          // BLK: lane e % SLOTS: of entry e
+  // BLK: the scales of the queued item's first list, and of the list that the
+  // item at work comes to next: its first, then those that its copies went on to.
+  float nx_ks = 1.f, nx_vs = 1.f, cn_ks = 1.f, cn_vs = 1.f;
   bool bad_seen = false;  // some tile lay in a missing page: from then on every tile is looked up
+  int plain_end = 0;      // BLK: end of the item's tiles that are known to be seen whole
   auto list_of = [&](KernArgs &a, const Item &it, int chunk) -> int {
     const int i = it.lo + 64 * chunk + lane;
     int at = 0;
@@ -468,6 +472,7 @@ __device__ __forceinline__ void span_body() {
       }
     }
     bad_seen = uni(bad_seen | (__builtin_amdgcn_ballot_w64(at < 0) != 0)) != 0;
+    if (BLK && bad_seen) plain_end = 0;
     return at;
   };
   auto scales_of = [&](KernArgs &a, int at, float &ks, float &vs) {
@@ -497,8 +502,6 @@ __device__ __forceinline__ void span_body() {
       nx_queued = false;
       nx_first = st_pos;
       st_list = nx_list;
-      st_ks = nx_ks;
-      st_vs = nx_vs;
       st_l = 0;
       st_left = nx_left;
       st_at = nx_at;
@@ -512,17 +515,12 @@ __device__ __forceinline__ void span_body() {
       ++st_chunk;
       st_l = 0;
       st_list = list_of(*kernel_args(), describe(st_at), st_chunk);
-      scales_of(*kernel_args(), st_list, st_ks, st_vs);
+      scales_of(*kernel_args(), st_list, cn_ks, cn_vs);
       // (here, where the list is needed at once: a load that the compiler cannot
       // see waited for on every path, it waits for in the loop, with the copies)
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     }
     const int at = __builtin_amdgcn_readlane(st_list, st_l);
-    if constexpr (BLK) {
-      const bool here = lane == ((st_pos - 1) & (SLOTS - 1));
-      ring_k = here ? u2f(__builtin_amdgcn_readlane(f2u(st_ks), st_l)) : ring_k;
-      ring_v = here ? u2f(__builtin_amdgcn_readlane(f2u(st_vs), st_l)) : ring_v;
-    }
     src = st_base + static_cast<int64_t>(static_cast<uint32_t>(max(at, 0))) * static_cast<uint32_t>(kKeys * kv_rs);
     nrec = at < 0 ? 0u : st_left == 1 ? st_last : static_cast<uint32_t>(kKeys * kv_rs);
     ++st_l;
@@ -593,15 +591,25 @@ __device__ __forceinline__ void span_body() {
   // (never 0: a masked score, -inf, must stay that under a scale of 0)
   const float sl2_head = FP8 && !BLK ? fmaxf(a0.scale_log2 * ld_const(a0.k_scale + h), 0x1p-126f) : a0.scale_log2;
   float sl2 = sl2_head, lsv = 0.f, inv_sv = 1.f;  // BLK: of the tile whose P is formed
-  auto tile_scales = [&](int entry) {
+  float list_sl2 = 0.f, list_lsv = 0.f, list_inv = 1.f;  // the same of 64 tiles of the item at work
+  auto take_scales = [&](float ks, float vs) {
     if constexpr (BLK) {
-      static_assert((SLOTS & (SLOTS - 1)) == 0, "ring slots by mask");
-      const int e = entry & (SLOTS - 1);
-      sl2 = fmaxf(sl2_head * u2f(__builtin_amdgcn_readlane(f2u(ring_k), e)), 0x1p-126f);
+      list_sl2 = fmaxf(sl2_head * ks, 0x1p-126f);
       // (a scale of 0, of a block of zeros, would make 0 * inf of w / v_scale)
-      const float sv = fminf(fmaxf(u2f(__builtin_amdgcn_readlane(f2u(ring_v), e)), 0x1p-100f), 0x1p100f);
-      lsv = __builtin_amdgcn_logf(sv);
-      inv_sv = __builtin_amdgcn_rcpf(sv);
+      const float sv = fminf(fmaxf(vs, 0x1p-100f), 0x1p100f);
+      list_lsv = __builtin_amdgcn_logf(sv);
+      list_inv = __builtin_amdgcn_rcpf(sv);
+    }
+  };
+  // Of the item's tile number `at`.  (The copies are a few tiles ahead, in the
+  // same item when they come to its next 64 tiles.)
+  auto tile_scales = [&](int at) {
+    if constexpr (BLK) {
+      if ((at & 63) == 0) take_scales(cn_ks, cn_vs);
+      sl2 = u2f(__builtin_amdgcn_readlane(f2u(list_sl2), at & 63));
+      lsv = u2f(__builtin_amdgcn_readlane(f2u(list_lsv), at & 63));
+      inv_sv = u2f(__builtin_amdgcn_readlane(f2u(list_inv), at & 63));
+      asm volatile("" : "+v"(sl2), "+v"(inv_sv));  // (the tile loop has no scalar register to spare)
     }
   };
 
@@ -619,7 +627,13 @@ __device__ __forceinline__ void span_body() {
   // ---------------------------------------------------------------- items
   Item cur = describe(pos0);
   bool careful = false;  // (see odd_values)
+  // BLK: the scales that a queued item's start reads have come, on every way
+  // to there (else the compiler waits there, and for the copies under way).
+  auto scales_here = [&]() {
+    if constexpr (BLK) asm volatile("" : "+v"(nx_ks), "+v"(nx_vs));
+  };
   queue(cur);
+  scales_here();
   // the item whose output is still in registers
   struct Done {
     bool live, whole;
@@ -663,6 +677,10 @@ __device__ __forceinline__ void span_body() {
 #pragma unroll
       for (int kk = 0; kk < NKK; ++kk) qf[qs][kk] = load16(qp + (8 * g + 32 * kk) * 2);
     }
+    if constexpr (BLK) {
+      cn_ks = nx_ks;
+      cn_vs = nx_vs;
+    }
     if (cur.live) queue(describe(cur.next));
     if (done.live) {
       const float vscale = FP8 && !BLK ? ld_const(a.v_scale + h) : 1.f;
@@ -702,7 +720,7 @@ __device__ __forceinline__ void span_body() {
       const int ta = uni(small_div(min(r0, r_last), a.G)), tb = uni(small_div(min(r0 + QS * 16 - 1, r_last), a.G));
       uint32_t slot = lds0 + (static_cast<unsigned>(p0) % SLOTS) * SLOT_B;  // of the tile computed next
       const int window = own_sgpr(a.window), sinks = own_sgpr(a.sinks);
-      const bool tree = window == 0;
+      const bool tree = !BLK && window == 0;
       if (tree) {
         // the masks of the tile's tokens, 32-bit words
         if constexpr (RW > 1) {  // the last item's have been read
@@ -727,7 +745,7 @@ __device__ __forceinline__ void span_body() {
 #pragma unroll
         for (int kk = 0; kk < NKK; ++kk) asm volatile("" : "+v"(qf[qs][kk]));
       asm volatile("" : "+v"(nx_list));
-      if constexpr (BLK) asm volatile("" : "+v"(nx_ks), "+v"(nx_vs));
+      scales_here();
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
         m_use[qs] = kNegInf;
@@ -858,12 +876,30 @@ __device__ __forceinline__ void span_body() {
           for (int j = 0; j < NJ; ++j) o[qs][j] *= alpha[qs];
       };
       // Elements 2 t, 2 t + 1 of a row block: P, its sum, packed.
+      float pref[QS], psum[QS];
       auto p_unit = [&](int qs, int t) -> uint32_t {
-        const float at0 = BLK ? lsv - mref[qs] : -mref[qs];
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, at0));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, at0));
-        lsum[qs] = BLK ? __builtin_fmaf(e0 + e1, inv_sv, lsum[qs]) : lsum[qs] + (e0 + e1);
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1)], sl2, -pref[qs]));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[qs][t >> 1][2 * (t & 1) + 1], sl2, -pref[qs]));
+        (BLK ? psum : lsum)[qs] += e0 + e1;
         return T::pack2(e0, e1);
+      };
+      // Before and after a tile's units.  BLK: its exponents' term and its own sum,
+      // formed outside the section that is scheduled among products.
+      auto p_begin = [&]() {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          pref[qs] = BLK ? mref[qs] - lsv : mref[qs];
+          if constexpr (BLK) {
+            asm volatile("" : "+v"(pref[qs]));
+            psum[qs] = 0.f;
+          }
+        }
+      };
+      auto p_end = [&]() {
+        if constexpr (BLK) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) lsum[qs] = __builtin_fmaf(psum[qs], inv_sv, lsum[qs]);
+        }
       };
       auto scores = [&](uint32_t kt) {
 #pragma unroll
@@ -1047,14 +1083,16 @@ __device__ __forceinline__ void span_body() {
           if (patched) patch(slot, false);
           scores(slot);
           wait_lgkmcnt0();  // the K operands are read: the slot's K is free
-          tile_scales(p0 + i - lo);
+          tile_scales(i - lo);
           const bool whole_tile = static_cast<unsigned>(i - plain.first) < plain.count && !bad_seen;
           if (!whole_tile) mask_tile(i, true);
           next_tile(src, nrec);
           copy_k(slot, src, nrec);
           if (check(alpha)) rescale(alpha);
+          p_begin();
 #pragma unroll
           for (int t = 0; t < 4; ++t) pb[0][t] = p_unit(0, t);
+          p_end();
           wait_vmcnt<(2 * SLOTS - 1) * COPS>();  // V of this tile
           asm volatile("" ::: "memory");
           if (patched) patch(slot, true);
@@ -1082,16 +1120,18 @@ __device__ __forceinline__ void span_body() {
         KV vf[NJ];  // V operands of the tile whose products are pending
         const Plain plain_w = wave_live ? plain_of(ta, tb) : Plain{0, 0}, plain_wg = plain_of(t_first, t_last);
         bool pend = false;
-        auto step = [&](auto first_tag, int i) {
-          constexpr bool FIRST = decltype(first_tag)::value;
+        // PLAIN: of a tile that is known to be seen whole, not carefully
+        auto step = [&](auto first_tag, auto plain_tag, int at) {
+          constexpr bool FIRST = decltype(first_tag)::value, PLAIN = decltype(plain_tag)::value;
+          const int i = lo + at;
           unhoist();
-          tile_scales(p0 + i - lo);
+          tile_scales(at);
           if (!FIRST && pend) rescale(alpha);  // tile i - 1's maxima, before its products join o
-          const bool whole_tile = static_cast<unsigned>(i - plain_w.first) < plain_w.count && !bad_seen;
+          const bool whole_tile = PLAIN || (static_cast<unsigned>(i - plain_w.first) < plain_w.count && !bad_seen);
           if (!whole_tile) mask_tile(i, wave_live);
           pend = check(alpha);
           // (for all of the workgroup's waves alike)
-          if (careful && !(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && !bad_seen) && odd_values(slot)) {
+          if (!PLAIN && careful && !(static_cast<unsigned>(i - plain_wg.first) < plain_wg.count && !bad_seen) && odd_values(slot)) {
             // o is brought up to date before the odd values join it
             if constexpr (!FIRST) {
 #pragma unroll
@@ -1111,6 +1151,7 @@ __device__ __forceinline__ void span_body() {
             clean(slot);
           }
           issue();
+          p_begin();
           KV kf[NKK][2];
           {
             const uint32_t slot_next = next_slot(slot);
@@ -1154,6 +1195,7 @@ __device__ __forceinline__ void span_body() {
             }
 #pragma unroll
             for (int qs = 0; qs < QS; ++qs) pb[qs] = u32x4{pw[qs][0], pw[qs][1], pw[qs][2], pw[qs][3]};
+            p_end();
           }
           __builtin_amdgcn_sched_barrier(0);  // the two sections are scheduled apart
           {
@@ -1198,11 +1240,37 @@ __device__ __forceinline__ void span_body() {
           wait_lgkmcnt0();
           raw_barrier();
         };
-        sync();
-        step(std::true_type{}, lo);
-        for (int i = lo + 1; i < hi; ++i) {
+        if constexpr (BLK) {
+          // Most tiles run in a loop of their own, which holds no scalar register for
+          // the others' tests (a chunk of 2048 tokens behind 14336 658 us in one loop,
+          // 624).  The first tile has products of zeros behind it: with a step of its
+          // own, as below, the kernel outgrew the instruction cache (98 KB; six chats
+          // 206 us, ZZZ).
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) vf[j] = KV{};
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) pb[qs] = u32x4{0, 0, 0, 0};
+          const int plain_begin = plain_w.first - lo;  // counted from the item's first tile
+          plain_end = careful || bad_seen ? 0 : min(plain_begin + static_cast<int>(plain_w.count), n);
+          for (int at = 0; at < n;) {
+            if (at >= plain_begin) {
+              for (; at < plain_end; ++at) {
+                sync();
+                step(std::false_type{}, std::true_type{}, at);
+              }
+              if (at >= n) break;
+            }
+            sync();
+            step(std::false_type{}, std::false_type{}, at);
+            ++at;
+          }
+        } else {
           sync();
-          step(std::false_type{}, i);
+          step(std::true_type{}, std::false_type{}, 0);
+          for (int at = 1; at < n; ++at) {
+            sync();
+            step(std::false_type{}, std::false_type{}, at);
+          }
         }
         if (pend) rescale(alpha);
 #pragma unroll
@@ -1237,6 +1305,7 @@ __device__ __forceinline__ void span_body() {
         st_left = 0;
         careful = true;
         queue(cur);
+        scales_here();
         done.live = false;
         continue;
       }
@@ -1660,7 +1729,7 @@ extern "C" int nq_window_prefill(const void *q, int64_t q_row_stride, int64_t q_
                         gate_row_stride, gate_head_stride, workspace, workspace_bytes, need, stream);
 }
 
-extern "C" int nq_varlen_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
+extern "C" int nq_window_prefill_blocks(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache,
                                         const void *v_cache, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
                                         int max_seqlen_q, int max_seqlen_k, const int32_t *block_tables,
                                         int64_t bt_stride, int max_blocks_per_seq, int64_t num_blocks, int window,
@@ -1670,11 +1739,11 @@ extern "C" int nq_varlen_prefill_blocks(const void *q, int64_t q_row_stride, int
                                         const float *v_scale, int scale_block, const void *gate, int64_t gate_row_stride,
                                         int64_t gate_head_stride, void *workspace, int64_t workspace_bytes,
                                         int64_t *need, void *stream) {
-  const char *what = "varlen_prefill_blocks";
+  const char *what = "window_prefill_blocks";
   if (scale_block <= 0) return fail(NQ_EUNSUPPORTED, "%s: blocks of %d tokens", what, scale_block);
   return window_prefill(what, scale_block, q, q_row_stride, q_head_stride, k_cache, v_cache, 0, 0, cu_seqlens_q,
                         cu_seqlens_k, max_seqlen_q, max_seqlen_k, block_tables, bt_stride, max_blocks_per_seq, num_blocks,
-                        window == 0 ? INT32_MAX : window, num_sinks, out, out_row_stride, out_head_stride, num_seqs,
+                        window, num_sinks, out, out_row_stride, out_head_stride, num_seqs,
                         total_q, num_q_heads, num_kv_heads, head_dim, block_size, softmax_scale, q_dtype, NQ_FP8_E4M3,
                         k_scale, v_scale, gate, gate_row_stride, gate_head_stride, workspace, workspace_bytes, need,
                         stream);

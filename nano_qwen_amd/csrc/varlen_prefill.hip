@@ -80,6 +80,9 @@ struct PrefillArgs {
   float *part_o;
   float *part_l;
   int4 *part_desc;  // (sequence, first head, first row, piece: kPieceNone / kPieceMore / kPieceLast)
+  // BLK: k_scale and v_scale are [num_blocks * tiles of a page >> scale_shift, Hkv],
+  // log2 of the key tiles of a block of tokens with one scale per head.
+  int scale_shift;
 };
 constexpr int kPieceNone = -1, kPieceMore = 0, kPieceLast = 1;
 
@@ -488,12 +491,24 @@ __device__ __forceinline__ Item range_next(const PrefillArgs &a, const CostQueue
 // An item's output is stored at the start of the next one, right after that
 // item's Q loads are issued, so the stores cover the Q latency.
 //
-// vmcnt accounting: each stream entry is 2 * COPS loads per wave, and the
+// BLK: paged fp8 K/V with a scale for each block of tokens and head.  A key tile
+// lies in one block.  With w_j = 2^(sl2 k_scale s_j + log2 v_scale - m) the outputs
+// are sum w_j c_j over sum w_j / v_scale, so that P is w: V's scale costs an addend
+// of the exponent's fma and a factor of the sum's, and w <= 2^kRescale whatever the
+// scales.  A tile's scales are copied with it, in one more load per wave and entry
+// (K's by the even waves, V's by the odd ones; every lane the same four bytes),
+// behind its K codes, which fill half of their part of the ring slot.
+// Codes that are NaN in values that a row does not see do not reach it there: in a
+// tile that is masked they are taken out of the operands, and given back to the
+// rows that see them (odd).
+//
+// vmcnt accounting: each stream entry is EOP loads per wave, and the
 // waits count only younger stream entries -- except that a new item's first
 // kAhead tiles may precede the Q loads and the previous item's output stores
 // (a fixed count per wave), which the waits then add.
-template <class T, int D, class S, bool GATED, bool FP8, int MODE>
+template <class T, int D, class S, bool GATED, bool FP8, int MODE, bool BLK>
 __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
+  static_assert(FP8 || !BLK, "block scales are those of fp8 K/V");
   using DT = DTile<T, D>;
   constexpr bool TAB = MODE == 1, RANGES = MODE == 2;
   constexpr int NW = S::NW, QS = S::QS, kSlots = S::SLOTS, kAhead = S::AHEAD;
@@ -514,10 +529,11 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   // operations shows it -- as it holds on the hardware, where at least these
   // kPad follow the Q loads -- that Q and the queue fetch before them are
   // complete, without a wait for the copies in flight.
-  constexpr int kPad = 2 * COPS * kAhead;
+  constexpr int EOP = 2 * COPS + (BLK ? 1 : 0);  // loads per wave and stream entry
+  constexpr int kPad = EOP * kAhead;
   constexpr int EOPS = QOPS + SOPS + kPad;
   static_assert(CR % 4 == 0, "a copy moves whole groups of 4 rows");
-  static_assert(2 * COPS * kAhead + EOPS < 64, "vmcnt range");
+  static_assert(EOP * kAhead + EOPS < 64, "vmcnt range");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   static_assert(S::RING_BYTES == kSlots * DT::SLOT_B, "ring size");
   int *lds_item = reinterpret_cast<int *>(smem + S::RING_BYTES);  // fetched queue indices
@@ -533,7 +549,8 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   // log2(e) x the softmax scale; with fp8 K also x the item's K scale (the
   // products are formed from the unscaled codes)
   float sl2 = a.scale_log2;
-  const bool paged = a.block_tables != nullptr;
+  [[maybe_unused]] float lsv = 0.f, inv_sv = 1.f;  // BLK: sl2 and these are of the tile whose P is formed
+  const bool paged = BLK || a.block_tables != nullptr;
   const int row_in_item = RW * (wave / a.G4);  // this wave's first row within an item
   const int head_in_item = wave % a.G4;
 
@@ -699,6 +716,14 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   int st_left = 0, st_bidx = 0, st_blk_next = 0;  // paged: tiles left in the block, next entry and its value
   int st_head = 0;                  // byte offset of the item's kv head within a row
   const int32_t *st_bt = nullptr;
+  // BLK: the next entry's tile, counted through the pool, and what its scale is read with
+  int st_tile = 0;
+  const int sc_shift = BLK ? own_sgpr(a.scale_shift) : 0, sc_row = BLK ? own_sgpr(4 * a.Hkv) : 0;
+  const u32x4 sc_rsrc =
+      BLK ? rsrc_words(wave & 1 ? a.v_scale : a.k_scale,
+                       static_cast<uint32_t>((static_cast<int64_t>(a.num_blocks) * (a.block_size / kKeys) >> a.scale_shift) * 4 * a.Hkv))
+          : u32x4{0, 0, 0, 0};
+  constexpr uint32_t kScaleAt = kKeys * D;  // of a ring slot: 256 bytes of K's scale, then V's
   // The item queued to be copied next, in the form the stream takes over.
   int nx_rem = 0;       // its keys (0: none queued)
   int nx_head = 0;      // its kv head's byte offset within a row
@@ -770,6 +795,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
         plain_end = 0;
       }
       st_src = kbase + static_cast<int64_t>(ok ? blk : 0) * blk_bytes + st_head;
+      if constexpr (BLK) st_tile = (ok ? blk : 0) * tiles_per_blk;
       st_left = tiles_per_blk;
     } else if (paged) {
       ok = st_nrec != 0;  // the same block as the previous run
@@ -792,6 +818,12 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
     const uint32_t dst = st_dst + wave * (CR * SRC_ROWB);
     dma16_group(dst, rsrc_words(st_src, st_nrec), src_k);
     dma16_group(dst + DT::TILE_B, rsrc_words(st_src + v_minus_k, st_nrec), src_v);
+    if constexpr (BLK) {
+      // (of a missing page or an empty entry, some block's: such a tile is masked)
+      dma4_spread(st_dst + kScaleAt + (wave & 1) * 256, sc_rsrc,
+                  static_cast<uint32_t>(st_tile >> sc_shift) * sc_row + st_head / (SRC_ROWB / 4));
+      ++st_tile;
+    }
     st_src += tile_bytes;
     st_dst = st_dst == lds_last ? lds0 : st_dst + DT::SLOT_B;
     --run_left;
@@ -882,7 +914,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   // end (and a wave with no rows) are dropped by the range check, not skipped.
   auto store_out_plain = [&](const Item &it) {
     const bool odd = (g & 1) != 0;
-    const float vscale = FP8 ? ld_const(a.v_scale + it.kvh) : 1.f;  // fp8: V's scale (P V from the codes)
+    const float vscale = FP8 && !BLK ? ld_const(a.v_scale + it.kvh) : 1.f;  // fp8: V's scale (P V from the codes)
     const int wrow0 = it.row_begin + row_in_item;
     const int head = it.head0 + head_in_item;
     const uint8_t *obase = a.out + static_cast<int64_t>(it.q0) * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
@@ -917,7 +949,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
 
   auto store_out_gated = [&](const Item &it) {
     const bool odd = (g & 1) != 0;
-    const float vscale = FP8 ? ld_const(a.v_scale + it.kvh) : 1.f;  // fp8: V's scale (P V from the codes)
+    const float vscale = FP8 && !BLK ? ld_const(a.v_scale + it.kvh) : 1.f;  // fp8: V's scale (P V from the codes)
     const int wrow0 = it.row_begin + row_in_item;
     const int head = it.head0 + head_in_item;
     const uint8_t *obase = a.out + static_cast<int64_t>(it.q0) * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
@@ -982,7 +1014,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
   // count: they are then stricter than they need be.
   [[maybe_unused]] float m_part[QS];
   auto store_part = [&](const Item &it) {
-    const float vscale = FP8 ? ld_const(a.v_scale + it.kvh) : 1.f;
+    const float vscale = FP8 && !BLK ? ld_const(a.v_scale + it.kvh) : 1.f;
 #pragma unroll
     for (int qs = 0; qs < QS; ++qs) {
       const float l = sum32(sum16(lsum[qs]));
@@ -1089,11 +1121,11 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
       // Wait for tile 0 (younger: kAhead - 1 stream entries, plus the Q
       // loads and stores above if tile 0 preceded them).
       if (p0 < epi_pos)
-        wait_vmcnt<2 * COPS * (kAhead - 1) + EOPS>();
+        wait_vmcnt<EOP * (kAhead - 1) + EOPS>();
       else
-        wait_vmcnt<2 * COPS * (kAhead - 1)>();
+        wait_vmcnt<EOP * (kAhead - 1)>();
       raw_barrier();
-      if constexpr (FP8) sl2 = a.scale_log2 * ld_const(a.k_scale + cur.kvh);
+      if constexpr (FP8 && !BLK) sl2 = a.scale_log2 * ld_const(a.k_scale + cur.kvh);
 
       const int Lq = cur.Lq, Lk = cur.Lk, P = cur.P, n_kt = cur.n_kt;
       const int wrow0 = cur.row_begin + row_in_item;
@@ -1135,6 +1167,20 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
             for (int qs = 0; qs < QS; ++qs) sc[qs][ks] = T::mfma16x16x32(op(kf[kk][ks]), qf[qs][kk], sc[qs][ks]);
       };
 
+      // BLK: the scales of the tile in ring slot `kt`, and what its P needs of them.
+      // (Never 0: a masked score, -inf, must stay that, and so must w / v_scale of a
+      // block of zeros.)
+      auto scales_at = [&](uint32_t kt, int which) -> float {
+        return *reinterpret_cast<const __attribute__((address_space(3))) float *>(
+            static_cast<uintptr_t>(kt + kScaleAt + 256 * which));
+      };
+      auto take_scales = [&](float ks, float vs) {
+        sl2 = fmaxf(a.scale_log2 * ks, 0x1p-126f);
+        const float sv = fmaxf(vs, 0x1p-100f);
+        lsv = __builtin_amdgcn_logf(sv);
+        inv_sv = __builtin_amdgcn_rcpf(sv);
+      };
+
       float m_use[QS];  // running row max, scaled (log2) domain
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
@@ -1155,6 +1201,10 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
         KV kf[DT::NKK][2];
         unhoist();
         kread(lds0 + (p0 % kSlots) * DT::SLOT_B, kf);
+        if constexpr (BLK) {
+          const uint32_t kt = lds0 + (p0 % kSlots) * DT::SLOT_B;
+          take_scales(scales_at(kt, 0), scales_at(kt, 1));
+        }
         qk(kf, sc);
       }
       const int epi_tiles = epi_pos - p0 - 1;  // leading tiles whose wait adds the item's start operations
@@ -1162,6 +1212,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
       // Scores of the tile whose P is being formed, and the subtrahend of its
       // exponents (the running maximum after the tile's rescale check).
       float xt[QS][8], mref[QS];
+      [[maybe_unused]] float psum[QS];  // BLK: the tile's own row sums of P
       float alpha[QS];    // rescale factors of o before the pending products join it
       bool pend = false;  // whether they differ from 1
       // One unit of P: elements 2t, 2t + 1 of rows block qs, exponentiated
@@ -1170,7 +1221,7 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
       auto p_unit = [&](int qs, int t) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(xt[qs][2 * t], sl2, -mref[qs]));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(xt[qs][2 * t + 1], sl2, -mref[qs]));
-        lsum[qs] += e0 + e1;
+        (BLK ? psum : lsum)[qs] += e0 + e1;
         return T::pack2(e0, e1);
       };
       // Lazy-rescale check of key tile jt (scores sc, masked as the tile
@@ -1207,7 +1258,8 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
             }
           // this lane's maximum over its 8 keys of row m (scaled)
           mnew[qs] = max3(max3(xt[qs][0], xt[qs][1], xt[qs][2]), max3(xt[qs][3], xt[qs][4], xt[qs][5]),
-                          __builtin_elementwise_maximum(xt[qs][6], xt[qs][7])) * sl2;
+                          __builtin_elementwise_maximum(xt[qs][6], xt[qs][7]));
+          mnew[qs] = BLK ? __builtin_fmaf(mnew[qs], sl2, lsv) : mnew[qs] * sl2;
           grow |= mnew[qs] > m_use[qs] + kRescale;
         }
         bool moved = false;
@@ -1222,7 +1274,13 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
           moved = true;
         }
 #pragma unroll
-        for (int qs = 0; qs < QS; ++qs) mref[qs] = (m_use[qs] == kNegInf) ? 0.f : m_use[qs];
+        for (int qs = 0; qs < QS; ++qs) {
+          mref[qs] = (m_use[qs] == kNegInf) ? 0.f : m_use[qs];
+          if constexpr (BLK) {
+            mref[qs] -= lsv;
+            psum[qs] = 0.f;
+          }
+        }
         return moved;
       };
       auto rescale = [&](const float (&alpha)[QS]) {
@@ -1352,6 +1410,48 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
           if (FP8) __builtin_amdgcn_sched_group_barrier(0x002, CK, 0);  // VALU
         }
       };
+      // BLK, a masked tile jt: NaN among the V^T operands vf, whose products with P
+      // are pending.  A weight of 0 would not keep it from the rows that do not see
+      // its key: it is added to the outputs of those that do -- the products of its
+      // places with the rows' visible keys -- and replaced by 0.
+      auto odd = [&](int jt, bool blk_ok, KV (&vf)[DT::NJ]) {
+        if constexpr (BLK) {
+          // top bit of every byte of w that is NaN: 0x7f and the sign
+          auto nan_bits = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
+          uint32_t any = 0;
+#pragma unroll
+          for (int j = 0; j < DT::NJ; ++j) any |= nan_bits(vf[j][0]) | nan_bits(vf[j][1]);
+          if (__builtin_amdgcn_ballot_w64(any != 0) == 0) return;
+          u32x4 seen[QS];  // 1.0 for the keys that a row sees, in the order of P
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) {
+            const int row = wrow0 + 16 * qs + m;
+            const int lim = !blk_ok ? -1 : a.causal ? min(Lk - 1, row + P) : Lk - 1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = jt * kKeys + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
+              seen[qs][e] = (key > lim ? 0u : T::kOne2 & 0xffffu) | (key + 1 > lim ? 0u : T::kOne2 & 0xffff0000u);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < DT::NJ; ++j) {
+            KV ones;  // code 1.0 in the places of NaN
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t n = nan_bits(vf[j][i]);
+              ones[i] = (n >> 7) * 0x38u;
+              vf[j][i] &= ~((n - (n >> 7)) | n);
+            }
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs) {
+              f32x4 hits = T::mfma16x16x32(op(ones), seen[qs], f32x4{0, 0, 0, 0});
+              asm volatile("s_nop 9" : "+v"(hits));  // (the wait states between a product and its readers)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[qs][j][r] = hits[r] != 0.f ? __builtin_nanf("") : o[qs][j][r];
+            }
+          }
+        }
+      };
       // One key tile jt (ring slot `slot`; tile jt + 1 in slot_next), after
       // the barrier that completes tile jt + 1: the pending rescale, the
       // check of tile jt, the next stream entry, O += P V of tile jt - 1 (vf,
@@ -1365,6 +1465,11 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
         if (pend) rescale(alpha);  // tile jt - 1's maxima, before its products join o
         pend = check(mask_tag, jt, blk_ok, alpha);
         issue();
+        float ks_next = 0.f, vs_next = 0.f;
+        if constexpr (BLK) {
+          ks_next = scales_at(slot_next, 0);
+          vs_next = scales_at(slot_next, 1);
+        }
         uint32_t pw[QS][4];
         KV kf[DT::NKK][2];  // tile jt + 1 (discarded past the last)
         if constexpr (decltype(pv_tag)::value) {
@@ -1375,6 +1480,10 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
         }
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) pb[qs] = u32x4{pw[qs][0], pw[qs][1], pw[qs][2], pw[qs][3]};
+        if constexpr (BLK) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) lsum[qs] = __builtin_fmaf(psum[qs], inv_sv, lsum[qs]);
+        }
         __builtin_amdgcn_sched_barrier(0);  // the two sections are scheduled apart
         f32x4 sn[QS][2];
         qk_v(kf, sn, slot, vf);
@@ -1382,6 +1491,10 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
         for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) sc[qs][ks] = sn[qs][ks];
+        if constexpr (BLK) {
+          take_scales(ks_next, vs_next);
+          if constexpr (decltype(mask_tag)::value) odd(jt, blk_ok, vf);
+        }
       };
       // Once per tile jt and wave, in tile order, in every loop below: wait
       // for this wave's copies of tile jt + 1 (younger: kAhead - 2 stream
@@ -1389,9 +1502,9 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
       // jt + 1 preceded them).
       auto sync = [&](int jt) {
         if (jt < epi_tiles)
-          wait_vmcnt<2 * COPS * (kAhead - 2) + EOPS>();
+          wait_vmcnt<EOP * (kAhead - 2) + EOPS>();
         else
-          wait_vmcnt<2 * COPS * (kAhead - 2)>();
+          wait_vmcnt<EOP * (kAhead - 2)>();
         wait_lgkmcnt0();  // and its reads of tiles jt - 1 and jt are done
         raw_barrier();    // tile jt + 1 complete; slot of tile jt - 1 free
       };
@@ -1498,10 +1611,10 @@ __device__ __forceinline__ void prefill_persistent(const PrefillArgs &a) {
 
 // The body lives in a device function: its inline assembly uses register
 // constraints that only the device compilation accepts.
-template <class T, int D, class S, bool GATED, bool FP8, int MODE>
+template <class T, int D, class S, bool GATED, bool FP8, int MODE, bool BLK = false>
 __global__ __launch_bounds__(64 * S::NW) __attribute__((amdgpu_waves_per_eu(S::WPE)))
 void varlen_prefill_dma_kernel(const PrefillArgs a) {
-  prefill_persistent<T, D, S, GATED, FP8, MODE>(a);
+  prefill_persistent<T, D, S, GATED, FP8, MODE, BLK>(a);
 }
 
 // Merge of the items cut by equal ranges: workgroups lin handle the item
@@ -1654,7 +1767,7 @@ struct RangePlan {
   }
 };
 
-template <class T, int D, class S, bool FP8>
+template <class T, int D, class S, bool FP8, bool BLK>
 int launch_prefill_dma(PrefillArgs a, int64_t total_q, uint8_t *split_ws, int64_t split_bytes, hipStream_t st) {
   const int rows_per_item = S::ITEM_ROWS / a.G4;
   a.n_qtiles = (a.max_seqlen_q + rows_per_item - 1) / rows_per_item;
@@ -1672,7 +1785,8 @@ int launch_prefill_dma(PrefillArgs a, int64_t total_q, uint8_t *split_ws, int64_
     a.part_o = reinterpret_cast<float *>(split_ws);
     a.part_l = reinterpret_cast<float *>(split_ws + 2 * grid * RP::kSlotO);
     a.part_desc = reinterpret_cast<int4 *>(split_ws + 2 * grid * (RP::kSlotO + RP::kSlotL));
-    auto *kern = a.gate ? varlen_prefill_dma_kernel<T, D, S, true, FP8, 2> : varlen_prefill_dma_kernel<T, D, S, false, FP8, 2>;
+    auto *kern = a.gate ? varlen_prefill_dma_kernel<T, D, S, true, FP8, 2, BLK>
+                        : varlen_prefill_dma_kernel<T, D, S, false, FP8, 2, BLK>;
     kern<<<grid, 64 * S::NW, S::LDS_BYTES, st>>>(a);
     const int rc = check_launch("varlen_prefill(ranges)");
     if (rc != NQ_OK) return rc;
@@ -1709,20 +1823,20 @@ int launch_prefill_dma(PrefillArgs a, int64_t total_q, uint8_t *split_ws, int64_
   // items; a multiple of 8 so every XCD gets the same count.
   int64_t grid = (static_cast<int64_t>(device_cus()) * S::WG_PER_CU + 7) / 8 * 8;
   if (grid > total) grid = total;  // work_grid() is a multiple of 8 when pinned
-  auto *kern = a.gate ? (a.by_cost == 2 ? varlen_prefill_dma_kernel<T, D, S, true, FP8, 1>
-                                        : varlen_prefill_dma_kernel<T, D, S, true, FP8, 0>)
-                     : (a.by_cost == 2 ? varlen_prefill_dma_kernel<T, D, S, false, FP8, 1>
-                                        : varlen_prefill_dma_kernel<T, D, S, false, FP8, 0>);
+  auto *kern = a.gate ? (a.by_cost == 2 ? varlen_prefill_dma_kernel<T, D, S, true, FP8, 1, BLK>
+                                        : varlen_prefill_dma_kernel<T, D, S, true, FP8, 0, BLK>)
+                     : (a.by_cost == 2 ? varlen_prefill_dma_kernel<T, D, S, false, FP8, 1, BLK>
+                                        : varlen_prefill_dma_kernel<T, D, S, false, FP8, 0, BLK>);
   kern<<<static_cast<int>(grid), 64 * S::NW, S::LDS_BYTES, st>>>(a);
   return check_launch(a.gate ? "varlen_prefill(gated)" : "varlen_prefill");
 }
 
-template <class T, bool FP8, int D>
+template <class T, bool FP8, int D, bool BLK = false>
 int launch_prefill(const PrefillArgs &a, int64_t total_q, uint8_t *split_ws, int64_t split_bytes, hipStream_t s) {
   if constexpr (D == 256) {
-    return launch_prefill_dma<T, D, ShapeD, FP8>(a, total_q, split_ws, split_bytes, s);
+    return launch_prefill_dma<T, D, ShapeD, FP8, BLK>(a, total_q, split_ws, split_bytes, s);
   } else {
-    return launch_prefill_dma<T, D, ShapeC, FP8>(a, total_q, split_ws, split_bytes, s);  // fp8 copies: one 1 KiB piece per wave
+    return launch_prefill_dma<T, D, ShapeC, FP8, BLK>(a, total_q, split_ws, split_bytes, s);  // fp8 copies: one 1 KiB piece per wave
   }
 }
 
@@ -1742,7 +1856,7 @@ static int varlen_prefill_impl(const void *q, int64_t q_row_stride, int64_t q_he
                                float softmax_scale, int causal, int q_dtype, int kv_dtype, const float *k_scale,
                                const float *v_scale, void *workspace, int64_t workspace_bytes, const void *gate,
                                int64_t gate_row_stride, int64_t gate_head_stride, int64_t total_q,
-                               void *split_workspace, int64_t split_bytes, void *stream) {
+                               void *split_workspace, int64_t split_bytes, void *stream, int scale_block = 0) {
   if (num_seqs == 0 || max_seqlen_q == 0) return NQ_OK;
   if (num_seqs < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_q_heads <= 0 || num_kv_heads <= 0)
     return fail(NQ_EINVAL, "varlen_prefill: bad sizes");
@@ -1761,6 +1875,11 @@ static int varlen_prefill_impl(const void *q, int64_t q_row_stride, int64_t q_he
     return fail(NQ_EUNSUPPORTED, "varlen_prefill: kv dtype %d with q dtype %d", kv_dtype, q_dtype);
   if (fp8 && (!k_scale || !v_scale)) return fail(NQ_EINVAL, "varlen_prefill: fp8 K/V needs scales");
   if (!q || !k || !v || !cu_seqlens_q || !cu_seqlens_k || !out) return fail(NQ_EINVAL, "varlen_prefill: null pointer");
+  if (scale_block != 0 && (!fp8 || !block_tables || num_blocks <= 0 || !block_scales_built(scale_block, block_size) ||
+                           num_blocks * (block_size / scale_block) * num_kv_heads > (1 << 29) ||
+                           num_blocks * (block_size / kKeys) > 0x7fffffff))
+    return fail(NQ_EUNSUPPORTED, "varlen_prefill: a scale per %d tokens in %lld pages of %d, kv dtype %d", scale_block,
+                (long long)num_blocks, block_size, kv_dtype);
   if (block_tables) {
     if (block_size <= 0 || block_size % kKeys != 0)
       return fail(NQ_EUNSUPPORTED, "varlen_prefill: block_size %d must be a multiple of %d", block_size, kKeys);
@@ -1827,6 +1946,14 @@ static int varlen_prefill_impl(const void *q, int64_t q_row_stride, int64_t q_he
   if (sw && (!aligned(sw, 256) || total_q < 0))
     return fail(NQ_EINVAL, "varlen_prefill: split workspace alignment or total_q");
   int rc;
+  if (scale_block != 0) {
+    a.scale_shift = __builtin_ctz(static_cast<unsigned>(scale_block / kKeys));
+    if (q_dtype == NQ_BF16)
+      return head_dim == 256 ? launch_prefill<BF16, true, 256, true>(a, total_q, sw, split_bytes, st)
+                             : launch_prefill<BF16, true, 128, true>(a, total_q, sw, split_bytes, st);
+    return head_dim == 256 ? launch_prefill<F16, true, 256, true>(a, total_q, sw, split_bytes, st)
+                           : launch_prefill<F16, true, 128, true>(a, total_q, sw, split_bytes, st);
+  }
   if (head_dim == 256) {
     if (q_dtype == NQ_BF16)
       rc = fp8 ? launch_prefill<BF16, true, 256>(a, total_q, sw, split_bytes, st) : launch_prefill<BF16, false, 256>(a, total_q, sw, split_bytes, st);
@@ -1916,4 +2043,30 @@ extern "C" int nq_varlen_prefill_split(
                              block_size, softmax_scale, causal, q_dtype, kv_dtype, k_scale, v_scale, workspace,
                              workspace_bytes, gate, gate_row_stride, gate_head_stride, total_q, split_workspace,
                              split_workspace_bytes, stream);
+}
+
+extern "C" int nq_varlen_prefill_blocks(
+    const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache, const void *v_cache,
+    const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
+    const int32_t *block_tables, int64_t bt_stride, int max_blocks_per_seq, int64_t num_blocks, void *out,
+    int64_t out_row_stride, int64_t out_head_stride, int num_seqs, int64_t total_q, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, float softmax_scale, int q_dtype, const float *k_scale, const float *v_scale,
+    int scale_block, const void *gate, int64_t gate_row_stride, int64_t gate_head_stride, void *workspace,
+    int64_t workspace_bytes, void *split_workspace, int64_t split_workspace_bytes, int64_t *need, void *stream) {
+  if (scale_block <= 0 || !block_tables)
+    return fail(NQ_EUNSUPPORTED, "varlen_prefill_blocks: paged K/V in blocks of %d tokens", scale_block);
+  if (need) {
+    const int64_t bytes =
+        prefill_split_bytes(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim, true);
+    if (bytes > 0 && (!split_workspace || split_workspace_bytes < bytes)) {
+      *need = bytes;
+      return 1;
+    }
+  }
+  return varlen_prefill_impl(q, q_row_stride, q_head_stride, k_cache, v_cache,
+                             static_cast<int64_t>(num_kv_heads) * head_dim, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                             max_seqlen_k, block_tables, bt_stride, max_blocks_per_seq, num_blocks, out, out_row_stride,
+                             out_head_stride, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size, softmax_scale, 1,
+                             q_dtype, NQ_FP8_E4M3, k_scale, v_scale, workspace, workspace_bytes, gate, gate_row_stride,
+                             gate_head_stride, total_q, split_workspace, split_workspace_bytes, stream, scale_block);
 }

@@ -1227,11 +1227,34 @@ def _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_s
         out = torch.empty(tq, hq, d, dtype=q.dtype, device=q.device)
     qa, oa = _rows_of(what, "q", q, q.shape, q.dtype), _rows_of(what, "out", out, q.shape, q.dtype)
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, q.shape, q.dtype)
-    _launch_span(what, lib().nq_varlen_prefill_blocks, dev, (
-        *qa, k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-        _int32(max_seqlen_q), _int32(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], nb,
-        _int32(window), _int32(num_sinks), *oa, n, tq, hq, hkv, d, bs, float(softmax_scale), dtype_code(q.dtype),
-        k_scale.data_ptr(), v_scale.data_ptr(), unit, *ga))
+    args = (*qa, k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+            _int32(max_seqlen_q), _int32(max_seqlen_k), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+            nb)
+    tail = (*oa, n, tq, hq, hkv, d, bs, float(softmax_scale), dtype_code(q.dtype), k_scale.data_ptr(), v_scale.data_ptr(),
+            unit, *ga)
+    # The causal kernel takes groups of 1, 2 and multiples of 4 query heads and lengths that the table holds; others
+    # run as a window that reaches every token.
+    group = hq // max(hkv, 1)
+    if window or (group > 2 and group % 4) or max_seqlen_k > block_table.shape[1] * bs:
+        _launch_span(what, lib().nq_window_prefill_blocks, dev, (*args, _int32(window or 0x7fffffff), _int32(num_sinks), *tail))
+        return out
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                                   softmax_scale, window, num_sinks, block_table, k_scale, v_scale, out, gate)
+    key, need = (dev, raw_stream(dev)), ctypes.c_int64()
+    with _launch_locks[hash(key) & 63]:
+        queue = prefill_workspace(q.device)
+        parts = _prefill_parts.get(key)
+        while True:
+            rc = lib().nq_varlen_prefill_blocks(*args, *tail, ptr(queue), queue.numel() * 4, ptr(parts),
+                                                0 if parts is None else parts.numel(), need, key[1])
+            if rc != 1:
+                break
+            parts = _grow(_prefill_parts, key, need.value, torch.uint8, q.device)
+    check(rc, what)
+    if _DEBUG_QUEUE:
+        _check_queue_zero(queue)
     return out
 
 

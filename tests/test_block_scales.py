@@ -7,6 +7,12 @@ from tests import test_gpu_blocks
 from tests.test_gpu_append import refusals
 
 
+def buffer(n):
+    """``n`` bytes, aligned as a device's are."""
+    t = torch.empty(n + 256, dtype=torch.uint8)
+    return t[-t.data_ptr() % 256:][:n]
+
+
 @pytest.fixture
 def host(monkeypatch):
     """The shim's and the library's checks, with tensors on the host: what passes them all fails at its launch (status -3)."""
@@ -15,8 +21,10 @@ def host(monkeypatch):
     monkeypatch.setattr(kernels, "_check_one_device", lambda *a: 0)
     monkeypatch.setattr(kernels, "_current_device", lambda: 0)
     monkeypatch.setattr(kernels, "raw_stream", lambda i: 0)
-    monkeypatch.setattr(kernels, "_decode_counters_and_workspace", lambda *a: (None, torch.empty(1 << 26, dtype=torch.uint8)))
-    monkeypatch.setitem(kernels._span_parts, (0, 0), torch.empty(1 << 27, dtype=torch.uint8))
+    monkeypatch.setattr(kernels, "_decode_counters_and_workspace", lambda *a: (None, buffer(1 << 26)))
+    monkeypatch.setattr(kernels, "prefill_workspace", lambda d: torch.zeros(64, dtype=torch.int32))
+    monkeypatch.setitem(kernels._prefill_parts, (0, 0), buffer(1 << 27))
+    monkeypatch.setitem(kernels._span_parts, (0, 0), buffer(1 << 27))
 
 
 def test_append_refusals(host):
