@@ -773,7 +773,8 @@ int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride
  * new rows, nq_varlen_prefill_split over the paged cache (causal), nq_window_prefill
  * over it and nq_window_decode without new rows: their arguments, with scale_block,
  * and the same terms for workspaces, `need` and `counters` (nq_decode_config,
- * nq_decode_workspace_bytes and the like with NQ_FP8_E4M3).
+ * nq_decode_workspace_bytes and the like with NQ_FP8_E4M3).  The causal prefill
+ * takes any group of up to 16 query heads; split_workspace is what `need` asks for.
  */
 int nq_paged_decode_blocks(const void *q, int64_t q_batch_stride, int64_t q_head_stride, const void *k_cache,
                            const void *v_cache, const int32_t *block_tables, int64_t bt_stride,

@@ -29,6 +29,8 @@
 //    operand reads are bank-conflict free.
 //  * Online softmax in the log2 domain with lazy rescaling: O and l are only
 //    rescaled when a row maximum grows by more than 2^8, so P <= 256.
+#include <stdlib.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -2045,6 +2047,36 @@ extern "C" int nq_varlen_prefill_split(
                              split_workspace_bytes, stream);
 }
 
+// Which kernel takes a causal prefill over a cache with block scales: this file's,
+// or the windowed one with a window that reaches every token.  That has shapes for
+// few rows, cheaper merges and no queue, but row tiles dealt out beforehand and
+// slower transitions between them.  Measured, this file's against the windowed
+// one's, head_dim 128, 8 kv heads, 4 query heads each: up to 64 rows of a kv head, one
+// sequence of 4 tokens behind 1500 32 and 18 us, 16 of 16 behind 8000 123 and 86; with
+// more of them, by the key tiles per resident workgroup: 4 of 1000 behind none (64) 93
+// and 70, 16 of 128 behind 200 (20) 55 and 32, 16 of 48 behind 1500 (24) 62 and 66, 4 of 128
+// behind 8000 (63) 125 and 119, 16 of 48 behind 8000 (125) 198 and 219, 4 of 300 behind
+// 8000 (162) 242 and 274, 16 of 300 behind 1500 (141) 195 and 236.  At head_dim 256 (4 kv
+// heads): 4 of 128 behind 200 (2) 50 and 32, one of 300 behind 1500 (9) 54 and 51, one of 1000
+// behind none (16) 50 and 61, 4 of 300 behind 1500 (36) 91 and 101.
+// NQ_PREFILL_BLOCKS=causal or =window chooses instead.
+// The causal kernel is not built for every group, and wants the table to hold
+// max_seqlen_k and outputs 16 bytes apart.
+static bool blocks_by_window(int num_seqs, int64_t total_q, int max_seqlen_q, int max_seqlen_k, int num_q_heads,
+                             int num_kv_heads, int head_dim, int64_t table_tokens, bool aligned_out) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0) return false;  // refused below
+  const int64_t G = num_q_heads / num_kv_heads;
+  if (G == 3 || (G > 4 && G % 4 != 0) || max_seqlen_k > table_tokens || !aligned_out) return true;
+  if (const char *v = getenv("NQ_PREFILL_BLOCKS")) {  // an explicit choice, where both can
+    if (v[0] == 'c') return false;
+    if (v[0] == 'w') return true;
+  }
+  if (max_seqlen_q * G <= 64) return true;
+  const int64_t items = std::min<int64_t>(total_q * G / 128 + num_seqs, num_seqs * ((max_seqlen_q * G + 127) / 128)) * num_kv_heads;
+  const int64_t resident = static_cast<int64_t>(device_cus()) * (head_dim == 256 ? 1 : 2);
+  return items * ((max_seqlen_k + kKeys - 1) / kKeys) <= resident * (head_dim == 256 ? 12 : 64);
+}
+
 extern "C" int nq_varlen_prefill_blocks(
     const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k_cache, const void *v_cache,
     const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int max_seqlen_q, int max_seqlen_k,
@@ -2055,6 +2087,16 @@ extern "C" int nq_varlen_prefill_blocks(
     int64_t workspace_bytes, void *split_workspace, int64_t split_workspace_bytes, int64_t *need, void *stream) {
   if (scale_block <= 0 || !block_tables)
     return fail(NQ_EUNSUPPORTED, "varlen_prefill_blocks: paged K/V in blocks of %d tokens", scale_block);
+  if (blocks_by_window(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim,
+                       static_cast<int64_t>(max_blocks_per_seq) * block_size,
+                       out_row_stride % 8 == 0 && out_head_stride % 8 == 0 && aligned(out, 16) &&
+                           (!gate || (gate_row_stride % 8 == 0 && gate_head_stride % 8 == 0 && aligned(gate, 16)))))
+    return nq_window_prefill_blocks(q, q_row_stride, q_head_stride, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k,
+                                    max_seqlen_q, max_seqlen_k, block_tables, bt_stride, max_blocks_per_seq, num_blocks,
+                                    INT32_MAX, 0, out, out_row_stride, out_head_stride, num_seqs, total_q, num_q_heads,
+                                    num_kv_heads, head_dim, block_size, softmax_scale, q_dtype, k_scale, v_scale,
+                                    scale_block, gate, gate_row_stride, gate_head_stride, split_workspace,
+                                    split_workspace_bytes, need, stream);
   if (need) {
     const int64_t bytes =
         prefill_split_bytes(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim, true);

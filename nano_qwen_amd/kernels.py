@@ -1232,28 +1232,31 @@ def _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_s
             nb)
     tail = (*oa, n, tq, hq, hkv, d, bs, float(softmax_scale), dtype_code(q.dtype), k_scale.data_ptr(), v_scale.data_ptr(),
             unit, *ga)
-    # The causal kernel takes groups of 1, 2 and multiples of 4 query heads and lengths that the table holds; others
-    # run as a window that reaches every token.
-    group = hq // max(hkv, 1)
-    if window or (group > 2 and group % 4) or max_seqlen_k > block_table.shape[1] * bs:
-        _launch_span(what, lib().nq_window_prefill_blocks, dev, (*args, _int32(window or 0x7fffffff), _int32(num_sinks), *tail))
+    if window:
+        _launch_span(what, lib().nq_window_prefill_blocks, dev, (*args, _int32(window), _int32(num_sinks), *tail))
         return out
     if dev != _current_device():
         with torch.cuda.device(dev):
             return _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                                    softmax_scale, window, num_sinks, block_table, k_scale, v_scale, out, gate)
     key, need = (dev, raw_stream(dev)), ctypes.c_int64()
+    capturing = key[1] != 0 and _capturing(key)
     with _launch_locks[hash(key) & 63]:
-        queue = prefill_workspace(q.device)
-        parts = _prefill_parts.get(key)
+        if capturing:    # the graph's own: replays may overlap other calls
+            queue, parts = torch.zeros(lib().nq_prefill_workspace_bytes() // 4, dtype=torch.int32, device=q.device), None
+        else:
+            queue, parts = prefill_workspace(q.device), _prefill_parts.get(key)
         while True:
             rc = lib().nq_varlen_prefill_blocks(*args, *tail, ptr(queue), queue.numel() * 4, ptr(parts),
                                                 0 if parts is None else parts.numel(), need, key[1])
             if rc != 1:
                 break
-            parts = _grow(_prefill_parts, key, need.value, torch.uint8, q.device)
+            if capturing:
+                parts = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            else:
+                parts = _grow(_prefill_parts, key, need.value, torch.uint8, q.device)
     check(rc, what)
-    if _DEBUG_QUEUE:
+    if _DEBUG_QUEUE and not capturing:
         _check_queue_zero(queue)
     return out
 

@@ -75,19 +75,19 @@ class Case:
         s = torch.where(has[:, None, None], s, 1.0)
         return torch.where(has[:, None, None], rows * s, 0.0), s[..., 0], has
 
-    def reference(self, window=1 << 40, sinks=0):
-        """(output, weighted mean of |v|, what fp16's subnormal weights may be off)."""
+    def reference(self, window=1 << 40, sinks=0, device="cpu"):
+        """(output, weighted mean of |v|, what fp16's subnormal weights may be off), in float64 on ``device``."""
         outs, mags, subs, q0 = [], [], [], 0
         g = self.hq // self.hkv
         for i, n in enumerate(self.new):
             have = max(self.have[i], 0)
             k, _, has = self.values_of(self.k, self.k_scale, i, have)
             v, sv, _ = self.values_of(self.v, self.v_scale, i, have)
-            vis = spans.window_visible(torch.arange(have - n, have), have, window, sinks) & has
-            o, mag, sub = (torch.zeros(n, self.hq, self.d, dtype=torch.float64) for _ in range(3))
-            q = self.q[q0:q0 + n].double()
+            vis = (spans.window_visible(torch.arange(have - n, have), have, window, sinks) & has).to(device)
+            o, mag, sub = (torch.zeros(n, self.hq, self.d, dtype=torch.float64, device=device) for _ in range(3))
+            q, k, v, sv = (x.to(device) for x in (self.q[q0:q0 + n].double(), k, v, sv))
             for h in range(self.hkv if have else 0):
-                t = torch.einsum("ngd,kd->ngk", q[:, h * g:(h + 1) * g], k[:, h]) * self.scale
+                t = (q[:, h * g:(h + 1) * g].reshape(-1, self.d) @ k[:, h].T.contiguous()).view(n, g, have) * self.scale
                 t = t.masked_fill(~vis[:, None], -torch.inf)
                 any_ = vis.any(1)[:, None, None]
                 p = torch.where(any_, torch.softmax(t, -1), 0.0)
@@ -97,9 +97,8 @@ class Case:
                 top = (p * sv[:, h]).amax(-1, keepdim=True)
                 codes = (v[:, h] / torch.where(sv[:, h, None] > 0, sv[:, h, None], 1.0)).abs()
                 sub[:, hs] = 2.0 ** -25 * top * (vis[:, None].double() @ codes)
-            outs.append(o)
-            mags.append(mag)
-            subs.append(sub)
+            for to, x in ((outs, o), (mags, mag), (subs, sub)):
+                to.append(x.cpu())
             q0 += n
         return torch.cat(outs), torch.cat(mags), torch.cat(subs)
 

@@ -75,7 +75,7 @@ def test_decode_empty_rows_and_gate(cuda):
 
 
 @pytest.mark.parametrize("d", [128, 256])
-def test_missing_pages(cuda, d):
+def test_missing_pages(cuda, kernel, d):
     """Keys without a page, or with one outside the pool, are not seen."""
     lost = [(0, 1), (0, 2), (1, 0), (2, 5)]
     c = Case([1, 1, 1], [300, 63, 400], 8, 2, d, BF, 64, 32, lost=lost).to(cuda)
@@ -89,15 +89,22 @@ STEPS = [([1], [0]), ([1, 7], [0, 3]), ([33], [0]), ([5, 64, 1, 130], [300, 0, 3
          ([200, 90], [40, 0]), ([257], [255]), ([40, 0, 3], [0, 9, 500])]
 
 
+@pytest.fixture(params=["causal", "window"])
+def kernel(request, monkeypatch):
+    """Either kernel of the causal prefill, where both can."""
+    monkeypatch.setenv("NQ_PREFILL_BLOCKS", request.param)
+    return request.param
+
+
 @pytest.mark.parametrize("new,pre", STEPS)
 @pytest.mark.parametrize("fine", [False, True])
-def test_prefill(cuda, new, pre, fine):
+def test_prefill(cuda, kernel, new, pre, fine):
     c = Case(new, pre, 8, 2, 128, BF, 64, 32, seed=len(new) + new[0], fine=fine).to(cuda)
     check(c.prefill(), c.reference(), BF)
 
 
 @pytest.mark.parametrize("hq,hkv,d,dtype,block,unit", HEADS)
-def test_prefill_heads_and_types(cuda, hq, hkv, d, dtype, block, unit):
+def test_prefill_heads_and_types(cuda, kernel, hq, hkv, d, dtype, block, unit):
     for new, pre in (([70, 3, 150], [100, 600, 0]), ([2, 5], [77, 10]), ([1, 1], [40, 3])):
         c = Case(new, pre, hq, hkv, d, dtype, block, unit, seed=hq).to(cuda)
         check(c.prefill(), c.reference(), dtype, f"{new}")
@@ -105,10 +112,27 @@ def test_prefill_heads_and_types(cuda, hq, hkv, d, dtype, block, unit):
 
 @pytest.mark.parametrize("new,pre,d,dtype", [([1500, 900], [600, 0], 128, BF), ([20], [9000], 128, BF), ([700], [3000], 256, HF),
                                              ([260] * 12, [500] * 12, 128, HF)])
-def test_prefill_long(cuda, new, pre, d, dtype):
+def test_prefill_long(cuda, kernel, new, pre, d, dtype):
     """More than 64 tiles to an item, items that are cut and those that are dealt out whole."""
     c = Case(new, pre, 4, 2, d, dtype, 256, 64, seed=new[0]).to(cuda)
     check(c.prefill(), c.reference(), dtype)
+
+
+@pytest.mark.parametrize("new,pre,hq,hkv,d,dtype", [([900, 1000, 17], [8000, 3000, 9000], 32, 8, 128, BF),
+                                                    ([1500] * 6, [0, 100, 700, 33, 256, 2000], 16, 4, 256, HF),
+                                                    ([300] * 40, [64] * 40, 32, 8, 128, BF), ([3000], [5000], 64, 8, 128, HF)])
+def test_prefill_large(cuda, new, pre, hq, hkv, d, dtype):
+    """What the rules give to the causal kernel: queues and ranges.  (The oracle's products on the device, in float64.)"""
+    c = Case(new, pre, hq, hkv, d, dtype, 256, 64, seed=new[0]).to(cuda)
+    check(c.prefill(), c.reference(device=cuda), dtype)
+
+
+def test_gated_prefill(cuda, kernel):
+    c = Case([70, 3], [100, 600], 8, 2, 128, BF, 64, 32).to(cuda)
+    gate = torch.randn(73, 8, 256, device=cuda).to(BF)[:, :, 128:]
+    wide = torch.full((73, 8, 256), 7.0, dtype=BF, device=cuda)
+    out = c.prefill(gate=gate, out=wide[:, :, :128])
+    assert torch.equal(out, kernels.output_gate(c.prefill(), gate)) and (wide[:, :, 128:] == 7).all()
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (33, 4), (200, 64), (100000, 0)])
@@ -122,7 +146,7 @@ def test_windows(cuda, window, sinks, hq, hkv, d, dtype, block, unit):
 
 
 @pytest.mark.parametrize("d", [128, 256])
-def test_values_that_are_not_finite(cuda, d):
+def test_values_that_are_not_finite(cuda, kernel, d):
     """NaN among the values reaches the rows that see it, and no others."""
     c = Case([40, 33], [70, 0], 8, 2, d, BF, 64, 32, seed=d)
     c.v.view(torch.uint8)[c.table[0, 1].long(), 30, 1, 5] = 0x7F    # token 94 of sequence 0: its query row 24 sees it
@@ -139,7 +163,7 @@ def test_values_that_are_not_finite(cuda, d):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-def test_scales_far_apart(cuda, dtype):
+def test_scales_far_apart(cuda, kernel, dtype):
     """Values of neighbouring blocks 2^40 apart, and one block of scale 0: what a 16-bit weight must not lose."""
     c = Case([1, 1, 30], [200, 700, 170], 8, 2, 128, dtype, 64, 32, seed=4)
     far = torch.tensor([2.0 ** -40, 1.0, 2.0 ** -20]).repeat(c.v_scale.numel())[:c.v_scale.numel()].view(c.v_scale.shape)
@@ -157,7 +181,7 @@ def test_scales_far_apart(cuda, dtype):
     check(one.prefill(), ref, dtype)
 
 
-def test_captured_and_on_other_streams(cuda):
+def test_captured_and_on_other_streams(cuda, kernel):
     """Replays follow their inputs, the scales among them; streams and threads that decode at once."""
     c = Case([1] * 4, [800, 20, 300, 1999], 8, 2, 128, BF, 64, 32, seed=1).to(cuda)
     p = Case([30, 70], [900, 10], 8, 2, 128, BF, 64, 32, seed=2).to(cuda)
