@@ -757,7 +757,8 @@ int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int bl
  * codes of the block's tokens before them are coded again where it grew.  What
  * lies behind them in the block is not kept.  The rows of one block must be
  * neighbours with rising slots, and no slot may occur twice.  Rows with a slot
- * outside [0, num_slots) are not stored.
+ * outside [0, num_slots) are not stored; without k_cache (then v, the scales and
+ * slot_mapping are ignored) none are.
  */
 int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k,
                       int64_t k_row_stride, const void *v, int64_t v_row_stride, const int64_t *positions,
@@ -767,6 +768,13 @@ int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_head_stride
                       float *k_scale, float *v_scale, const int32_t *slot_mapping, int64_t num_slots,
                       int scale_block, int64_t num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                       void *stream);
+
+/*
+ * The scales of pages src_blocks[i] to those of pages dst_blocks[i], on the terms
+ * of nq_copy_kv_blocks: kv_scales [num_slabs, num_blocks, scales_per_block].
+ */
+int nq_copy_kv_scales(float *kv_scales, int64_t num_slabs, int64_t num_blocks, int scales_per_block,
+                      const int32_t *src_blocks, const int32_t *dst_blocks, int64_t num_pairs, void *stream);
 
 /*
  * Attention over such a cache; any positive scales.  nq_paged_decode_auto without

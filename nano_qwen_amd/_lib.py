@@ -141,6 +141,7 @@ _SIGS = {
                                         c_int, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int,
                                         c_int64, c_float, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64,
                                         c_void_p, c_int64, POINTER(c_int64), c_void_p]),
+    "nq_copy_kv_scales": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "nq_append_kvcache": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                   c_int64, c_int, c_void_p, c_void_p, c_float, c_float, c_void_p, c_int64, c_int64,
                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,

@@ -136,7 +136,7 @@ __device__ inline u32x2 recode(const u32x2 &c, float f) {
   return r;
 }
 
-// Workgroups 0 .. run_wgs - 1: the runs that start in rows chunk * i .. of one
+// Workgroups 0 .. run_wgs - 1 (with a cache): the runs that start in rows chunk * i .. of one
 // head, of K or of V.  The others: the query rows of one token each.
 template <class T, int LPU>
 __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
@@ -151,6 +151,13 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
       transform<T, LPU>(a, a.q_w, pos, x);
       store8<T>(a.q_out + tok * a.qo_row + h * a.qo_head + 16 * l, x);
     }
+    if (!a.k_cache)  // no runs: the keys are these workgroups' too
+      for (int h = r0; h < a.hkv; h += RPP) {
+        float x[8];
+        row8<T>(a.k + tok * a.k_row + (h * D + 8 * l) * 2, x);
+        transform<T, LPU>(a, a.k_w, pos, x);
+        store8<T>(a.k_out + tok * a.ko_row + (h * D + 8 * l) * 2, x);
+      }
     return;
   }
   __shared__ float lds_max[kThreads / 64];
@@ -257,18 +264,18 @@ extern "C" int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_
   if (head_dim != 128 && head_dim != 256)
     return fail(NQ_EUNSUPPORTED, "%s: head_dim %d (built: 128, 256)", what, head_dim);
   if (dtype != NQ_BF16 && dtype != NQ_F16) return fail(NQ_EUNSUPPORTED, "%s: dtype %d (need f16/bf16)", what, dtype);
-  if (scale_block != 32 && scale_block != 64 && scale_block != 128 && scale_block != 256)
+  if (k_cache && scale_block != 32 && scale_block != 64 && scale_block != 128 && scale_block != 256)
     return fail(NQ_EUNSUPPORTED, "%s: blocks of %d tokens (built: 32, 64, 128, 256)", what, scale_block);
   if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0)
     return fail(NQ_EUNSUPPORTED, "%s: rotary_dim %d must be a multiple of 16 in [0, %d]", what, rotary_dim, head_dim);
-  if (num_slots % scale_block != 0 || num_slots > 0x7fffffff)
+  if (k_cache && (num_slots % scale_block != 0 || num_slots > 0x7fffffff))
     return fail(NQ_EINVAL, "%s: %lld slots in blocks of %d", what, (long long)num_slots, scale_block);
   if (num_tokens == 0) return NQ_OK;
-  if (!k || !v || !k_cache || !v_cache || !k_scale || !v_scale || !slot_mapping || (q && (!q_out || num_q_heads == 0)) ||
+  if (!k || (k_cache ? !v || !v_cache || !k_scale || !v_scale || !slot_mapping : !k_out) || (q && (!q_out || num_q_heads == 0)) ||
       (rotary_dim > 0 && (!positions || !cos_sin_cache)))
     return fail(NQ_EINVAL, "%s: null pointer", what);
   const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
-  if (k_row_stride < row || v_row_stride < row || (k_out && k_out_row_stride < row))
+  if (k_row_stride < row || (k_cache && v_row_stride < row) || (k_out && k_out_row_stride < row))
     return fail(NQ_EINVAL, "%s: rows narrower than their heads", what);
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16) || !aligned(k_out, 16) ||
       !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(cos_sin_cache, 16) || !aligned(k_cache, 16) ||
@@ -309,8 +316,8 @@ extern "C" int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_
   // Rows per workgroup of runs: few rows are a decode step's, every one a run of
   // its own; of many, most continue the row before them.
   a.chunk = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, num_tokens / 512)));
-  const int64_t runs = (num_tokens + a.chunk - 1) / a.chunk * 2 * num_kv_heads;
-  const int64_t grid = runs + (q ? num_tokens : 0);
+  const int64_t runs = k_cache ? (num_tokens + a.chunk - 1) / a.chunk * 2 * num_kv_heads : 0;
+  const int64_t grid = runs + (q || !k_cache ? num_tokens : 0);
   if (grid > 0x7fffffff) return fail(NQ_EINVAL, "%s: %lld tokens of %d heads", what, (long long)num_tokens, num_kv_heads);
   a.run_wgs = static_cast<int>(runs);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -45,6 +45,18 @@ __global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(uint8_t *pool
     if (at + u * kCopyThreads * 16 < bytes) store16(d + at + u * kCopyThreads * 16, x[u]);
 }
 
+// The scales of pages (of a cache with a scale for each block of tokens and head):
+// `per` floats a page and slab, one per thread.
+__global__ __launch_bounds__(kCopyThreads) void copy_scales_kernel(float *pool, const int32_t *src, const int32_t *dst,
+                                                                   int64_t num_blocks, int per, int parts) {
+  const int pair = static_cast<int>(blockIdx.x / parts);
+  const int i = static_cast<int>(blockIdx.x % parts) * kCopyThreads + threadIdx.x;
+  const int32_t from = ld_const(src + pair), to = ld_const(dst + pair);
+  if (from < 0 || to < 0 || from >= num_blocks || to >= num_blocks || from == to || i >= per) return;
+  float *slab = pool + static_cast<int64_t>(blockIdx.y) * num_blocks * per + i;
+  slab[to * static_cast<int64_t>(per)] = slab[from * static_cast<int64_t>(per)];
+}
+
 // ---------------------------------------------------------------- trees
 // Every wave walks its sequence's tree itself (nodes lane, lane + 64, ... in
 // registers, one ballot per 64 nodes and step) and then moves its columns.  A
@@ -225,6 +237,21 @@ extern "C" int nq_copy_kv_blocks(void *kv_cache, int64_t num_slabs, int64_t num_
       static_cast<uint8_t *>(kv_cache), src_blocks, dst_blocks, num_tokens, num_blocks, block_size, row_bytes,
       static_cast<int>(chunks));
   return check_launch("copy_kv_blocks");
+}
+
+extern "C" int nq_copy_kv_scales(float *kv_scales, int64_t num_slabs, int64_t num_blocks, int scales_per_block,
+                                 const int32_t *src_blocks, const int32_t *dst_blocks, int64_t num_pairs, void *stream) {
+  if (num_pairs < 0 || num_slabs < 0 || num_blocks < 0 || scales_per_block <= 0)
+    return fail(NQ_EINVAL, "copy_kv_scales: bad sizes");
+  if (num_pairs == 0 || num_slabs == 0 || num_blocks == 0) return NQ_OK;
+  if (!kv_scales || !src_blocks || !dst_blocks) return fail(NQ_EINVAL, "copy_kv_scales: null pointer");
+  if (num_slabs > 65535) return fail(NQ_EUNSUPPORTED, "copy_kv_scales: %lld slabs > 65535", (long long)num_slabs);
+  const int64_t parts = (static_cast<int64_t>(scales_per_block) + kCopyThreads - 1) / kCopyThreads;
+  if (parts * num_pairs > 0x7fffffff) return fail(NQ_EINVAL, "copy_kv_scales: %lld pages", (long long)num_pairs);
+  copy_scales_kernel<<<dim3(static_cast<unsigned>(parts * num_pairs), static_cast<unsigned>(num_slabs)), kCopyThreads, 0,
+                       static_cast<hipStream_t>(stream)>>>(kv_scales, src_blocks, dst_blocks, num_blocks,
+                                                           scales_per_block, static_cast<int>(parts));
+  return check_launch("copy_kv_scales");
 }
 
 extern "C" int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int block_size, int64_t row_bytes,

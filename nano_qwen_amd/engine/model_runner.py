@@ -62,11 +62,14 @@ class ModelRunner:
         self.allocate_decode_buffers()
 
     # ------------------------------------------------------------- KV pool
-    def kv_block_bytes(self, num_layers: int, num_kv_heads: int, head_dim: int, kv_dtype: torch.dtype) -> int:
+    def kv_block_bytes(self, num_layers: int, num_kv_heads: int, head_dim: int, kv_dtype: torch.dtype,
+                       kv_scale_block: int | None = None) -> int:
         """Bytes of one block of every layer's K and V
-        (engine/model_runner.py:195), with the cache dtype's item size."""
+        (engine/model_runner.py:195), with the cache dtype's item size, and
+        of its scales if every ``kv_scale_block`` tokens have their own."""
         item = torch.empty((), dtype=kv_dtype).element_size()
-        return 2 * num_layers * self.block_size * num_kv_heads * head_dim * item
+        scales = 4 * (self.block_size // kv_scale_block) if kv_scale_block else 0
+        return 2 * num_layers * num_kv_heads * (self.block_size * head_dim * item + scales)
 
     def budget_blocks(self, block_bytes: int, gpu_memory_utilization: float, mem_info=None, stats=None) -> int:
         """Blocks that fit the memory budget (engine/model_runner.py:189-196):
@@ -85,7 +88,7 @@ class ModelRunner:
     def allocate_kv_cache(self, model=None, num_layers: int | None = None, num_blocks: int | None = None,
                           num_kv_heads: int | None = None, head_dim: int | None = None,
                           dtype: torch.dtype | None = None, kv_cache_dtype: torch.dtype | None = None,
-                          gpu_memory_utilization: float | None = None):
+                          gpu_memory_utilization: float | None = None, kv_scale_block: int | None = None):
         """One tensor ``[2, L, num_blocks, block_size, Hkv, D]`` and per-layer
         views bound to every module with ``k_cache``/``v_cache`` attributes
         (engine/model_runner.py:186-204).
@@ -96,7 +99,13 @@ class ModelRunner:
         stores in ``config.num_kvcache_blocks``.  Explicit arguments override
         those; ``num_blocks=None`` sizes from the budget
         (``gpu_memory_utilization``, default the config's or 0.9).  Returns
-        the number of layers bound."""
+        the number of layers bound.
+
+        ``kv_scale_block`` (or ``config.kv_scale_block``), with a
+        ``float8_e4m3fn`` cache: that many tokens (32, 64, 128 or 256) of a
+        page and head have a scale of their own, set by the store, in place of
+        one per (layer, head): ``kv_scales [2, L, num_blocks, block_size /
+        kv_scale_block, Hkv]``."""
         cfg = self.config
         hf = getattr(cfg, "hf_config", None)
         model = model if model is not None else self.model
@@ -109,22 +118,30 @@ class ModelRunner:
                 head_dim = getattr(hf, "head_dim", None) or hf.hidden_size // hf.num_attention_heads
             dtype = dtype if dtype is not None else hf.dtype
             kv_cache_dtype = kv_cache_dtype if kv_cache_dtype is not None else getattr(cfg, "kv_cache_dtype", None)
+            kv_scale_block = kv_scale_block if kv_scale_block is not None else getattr(cfg, "kv_scale_block", None)
         if None in (num_layers, num_kv_heads, head_dim, dtype):
             raise ValueError("allocate_kv_cache: layers, kv heads, head_dim and dtype are needed "
                              "(as arguments or from config.hf_config)")
         kv_dtype = kv_cache_dtype or dtype
+        if kv_scale_block and (kv_dtype != torch.float8_e4m3fn or kv_scale_block not in kernels.SCALE_BLOCKS
+                               or self.block_size % kv_scale_block):
+            raise ValueError(f"allocate_kv_cache: a scale per {kv_scale_block} tokens of a {kv_dtype} cache in pages of "
+                             f"{self.block_size}")
         if num_blocks is None:
             util = gpu_memory_utilization if gpu_memory_utilization is not None else \
                 getattr(cfg, "gpu_memory_utilization", 0.9)
-            num_blocks = self.budget_blocks(self.kv_block_bytes(num_layers, num_kv_heads, head_dim, kv_dtype), util)
+            num_blocks = self.budget_blocks(
+                self.kv_block_bytes(num_layers, num_kv_heads, head_dim, kv_dtype, kv_scale_block), util)
             assert num_blocks > 0, "allocate_kv_cache: the memory budget holds no KV block"
         if cfg is not None:
             cfg.num_kvcache_blocks = num_blocks
         self.model = model
         self.kv_cache = torch.empty(2, num_layers, num_blocks, self.block_size, num_kv_heads, head_dim,
                                     dtype=kv_dtype, device=self.device)
+        self.kv_scales = None
         if kv_dtype == torch.float8_e4m3fn:
-            self.kv_scales = torch.ones(2, num_layers, num_kv_heads, dtype=torch.float32,
+            per_block = (num_blocks, self.block_size // kv_scale_block) if kv_scale_block else ()
+            self.kv_scales = torch.ones(2, num_layers, *per_block, num_kv_heads, dtype=torch.float32,
                                         device=self.device)
         modules = model.modules() if hasattr(model, "modules") else model
         layer_id = 0
@@ -135,6 +152,8 @@ class ModelRunner:
                 if self.kv_scales is not None:
                     module.k_scale = self.kv_scales[0, layer_id]
                     module.v_scale = self.kv_scales[1, layer_id]
+                elif getattr(module, "k_scale", None) is not None:    # an earlier pool's
+                    module.k_scale = module.v_scale = None
                 layer_id += 1
         return layer_id
 
@@ -153,6 +172,8 @@ class ModelRunner:
         states (per-(layer, kv_head) absmax/448)."""
         if self.kv_scales is None:
             raise RuntimeError("calibrate_kv_scales: the KV pool is not float8_e4m3fn")
+        if self.scales_by_block:
+            raise RuntimeError("calibrate_kv_scales: every block has scales of its own, which the store sets")
         _, n_layers, hkv = self.kv_scales.shape
         if len(kv_per_layer) != n_layers:
             raise ValueError(f"calibrate_kv_scales: {len(kv_per_layer)} layers given, the pool has {n_layers}")
@@ -167,6 +188,11 @@ class ModelRunner:
                 s = (amax / 448.0).to(self.kv_scales.device)
                 self.kv_scales[which, layer] = torch.where(s > 0, s, torch.ones_like(s))
         return self.kv_scales
+
+    @property
+    def scales_by_block(self) -> bool:
+        """Whether the pool has a scale for each block of tokens and head."""
+        return self.kv_scales is not None and self.kv_scales.dim() == 5
 
     def allocate_decode_buffers(self):
         size = self.max_num_seqs
@@ -265,6 +291,8 @@ class ModelRunner:
         own.  Node j goes to position ``len(seq) - 1 + j`` of the cache, for which the block table has to have
         room, and has the position of its depth.  Returns ``(input_ids, positions)`` of all nodes; the model then
         runs as in a prefill, and ``commit_tree`` ends the step."""
+        if self.scales_by_block:
+            raise RuntimeError("prepare_tree: not over a cache with a scale for each block")
         input_ids, positions, slots, all_parents = [], [], [], []
         cu_q, cu_k = [0], [0]
         bs = self.block_size
@@ -325,7 +353,8 @@ class ModelRunner:
 
     # ------------------------------------------------------ pages of the pool
     def copy_blocks(self, src, dst, num_tokens=None):
-        """Pages ``src`` to pages ``dst`` (lists of ids) in every layer, in one launch; ``num_tokens``: the first
+        """Pages ``src`` to pages ``dst`` (lists of ids) in every layer, in one launch (and their scales in another, where
+        every block has its own); ``num_tokens``: the first
         tokens of each only.  A page that is written may appear in no other pair."""
         if len(src) != len(dst) or (num_tokens is not None and len(num_tokens) != len(src)):
             raise ValueError(f"copy_blocks: {len(src)} pages to {len(dst)}")
@@ -338,6 +367,8 @@ class ModelRunner:
             up = [self._to_device(x, torch.int32) for x in (src, dst)]
             kernels.copy_kv_blocks(self.kv_cache, *up,
                                    None if num_tokens is None else self._to_device(num_tokens, torch.int32))
+            if self.scales_by_block:    # a partly filled page's too: a block's first token sets its scale anew
+                kernels.copy_kv_scales(self.kv_scales, *up)
 
     def fork(self, seqs, new_blocks):
         """A continuation of every sequence with a cache of its own: full pages are shared, the next tokens go to

@@ -113,8 +113,12 @@ def store_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale=None, v_sc
 
     Same-dtype caches get a byte-exact copy; a ``float8_e4m3fn`` cache is
     quantized with ``k_scale/v_scale [Hkv]`` (``x * (1/scale)``, saturate to
-    +-448, round to nearest even).
+    +-448, round to nearest even).  Scales for each block of tokens and head:
+    ``append_kvcache``, on its terms.
     """
+    if k_scale is not None and k_scale.dim() == 3:
+        append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        return
     require_cuda(key, value, k_cache, v_cache, slot_mapping, what="store_kvcache")
     n, hkv, d = key.shape
     if slot_mapping.dtype != torch.int32:
@@ -512,7 +516,12 @@ def qk_norm_rope_store(positions, query, key, value, q_weight, k_weight, eps, co
     inputs rotates in place).  Without caches nothing is stored.
     ``_return_args`` returns the checked C-ABI argument tuple instead of
     launching (for timing loops that call the library directly).
+    Scales for each block of tokens and head: ``append_kvcache``, whose
+    results are rounded once, and which has no key rotated in place.
     """
+    if k_scale is not None and k_scale.dim() == 3 and not _return_args:
+        return append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query, positions, cos_sin_cache,
+                              rotary_dim, q_weight, k_weight, eps, weight_offset, q_out, k_out)
     require_cuda(positions, query, key, value, q_weight, k_weight, cos_sin_cache, k_cache, v_cache,
                  slot_mapping, what="qk_norm_rope_store")
     n, hq, d = query.shape
@@ -817,6 +826,9 @@ def tree_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_seqlen_q
     what = "tree_attention"
     dev = _check_one_device(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, block_table, tree_mask, k_scale,
                             v_scale, out, gate)
+    if k_scale is not None and k_scale.dim() == 3:
+        raise RuntimeError(f"{what}: caches with a scale for each block are not built for trees (commit_tree moves rows "
+                           "between blocks)")
     if q.dim() != 3:
         raise RuntimeError(f"{what}: q must be [T, Hq, D]")
     tq, hq, d = q.shape
@@ -995,6 +1007,26 @@ def copy_kv_blocks(kv_cache, src_blocks, dst_blocks, num_tokens=None):
     check(lib().nq_copy_kv_blocks(kv_cache.data_ptr(), slabs, nb, bs, row, *args, n, raw_stream(dev)), what)
 
 
+def copy_kv_scales(kv_scales, src_blocks, dst_blocks):
+    """The scales of pages ``src_blocks [n]`` to those of pages ``dst_blocks [n]`` in every layer's K and V, in one launch:
+    ``kv_scales`` is the runner's ``[2, L, num_blocks, block_size / tokens, Hkv]`` or any contiguous float32 ``[...,
+    num_blocks, block_size / tokens, Hkv]``; on the terms of ``copy_kv_blocks``, whose pages they belong to."""
+    what = "copy_kv_scales"
+    dev = _check_one_device(what, kv_scales, src_blocks, dst_blocks)
+    if kv_scales.dim() < 3 or kv_scales.dtype != torch.float32 or not kv_scales.is_contiguous():
+        raise RuntimeError(f"{what}: kv_scales must be contiguous float32 [..., num_blocks, block_size / tokens, Hkv]")
+    n = src_blocks.numel()
+    args = _id_list(what, "src_blocks", src_blocks, n), _id_list(what, "dst_blocks", dst_blocks, n)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return copy_kv_scales(kv_scales, src_blocks, dst_blocks)
+    *lead, nb, units, hkv = kv_scales.shape
+    slabs = 1
+    for x in lead:
+        slabs *= x
+    check(lib().nq_copy_kv_scales(kv_scales.data_ptr(), slabs, nb, units * hkv, *args, n, raw_stream(dev)), what)
+
+
 def commit_tree(kv_cache, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, parents=None, tokens=None,
                 target_tokens=None, path=None, num_accepted=None):
     """The accepted path of every verified tree, its K/V rows moved to where the sequences go on.
@@ -1088,7 +1120,7 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
     value; the block's first token sets it anew, later ones can only raise it, and then the block's earlier codes are
     coded again.  A block's tokens are appended in order: those of one call are neighbouring rows with rising slots, no
     slot occurs twice, and nothing is kept of what lies behind them in the block.  Rows with a slot outside the pool
-    are transformed and not stored.
+    are transformed and not stored.  Without a ``k_cache`` the rows are only transformed.
     """
     what = "append_kvcache"
     dev = _check_one_device(what, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query, positions,
@@ -1100,14 +1132,17 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
     if key.dim() != 3:
         raise RuntimeError(f"{what}: key and value must be [N, Hkv, D]")
     n, hkv, d = key.shape
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[2:] != (hkv, d) or \
-            v_cache.dtype != k_cache.dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    stored = k_cache is not None
+    if stored and (v_cache is None or slot_mapping is None or value is None):
+        raise RuntimeError(f"{what}: a cache needs value, v_cache and slot_mapping")
+    if stored and (k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[2:] != (hkv, d) or \
+            v_cache.dtype != k_cache.dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous())):
         raise RuntimeError(f"{what}: caches must be contiguous [num_blocks, block_size, {hkv}, {d}] of one dtype")
-    unit = _block_scales(what, k_cache, k_scale, v_scale)
-    for name, t in (("key", key), ("value", value)):
+    unit = _block_scales(what, k_cache, k_scale, v_scale) if stored else 0
+    for name, t in (("key", key), ("value", value)) if stored else (("key", key),):
         if t.shape != key.shape or t.dtype != key.dtype or t.stride(2) != 1 or (t.stride(1) != d and hkv > 1):
             raise RuntimeError(f"{what}: {name} must be [N, Hkv, D] of key's dtype with contiguous heads")
-    if slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous():
+    if stored and (slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous()):
         raise RuntimeError(f"{what}: slot_mapping must be contiguous int32 [{n}]")
     norm = q_weight is not None or k_weight is not None
     for t in (q_weight, k_weight) if norm else ():
@@ -1149,12 +1184,16 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
         ko = _rows_of(what, "k_out", k_out, key.shape, key.dtype)
         if ko[2] != d and hkv > 1:
             raise RuntimeError(f"{what}: k_out must have contiguous heads")
+    if not stored:
+        if not transforms:
+            return q_out, k_out
+        value = k_scale = v_scale = v_cache = slot_mapping = None
     one = hkv * d    # (row strides of single rows mean nothing)
     check(lib().nq_append_kvcache(
-        *qa, ptr(key), key.stride(0) if n > 1 else one, ptr(value), value.stride(0) if n > 1 else one, ptr(positions),
+        *qa, ptr(key), key.stride(0) if n > 1 else one, ptr(value), value.stride(0) if stored and n > 1 else one, ptr(positions),
         ptr(cos_sin_cache), max_pos, int(rotary_dim), ptr(q_weight), ptr(k_weight), float(eps), float(weight_offset), *qo,
         ko[0], ko[1] if n > 1 else one, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(slot_mapping),
-        k_cache.shape[0] * k_cache.shape[1], unit, n, 0 if qa[0] is None else query.shape[-2], hkv, d,
+        k_cache.shape[0] * k_cache.shape[1] if stored else 0, unit, n, 0 if qa[0] is None else query.shape[-2], hkv, d,
         dtype_code(key.dtype), raw_stream(dev)), what)
     return q_out, k_out
 
@@ -1264,4 +1303,4 @@ def _prefill_blocks(what, q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, max_s
 __all__ = ["store_kvcache", "paged_decode", "varlen_prefill", "prepare_decode", "decode_plan", "qk_norm_rope_store",
            "output_gate", "gdn_decode", "gdn_prefill", "gated_rmsnorm", "gdn_conv1d", "tree_attention",
            "tree_masks", "window_prefill", "window_decode", "copy_kv_blocks", "commit_tree", "decode_workspace",
-           "prefill_workspace", "release_workspaces", "decode_schedule", "append_kvcache", "_lib"]
+           "prefill_workspace", "release_workspaces", "decode_schedule", "append_kvcache", "copy_kv_scales", "_lib"]

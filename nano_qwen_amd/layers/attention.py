@@ -9,6 +9,10 @@ fp8 extension (absent from the reference): when the runner binds
 ``[Hkv]``, one scale per kv head of this layer); the store quantizes with
 them and both attention kernels dequantize in registers.
 
+A ``k_scale`` / ``v_scale`` of ``[num_blocks, block_size / tokens, Hkv]`` is a
+scale for each block of tokens and head instead, which the store sets: it is a
+launch of its own then (``kernels.append_kvcache``), in decode too.
+
 Windows and trees (absent from the reference): a layer with a ``window`` sees
 that many tokens up to the query's own, and the sequence's first ``num_sinks``;
 under a ``TreeContext`` a layer without one attends to trees of drafted tokens.
@@ -52,6 +56,10 @@ class Attention(nn.Module):
         self.window = window
         self.num_sinks = num_sinks
 
+    @property
+    def scales_by_block(self) -> bool:
+        return self.k_scale is not None and self.k_scale.dim() == 3
+
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_stored: bool = False,
                 gate: torch.Tensor | None = None):
         """layers/attention.py:59-75: store, then prefill or paged decode
@@ -69,7 +77,7 @@ class Attention(nn.Module):
             return self._forward_span(context, tree_mask, q, k, v, kv_stored, gate)
         k_cache, v_cache = self.k_cache, self.v_cache
         store = k_cache.numel() and v_cache.numel() and not kv_stored
-        if store and not context.is_prefill:
+        if store and not context.is_prefill and not self.scales_by_block:
             # decode: the store rides in the decode launch (nq_paged_decode_store);
             # the reference's asserts of the store still apply
             N, num_heads, head_dim = k.shape
@@ -105,6 +113,11 @@ class Attention(nn.Module):
             raise RuntimeError("Attention: trees of drafted tokens are not supported in layers with a window")
         k_cache, v_cache = self.k_cache, self.v_cache
         store = k_cache.numel() and v_cache.numel() and not kv_stored
+        if tree_mask is not None and self.scales_by_block:
+            raise RuntimeError("Attention: trees of drafted tokens are not supported over a cache with a scale for each block")
+        if store and self.scales_by_block:
+            store_kvcache(k, v, k_cache, v_cache, context.slot_mapping, self.k_scale, self.v_scale)
+            store = False
         if not context.is_prefill:
             new = dict(k=k, v=v, slot_mapping=context.slot_mapping) if store else {}
             return kernels.window_decode(q.unsqueeze(1), k_cache, v_cache, context.context_lens, context.block_tables,

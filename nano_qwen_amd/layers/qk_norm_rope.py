@@ -37,9 +37,11 @@ def qk_norm_rope_store(positions: torch.Tensor, query: torch.Tensor, key: torch.
 
     ``query [N, Hq, D]`` may be the strided query half of ``q_proj``'s output.
     ``weight_offset`` is 1.0 for the Gemma norm (``x * (1 + w)``) and 0.0 for a
-    plain RMSNorm (``x * w``).
+    plain RMSNorm (``x * w``).  ``q_norm`` and ``k_norm`` may both be ``None``, for
+    models that only rotate, where ``attn``'s cache has a scale for each block of
+    tokens and head, or no cache yet.
     """
-    if q_norm.eps != k_norm.eps:
+    if (q_norm is None) != (k_norm is None) or (q_norm is not None and q_norm.eps != k_norm.eps):
         raise RuntimeError("qk_norm_rope_store: q_norm and k_norm must share eps")
     table = rotary_emb.cos_sin_cache
     rot = int(getattr(rotary_emb, "rotary_dim", table.shape[-1]))
@@ -48,6 +50,11 @@ def qk_norm_rope_store(positions: torch.Tensor, query: torch.Tensor, key: torch.
         k_cache, v_cache = attn.k_cache, attn.v_cache
         slots = get_context().slot_mapping
         k_scale, v_scale = attn.k_scale, attn.v_scale
+    if q_norm is None:
+        if k_cache is not None and not attn.scales_by_block:
+            raise RuntimeError("qk_norm_rope_store: without norms only into a cache with a scale for each block")
+        return kernels.append_kvcache(key, value, k_cache, v_cache, slots, k_scale, v_scale, query=query, positions=positions,
+                                      cos_sin_cache=table, rotary_dim=rot)
     return kernels.qk_norm_rope_store(positions, query, key, value, q_norm.weight.detach(),
                                       k_norm.weight.detach(), q_norm.eps, table, rot,
                                       k_cache=k_cache, v_cache=v_cache, slot_mapping=slots,
