@@ -19,6 +19,7 @@
 // but for codes that end below 2^-6.  e4m3's precision is relative, so a finer
 // scale than a power of two would gain nothing but the range's last factor of 2.
 #include <algorithm>
+#include <type_traits>
 
 #include "nq_device.hpp"
 
@@ -26,6 +27,7 @@ namespace nq {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr uint32_t kOdd = (60 + 8 + 127) << 23 | 0x600000;  // bits of 448 * 2^60
 constexpr int kMinExp = -60, kMaxExp = 60;  // of a scale: products with it stay far inside fp32
 
 struct AppendArgs {
@@ -47,13 +49,12 @@ struct AppendArgs {
   float *k_scale, *v_scale;  // [num_slots / unit, hkv]
   const int32_t *slots;
   int64_t num_slots;
-  int unit, n, hq, hkv;
-  int chunk, run_wgs;  // rows whose runs a workgroup takes, and workgroups of runs
+  int unit, unit_log, n, hq, hkv;
+  int chunk, spread, run_wgs;  // rows whose runs a workgroup takes, chunks in turn, workgroups of runs
 };
 
 template <class T>
-__device__ inline void row8(const uint8_t *p, float (&x)[8]) {
-  const u32x4 w = load16(p);
+__device__ inline void widen(const u32x4 &w, float (&x)[8]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     x[2 * t] = T::to_float(static_cast<uint16_t>(w[t] & 0xffffu));
@@ -61,52 +62,99 @@ __device__ inline void row8(const uint8_t *p, float (&x)[8]) {
   }
 }
 template <class T>
+__device__ inline void row8(const uint8_t *p, float (&x)[8]) {
+  widen<T>(load16(p), x);
+}
+template <class T>
 __device__ inline void store8(uint8_t *p, const float (&x)[8]) {
   const u32x4 w{T::pack2(x[0], x[1]), T::pack2(x[2], x[3]), T::pack2(x[4], x[5]), T::pack2(x[6], x[7])};
   __builtin_nontemporal_store(w, reinterpret_cast<u32x4 *>(p));
 }
 
-// Row of one head, 8 dims in each of LPU adjacent lanes (lane l of them): normed
-// and rotated.  The rotary partner of dim e, e +- rot / 2, is rot / 16 lanes away.
+// Rows of one head, 8 dims in each of LPU adjacent lanes (lane l of them), normed and
+// rotated.  The rotary partner of dim e, e +- rot / 2, is rot / 16 lanes away.  N rows
+// at a time, so that their loads and lane exchanges are in flight together.
 template <class T, int LPU>
-__device__ inline void transform(const AppendArgs &a, const uint8_t *weight, int64_t pos, float (&x)[8]) {
-  constexpr int D = 8 * LPU;
-  const int lane = threadIdx.x & 63, e0 = 8 * (threadIdx.x % LPU);
-  if (weight) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-#pragma unroll
-    for (int off = LPU / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, LPU);
-    const float r = 1.0f / __builtin_sqrtf(ss * (1.0f / D) + a.eps);
-    float w[8];
-    row8<T>(weight + 2 * e0, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (w[i] + a.w_off);
+struct Transform {
+  const AppendArgs &a;
+  bool norm, rotates;
+  int partner;
+  float sign;          // of the sines
+  const float *table;  // this lane's cosines in row 0 of the table
+  u32x4 w;             // the norm's factors, before the offset
+
+  __device__ Transform(const AppendArgs &args, const uint8_t *weight) : a(args), norm(weight != nullptr) {
+    const int lane = threadIdx.x & 63, e0 = 8 * (threadIdx.x % LPU), half = a.rot >> 1;
+    const bool first = e0 < half;
+    rotates = e0 < a.rot;
+    sign = first ? -1.f : 1.f;
+    partner = rotates ? (first ? lane + (half >> 3) : lane - (half >> 3)) : lane;
+    table = a.cos_sin + (rotates ? (first ? e0 : e0 - half) : 0);
+    if (norm) w = load16(weight + 2 * e0);
   }
-  if (a.rot > 0) {
-    const int half = a.rot >> 1;
-    const bool rotates = e0 < a.rot, first = e0 < half;
-    const int partner = rotates ? (first ? lane + (half >> 3) : lane - (half >> 3)) : lane;
-    float y[8];
+  __device__ int64_t position(int64_t row) const { return a.rot > 0 ? a.positions[row] : 0; }
+  template <int N>
+  __device__ void operator()(const int64_t (&pos)[N], float (&x)[N][8]) const {
+    bool bad[N];
+    f32x4 c[N][2], s[N][2];
+    if (a.rot > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], partner, 64);
-    const bool bad = pos < 0 || pos >= a.max_position;
-    if (rotates) {
-      const float *cs = a.cos_sin + (bad ? 0 : pos) * a.rot + (first ? e0 : e0 - half);
+      for (int n = 0; n < N; ++n) {
+        bad[n] = static_cast<uint64_t>(pos[n]) >= static_cast<uint64_t>(a.max_position);
+        const float *cs = table + (bad[n] ? 0 : pos[n]) * a.rot;
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const f32x4 c = *reinterpret_cast<const f32x4 *>(cs + i), s = *reinterpret_cast<const f32x4 *>(cs + half + i);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[i + t] = x[i + t] * c[t] + y[i + t] * (first ? -s[t] : s[t]);
+        for (int i = 0; i < 2; ++i) {
+          c[n][i] = *reinterpret_cast<const f32x4 *>(cs + 4 * i);
+          s[n][i] = *reinterpret_cast<const f32x4 *>(cs + (a.rot >> 1) + 4 * i);
+        }
       }
     }
-    if (bad) {
+    if (norm) {
+      float f[8], ss[N];
+      widen<T>(w, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __builtin_nanf("");
+      for (int i = 0; i < 8; ++i) f[i] += a.w_off;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        ss[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss[n] += x[n][i] * x[n][i];
+      }
+#pragma unroll
+      for (int off = LPU / 2; off >= 1; off >>= 1) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) ss[n] += __shfl_xor(ss[n], off, LPU);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float mean = ss[n] * (1.0f / (8 * LPU)) + a.eps;
+        const bool tiny = mean < 0x1p-100f;  // (v_rsq_f32 takes no subnormals)
+        const float r = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p64f : mean) * (tiny ? 0x1p32f : 1.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[n][i] = x[n][i] * r * f[i];
+      }
+    }
+    if (a.rot > 0) {
+      float y[N][8];
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[n][i] = __shfl(x[n][i], partner, 64);
+      if (rotates) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[n][i] = x[n][i] * c[n][i / 4][i % 4] + y[n][i] * sign * s[n][i / 4][i % 4];
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (bad[n]) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[n][i] = __builtin_nanf("");
+        }
     }
   }
-}
+};
 
 __device__ inline float block_scale(float amax) {
   const uint32_t b = f2u(amax);
@@ -114,6 +162,12 @@ __device__ inline float block_scale(float amax) {
   return u2f(static_cast<uint32_t>(min(max(e, kMinExp), kMaxExp) + 127) << 23);
 }
 
+// Largest |x| so far as bits: infinities and NaN come out above all finite ones.
+__device__ inline uint32_t bits_max(uint32_t m, const float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, f2u(x[i]) & 0x7fffffffu);
+  return m;
+}
 // Largest finite |x| so far.
 __device__ inline float finite_max(float m, const float (&x)[8]) {
 #pragma unroll
@@ -124,6 +178,16 @@ __device__ inline float finite_max(float m, const float (&x)[8]) {
   return m;
 }
 
+// Eight codes of values of at most 448 (or NaN).
+__device__ inline u32x2 codes8(const float (&y)[8], float inv) {
+  u32x2 r;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * t] * inv, y[4 * t + 1] * inv, 0, false);
+    r[t] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * t + 2] * inv, y[4 * t + 3] * inv, w, true));
+  }
+  return r;
+}
 // Eight codes times f, coded again.
 __device__ inline u32x2 recode(const u32x2 &c, float f) {
   u32x2 r;
@@ -136,102 +200,194 @@ __device__ inline u32x2 recode(const u32x2 &c, float f) {
   return r;
 }
 
-// Workgroups 0 .. run_wgs - 1 (with a cache): the runs that start in rows chunk * i .. of one
-// head, of K or of V.  The others: the query rows of one token each.
+// The query rows of one token (and its keys, without a cache).
 template <class T, int LPU>
-__global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
-  constexpr int D = 8 * LPU, RPP = kThreads / LPU;  // rows per pass of the workgroup
-  const int lane = threadIdx.x & 63, l = threadIdx.x % LPU, r0 = threadIdx.x / LPU;
-  if (static_cast<int>(blockIdx.x) >= a.run_wgs) {
-    const int64_t tok = static_cast<int>(blockIdx.x) - a.run_wgs;
-    const int64_t pos = a.rot > 0 ? a.positions[tok] : 0;
+__device__ inline void token_rows(const AppendArgs &a, int64_t tok) {
+  constexpr int D = 8 * LPU, RPP = kThreads / LPU;
+  const int l = threadIdx.x % LPU, r0 = threadIdx.x / LPU;
+  if (a.q) {
+    const Transform<T, LPU> f(a, a.q_w);
+    const int64_t pos[1] = {f.position(tok)};
     for (int h = r0; h < a.hq; h += RPP) {
-      float x[8];
-      row8<T>(a.q + tok * a.q_row + h * a.q_head + 16 * l, x);
-      transform<T, LPU>(a, a.q_w, pos, x);
-      store8<T>(a.q_out + tok * a.qo_row + h * a.qo_head + 16 * l, x);
+      float x[1][8];
+      row8<T>(a.q + tok * a.q_row + h * a.q_head + 16 * l, x[0]);
+      f(pos, x);
+      store8<T>(a.q_out + tok * a.qo_row + h * a.qo_head + 16 * l, x[0]);
     }
-    if (!a.k_cache)  // no runs: the keys are these workgroups' too
-      for (int h = r0; h < a.hkv; h += RPP) {
-        float x[8];
-        row8<T>(a.k + tok * a.k_row + (h * D + 8 * l) * 2, x);
-        transform<T, LPU>(a, a.k_w, pos, x);
-        store8<T>(a.k_out + tok * a.ko_row + (h * D + 8 * l) * 2, x);
-      }
-    return;
   }
-  __shared__ float lds_max[kThreads / 64];
-  const int heads = 2 * a.hkv, hw = blockIdx.x % heads, i = blockIdx.x / heads;
+  if (!a.k_cache) {
+    const Transform<T, LPU> f(a, a.k_w);
+    const int64_t pos[1] = {f.position(tok)};
+    for (int h = r0; h < a.hkv; h += RPP) {
+      float x[1][8];
+      row8<T>(a.k + tok * a.k_row + (h * D + 8 * l) * 2, x[0]);
+      f(pos, x);
+      store8<T>(a.k_out + tok * a.ko_row + (h * D + 8 * l) * 2, x[0]);
+    }
+  }
+}
+
+// The runs that start in the rows of one chunk, of one head of K or of V.  Of `spread`
+// chunks in turn, one head each: so all heads of a chunk are on one of the eight XCDs
+// and fill whole lines and all channels of its L2 (head after head, one head's rows on
+// each XCD: 6 us more of 97).
+// kHold passes of rows are held in registers between their maximum and their codes;
+// the rows of a longer run are read and transformed a second time.  (Held four, for
+// runs of 64 rows whole: 209 registers, 94 us with the query rows' kernel apart, where
+// two took 98.)
+template <class T, int LPU>
+__device__ inline void run_rows(const AppendArgs &a, int wg) {
+  constexpr int D = 8 * LPU, RPP = kThreads / LPU, kHold = 2;  // (RPP: rows per pass of the workgroup)
+  __shared__ uint32_t lds_max[kThreads / 64];
+  const int lane = threadIdx.x & 63, l = threadIdx.x % LPU, r0 = threadIdx.x / LPU;
+  const int heads = 2 * a.hkv, j = wg / a.spread, hw = j % heads, i = j / heads * a.spread + (wg - j * a.spread);
   const bool is_v = hw >= a.hkv;
   const int h = is_v ? hw - a.hkv : hw;
   const uint8_t *src = (is_v ? a.v : a.k) + h * D * 2 + 16 * l;
   const int64_t src_row = is_v ? a.v_row : a.k_row;
   uint8_t *cache = is_v ? a.v_cache : a.k_cache;
   float *scales = is_v ? a.v_scale : a.k_scale;
-  // rows of the chunk that begin a run
-  const int row = i * a.chunk + lane;
-  bool begins = false;
-  if (lane < a.chunk && row < a.n) {
-    const int32_t s = a.slots[row];
-    const bool stored = s >= 0 && s < a.num_slots;
-    begins = !stored || row == 0 || s % a.unit == 0 || a.slots[row - 1] != s - 1;
-  }
-  uint64_t todo = __builtin_amdgcn_ballot_w64(begins);
-  while (todo != 0) {
-    const int r = i * a.chunk + static_cast<int>(__builtin_ctzll(todo));
-    todo &= todo - 1;
-    const int32_t slot = __builtin_amdgcn_readfirstlane(a.slots[r]);
-    const bool stored = slot >= 0 && slot < a.num_slots;
-    const int off = stored ? slot % a.unit : 0;
-    int len = 1;
-    if (stored) {
-      const int most = min(a.unit - off, a.n - r);
-      for (int b = 0; b < most; b += 64) {
-        const bool stop = b + lane >= most || a.slots[r + b + lane] != slot + b + lane;
-        const uint64_t m = __builtin_amdgcn_ballot_w64(stop);
-        len = b + (m ? static_cast<int>(__builtin_ctzll(m)) : 64);
-        if (m) break;
-      }
-    }
-    auto value = [&](int t, float (&x)[8]) {
-      row8<T>(src + (r + t) * src_row, x);
-      if (!is_v) transform<T, LPU>(a, a.k_w, a.rot > 0 ? a.positions[r + t] : 0, x);
-    };
-    float amax = 0.f;
-    for (int t = r0; t < len; t += RPP) {
-      float x[8];
-      value(t, x);
-      if (!is_v && a.k_out) store8<T>(a.k_out + (r + t) * a.ko_row + h * D * 2 + 16 * l, x);
-      amax = finite_max(amax, x);
-    }
-    if (!stored) continue;  // the whole workgroup
+  uint8_t *k_out = is_v ? nullptr : a.k_out;
+  const int unit = a.unit, row0 = i * a.chunk;
+  // The slots of 64 rows from the chunk's first on (-1: not stored), and which of
+  // them begin a run: the first of its sequence or block, or one that is not stored.
+  auto slot_of = [&](int row) -> int32_t {
+    const int32_t s = row >= 0 && row < a.n ? a.slots[row] : -1;
+    return s >= 0 && s < a.num_slots ? s : -1;
+  };
+  const int32_t slots = slot_of(row0 + lane), ahead = slot_of(row0 - 1);
+  const int32_t below = __shfl_up(slots, 1);  // (by every lane: one that is masked off gives nothing)
+  const int32_t before = lane > 0 ? below : ahead;
+  const uint64_t begins = __builtin_amdgcn_ballot_w64(slots < 0 || (slots & (unit - 1)) == 0 || before != slots - 1);
+  uint64_t todo = begins & (a.chunk == 64 ? ~0ull : (1ull << a.chunk) - 1);
+  if (a.n - row0 < 64) todo &= row0 < a.n ? (1ull << (a.n - row0)) - 1 : 0;
+  if (todo == 0) return;
+  const Transform<T, LPU> f(a, is_v ? nullptr : a.k_w);
+  auto over_workgroup = [&](uint32_t m) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    const int64_t c = slot / a.unit * static_cast<int64_t>(a.hkv) + h;
-    const float was = off > 0 ? scales[c] : 0.f;
-    __syncthreads();  // the last run's maxima have been read
-    if (lane == 0) lds_max[threadIdx.x / 64] = amax;
+    for (int o = 32; o >= 1; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o, 64)));
+    __syncthreads();  // the last maxima have been read
+    if (lane == 0) lds_max[threadIdx.x / 64] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) amax = fmaxf(amax, lds_max[w]);
-    const float need = block_scale(amax);
-    const float s = off > 0 ? fminf(fmaxf(was, need), u2f((kMaxExp + 127u) << 23)) : need;
+    for (int w = 0; w < kThreads / 64; ++w) m = max(m, lds_max[w]);
+    return m;
+  };
+  while (todo != 0) {
+    const int at = static_cast<int>(__builtin_ctzll(todo));
+    todo &= todo - 1;
+    const int r = row0 + at;
+    const int32_t slot = __builtin_amdgcn_readlane(slots, at);
+    const bool stored = slot >= 0;
+    const int off = stored ? slot & (unit - 1) : 0;
+    int len = 1;
+    if (stored) {
+      const uint64_t later = at < 63 ? begins >> (at + 1) : 0;
+      len = later ? 1 + static_cast<int>(__builtin_ctzll(later)) : 64 - at;
+      if (later == 0)  // to the end of the 64 rows: on from there
+        for (int b = len;; b += 64) {
+          const bool stop = off + b + lane >= unit || slot_of(r + b + lane) != slot + b + lane;
+          const uint64_t m = __builtin_amdgcn_ballot_w64(stop);
+          len = b + (m ? static_cast<int>(__builtin_ctzll(m)) : 64);
+          if (m) break;
+        }
+    }
+    const int64_t c = static_cast<int64_t>(static_cast<uint32_t>(slot) >> a.unit_log) * a.hkv + h;
+    const float was = off > 0 ? scales[c] : 0.f;
+    uint32_t top = 0;
+    // Rows t, t + RPP .. of the run; a lane past its end takes the last row.
+    auto value = [&](int t, auto &y) {
+      constexpr int N = sizeof(y) / sizeof(y[0]);
+      int64_t pos[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int64_t row = r + min(t + n * RPP, len - 1);
+        row8<T>(src + row * src_row, y[n]);
+        pos[n] = is_v ? 0 : f.position(row);
+      }
+      if (!is_v) f(pos, y);
+    };
+    auto see = [&](int t, const auto &y) {
+#pragma unroll
+      for (int n = 0; n < static_cast<int>(sizeof(y) / sizeof(y[0])); ++n) {
+        const int i = t + n * RPP;
+        if (k_out && i < len) store8<T>(k_out + (r + i) * a.ko_row + h * D * 2 + 16 * l, y[n]);
+        top = bits_max(top, y[n]);
+      }
+    };
+    float held[kHold][8];
+    if (len <= RPP) {
+      float(&one)[1][8] = reinterpret_cast<float(&)[1][8]>(held);
+      value(r0, one);
+      see(r0, one);
+    } else {
+      value(r0, held);
+      see(r0, held);
+    }
+    for (int t = kHold * RPP; t < len; t += 2 * RPP) {
+      float y[2][8];
+      value(t + r0, y);
+      see(t + r0, y);
+    }
+    if (!stored) continue;  // the whole workgroup
+    uint32_t m = over_workgroup(top);
+    const bool odd = m > kOdd;  // infinities or NaN among them, or more than the largest scale reaches
+    if (odd) {
+      float amax = 0.f;
+#pragma unroll
+      for (int p = 0; p < kHold; ++p)
+        if (p * RPP + r0 < len) amax = finite_max(amax, held[p]);
+      for (int t = kHold * RPP; t < len; t += RPP) {
+        float y[1][8];
+        value(t + r0, y);
+        amax = finite_max(amax, y[0]);
+      }
+      m = over_workgroup(f2u(amax));
+    }
+    const float amax = u2f(m);
+    const float s = off > 0 ? fmaxf(was, block_scale(amax)) : block_scale(amax);
     const float inv = 1.0f / s;
     if (threadIdx.x == 0 && s != was) scales[c] = s;
+    const int64_t row_b = static_cast<int64_t>(a.hkv) * D;
     uint8_t *dst = cache + (static_cast<int64_t>(slot - off) * a.hkv + h) * D + 8 * l;
-    if (off > 0 && s > was) {
+    if (off > 0 && s > was)
       for (int t = r0; t < off; t += RPP) {
-        u32x2 *p = reinterpret_cast<u32x2 *>(dst + static_cast<int64_t>(t) * a.hkv * D);
+        u32x2 *p = reinterpret_cast<u32x2 *>(dst + t * row_b);
         *p = recode(*p, was * inv);
       }
-    }
-    for (int t = r0; t < len; t += RPP) {
-      float x[8];
-      value(t, x);
-      *reinterpret_cast<u32x2 *>(dst + static_cast<int64_t>(off + t) * a.hkv * D) =
-          u32x2{fp8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv), fp8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
+    auto code = [&](int t, const float (&y)[8]) {
+      if (t < len)
+        *reinterpret_cast<u32x2 *>(dst + (off + t) * row_b) =
+            odd ? u32x2{fp8x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv), fp8x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)}
+                : codes8(y, inv);
+    };
+#pragma unroll
+    for (int p = 0; p < kHold; ++p) code(p * RPP + r0, held[p]);
+    for (int t = kHold * RPP; t < len; t += 2 * RPP) {
+      float y[2][8];
+      value(t + r0, y);
+      code(t + r0, y[0]);
+      code(t + RPP + r0, y[1]);
     }
   }
+}
+
+template <class T>
+constexpr int kWaves = std::is_same<T, BF16>::value ? 4 : 3;  // per SIMD
+
+// The first run_wgs workgroups take the runs, the others the query rows of a token
+// each.  Bound: with many rows by their traffic and by the arithmetic of the runs
+// about equally (14533 prompt tokens of 32 and 8 heads of 128 with norms: 97 us for
+// 365 MB, 3.7 TB/s; a copy of as much takes 72); a step's few rows by one
+// workgroup's chain of round trips (4.5 us).  Four waves per SIMD, which fp16's
+// registers miss by three.  Two kernels, the query rows' with 57 registers: 97 us
+// too, 6 us more at 1024 tokens.
+template <class T, int LPU>
+__global__ __launch_bounds__(kThreads, kWaves<T>) void append_kernel(const AppendArgs a) {
+  if (static_cast<int>(blockIdx.x) < a.run_wgs)
+    run_rows<T, LPU>(a, blockIdx.x);
+  else
+    token_rows<T, LPU>(a, static_cast<int>(blockIdx.x) - a.run_wgs);
 }
 
 template <class T>
@@ -310,20 +466,25 @@ extern "C" int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_
   a.slots = slot_mapping;
   a.num_slots = num_slots;
   a.unit = scale_block;
+  a.unit_log = k_cache ? __builtin_ctz(scale_block) : 0;
   a.n = static_cast<int>(num_tokens);
   a.hq = num_q_heads;
   a.hkv = num_kv_heads;
   // Rows per workgroup of runs: few rows are a decode step's, every one a run of
-  // its own; of many, most continue the row before them.
-  a.chunk = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, num_tokens / 512)));
-  const int64_t runs = k_cache ? (num_tokens + a.chunk - 1) / a.chunk * 2 * num_kv_heads : 0;
-  const int64_t grid = runs + (q || !k_cache ? num_tokens : 0);
-  if (grid > 0x7fffffff) return fail(NQ_EINVAL, "%s: %lld tokens of %d heads", what, (long long)num_tokens, num_kv_heads);
+  // its own; of many, most continue the row before them (a prompt's rows 64 at a
+  // time from 8192 rows on: 97 us at 14533; a quarter as many, 110).
+  a.chunk = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, num_tokens / 128)));
+  const int64_t chunks = (num_tokens + a.chunk - 1) / a.chunk;
+  a.spread = static_cast<int>(std::min<int64_t>(chunks, 8));
+  const int64_t runs = k_cache ? (chunks + a.spread - 1) / a.spread * a.spread * 2 * num_kv_heads : 0;
+  const int64_t tokens = q || !k_cache ? num_tokens : 0;
+  if (runs + tokens > 0xffffffffll / kThreads)  // (threads of a launch are counted in 32 bits)
+    return fail(NQ_EINVAL, "%s: %lld tokens of %d heads", what, (long long)num_tokens, num_kv_heads);
   a.run_wgs = static_cast<int>(runs);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == NQ_BF16)
-    launch<BF16>(a, head_dim, static_cast<unsigned>(grid), s);
+    launch<BF16>(a, head_dim, static_cast<unsigned>(runs + tokens), s);
   else
-    launch<F16>(a, head_dim, static_cast<unsigned>(grid), s);
+    launch<F16>(a, head_dim, static_cast<unsigned>(runs + tokens), s);
   return check_launch(what);
 }
