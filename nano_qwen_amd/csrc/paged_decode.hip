@@ -995,11 +995,16 @@ int decode_heads_per_wg(int hkv, bool fp8) { return (fp8 && hkv >= 8) ? 8 : 4; }
 // shape: HPW kv heads (waves) per workgroup, DEPTH steps of raw K/V in
 // flight, WPE waves per SIMD.  Register budget per wave = in-flight K/V +
 // state: two steps deep (bf16: 2 waves/SIMD, fp8: 3).  head_dim 256: twice
-// the raw K/V per step, one step in flight, one wave per SIMD.
-template <bool FP8, int D, class F>
+// the raw K/V per step, one step in flight, one wave per SIMD.  There, with block
+// scales and at most two kv heads, workgroups of two waves, two per CU: of four, two
+// would have no head (96 sequences of 0-5000 tokens, 2 kv heads: 84 us with four).
+template <bool FP8, int D, bool BLK = false, class F>
 int with_decode_shape(int hpw, F &&f) {
   if constexpr (D == 256) {
     if constexpr (FP8) {
+      if constexpr (BLK) {
+        if (hpw == 2) return f.template run<2, 1, 1>();
+      }
       if (hpw == 8) return f.template run<8, 1, 1>();
       return f.template run<4, 1, 1>();
     } else {
@@ -1010,9 +1015,10 @@ int with_decode_shape(int hpw, F &&f) {
     return f.template run<4, 2, FP8 ? 3 : 2>();
   }
 }
-template <bool FP8, int D>
+template <bool FP8, int D, bool BLK = false>
 int decode_hpw(int hkv) {
   const int hpw = decode_heads_per_wg(hkv, FP8);
+  if (BLK && D == 256 && hkv <= 2) return 2;
   return (D == 256 && !FP8) ? 4 : hpw;  // eight waves of ~360 registers do not fit a CU
 }
 
@@ -1079,8 +1085,9 @@ int sk_ranges(int batch, int hq, int hkv, int64_t max_tokens, int block_size, in
   if (num_splits <= 1 || !sk_eligible(batch, max_tokens, block_size)) return 0;
   const size_t lds = static_cast<size_t>(H) * DecodeWave<T, FP8, D>::LDS_PER_WAVE_B;
   auto *kern = paged_decode_sk_kernel<T, FP8, D, H, DP, (WP > 2 ? 2 : WP), BLK>;
-  if (kernel_occupancy(reinterpret_cast<const void *>(kern), 64 * H, lds) != 1) return 0;
-  const int W = sk_workgroups(1, (hkv + H - 1) / H, batch, max_tokens, block_size);
+  constexpr int kOcc = H == 2 ? 2 : 1;
+  if (kernel_occupancy(reinterpret_cast<const void *>(kern), 64 * H, lds) != kOcc) return 0;
+  const int W = sk_workgroups(kOcc, (hkv + H - 1) / H, batch, max_tokens, block_size);
   return sk_workspace_bytes(W, hq, D) <= ws_bytes ? W : 0;
 }
 
@@ -1110,7 +1117,7 @@ struct DecodeLaunch {
         k.ws_lse = reinterpret_cast<float *>(a.ws_raw + align256(static_cast<int64_t>(W) * 2 * a.Hq * D * 4));
         k.sk_bnd = reinterpret_cast<int2 *>(a.ws_raw + align256(static_cast<int64_t>(W) * 2 * a.Hq * D * 4) +
                                             align256(static_cast<int64_t>(W) * 2 * a.Hq * 4));
-        kern<<<dim3(W, groups), 64 * H, lds, s>>>(k, batch, W, std::max(1, device_cus() / groups));
+        kern<<<dim3(W, groups), 64 * H, lds, s>>>(k, batch, W, std::max(1, device_cus() * (H == 2 ? 2 : 1) / groups));
         const int rc = check_launch("paged_decode(stream-K)");
         if (rc != NQ_OK) return rc;
         if (W <= kMergeUnroll / 2 * batch)
@@ -1161,7 +1168,7 @@ struct DecodeSchedule {
 
 template <class T, bool FP8, int D, bool BLK = false>
 int launch_decode(const DecodeArgs &a, int batch, hipStream_t s) {
-  return with_decode_shape<FP8, D>(decode_hpw<FP8, D>(a.Hkv), DecodeLaunch<T, FP8, D, BLK>{a, batch, s});
+  return with_decode_shape<FP8, D, BLK>(decode_hpw<FP8, D, BLK>(a.Hkv), DecodeLaunch<T, FP8, D, BLK>{a, batch, s});
 }
 
 // Stream-K workgroups per group the head_dim-D kernel would launch for
@@ -1556,6 +1563,11 @@ static int decode_auto(const void *q, int64_t q_batch_stride, int64_t q_head_str
     rc = nq_decode_plan(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size, kv_dtype, &ns, &st);
     if (rc != NQ_OK) return rc;
     bytes = nq_decode_workspace_bytes(batch, num_q_heads, head_dim, ns);
+  }
+  if (scale_block > 0 && head_dim == 256 && num_kv_heads <= 2 && bytes > 0 && !fused) {  // (two ranges per CU)
+    const int64_t tokens = static_cast<int64_t>(max_blocks_per_seq) * block_size;
+    if (sk_eligible(batch, tokens, block_size))
+      bytes = std::max(bytes, sk_workspace_bytes(sk_workgroups(2, 1, batch, tokens, block_size), num_q_heads, head_dim));
   }
   if (bytes > 0 && (!workspace || workspace_bytes < bytes)) {
     if (!need) return fail(NQ_EINVAL, "paged_decode_auto: workspace %lld bytes < %lld", (long long)workspace_bytes, (long long)bytes);

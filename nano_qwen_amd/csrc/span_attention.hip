@@ -252,7 +252,8 @@ __device__ __forceinline__ int item_cost(const A &a, const Seq &q) {
 // whatever the scales.  The scales of 64 tiles are loaded with the list of where
 // they lie; what a tile needs of them is formed for all 64 at once, a tile per
 // lane, and read from there (formed tile by tile, with a select per ring slot on
-// top: a chunk of 2048 tokens behind 14336 662 us, against XXX).
+// top, and all tiles in one loop: a chunk of 2048 tokens behind 14336 in 662 us; this
+// and a loop for most tiles: 637, where a scale per head takes 597).
 template <class T, bool FP8, class S, bool BLK>
 __device__ __forceinline__ void span_body() {
   constexpr int D = S::D, RW = S::RW, QS = S::QS, M = S::M, SLOTS = S::SLOTS, COPS = S::COPS;
@@ -1242,10 +1243,10 @@ __device__ __forceinline__ void span_body() {
         };
         if constexpr (BLK) {
           // Most tiles run in a loop of their own, which holds no scalar register for
-          // the others' tests (a chunk of 2048 tokens behind 14336 658 us in one loop,
-          // 624).  The first tile has products of zeros behind it: with a step of its
-          // own, as below, the kernel outgrew the instruction cache (98 KB; six chats
-          // 206 us, ZZZ).
+          // the others' tests (a chunk of 2048 tokens behind 14336: 658 us in one loop,
+          // 637 in two).  The first tile has products of zeros behind it: with a step of
+          // its own, as below, there is one more copy of the step, 98 KB of code in all,
+          // more than the instruction cache holds.
 #pragma unroll
           for (int j = 0; j < NJ; ++j) vf[j] = KV{};
 #pragma unroll

@@ -1091,13 +1091,14 @@ _APPEND_FIRST = "append_kvcache stores the new token of a cache with a scale for
 
 def _block_scales(what, k_cache, k_scale, v_scale):
     """Tokens per block of scales ``[num_blocks, block_size / tokens, Hkv]``, checked against their e4m3 cache."""
-    nb, bs, hkv, _ = k_cache.shape
-    for t in (k_scale, v_scale):
-        if t is None or t.dtype != torch.float32 or t.dim() != 3 or t.shape != k_scale.shape or not t.is_contiguous():
-            raise RuntimeError(f"{what}: k_scale and v_scale must be contiguous float32 [num_blocks, block_size / tokens, Hkv]")
-    units = k_scale.shape[1]
-    if k_scale.shape[0] != nb or k_scale.shape[2] != hkv or units == 0 or bs % units or bs // units not in SCALE_BLOCKS:
-        raise RuntimeError(f"{what}: scales {list(k_scale.shape)} of a cache {list(k_cache.shape)}: blocks of "
+    shape = None if k_scale is None else k_scale.shape
+    if shape is None or v_scale is None or len(shape) != 3 or v_scale.shape != shape or \
+            k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or \
+            not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise RuntimeError(f"{what}: k_scale and v_scale must be contiguous float32 [num_blocks, block_size / tokens, Hkv]")
+    (nb, bs, hkv, _), (pages, units, heads) = k_cache.shape, shape
+    if pages != nb or heads != hkv or units == 0 or bs % units or bs // units not in SCALE_BLOCKS:
+        raise RuntimeError(f"{what}: scales {list(shape)} of a cache {list(k_cache.shape)}: blocks of "
                            f"{', '.join(map(str, SCALE_BLOCKS))} tokens")
     if k_cache.dtype != torch.float8_e4m3fn:
         raise RuntimeError(f"{what}: a scale for each block needs a float8_e4m3fn cache")
@@ -1139,9 +1140,12 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
             v_cache.dtype != k_cache.dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous())):
         raise RuntimeError(f"{what}: caches must be contiguous [num_blocks, block_size, {hkv}, {d}] of one dtype")
     unit = _block_scales(what, k_cache, k_scale, v_scale) if stored else 0
-    for name, t in (("key", key), ("value", value)) if stored else (("key", key),):
-        if t.shape != key.shape or t.dtype != key.dtype or t.stride(2) != 1 or (t.stride(1) != d and hkv > 1):
-            raise RuntimeError(f"{what}: {name} must be [N, Hkv, D] of key's dtype with contiguous heads")
+    if stored and (value.shape != key.shape or value.dtype != key.dtype):
+        raise RuntimeError(f"{what}: value must be {list(key.shape)} of {key.dtype}")
+    k_strides, v_strides = key.stride(), value.stride() if stored else (hkv * d, d, 1)
+    for x in (k_strides, v_strides):
+        if x[2] != 1 or (x[1] != d and hkv > 1):
+            raise RuntimeError(f"{what}: key and value must be [N, Hkv, D] with contiguous heads")
     if stored and (slot_mapping.dtype != torch.int32 or slot_mapping.shape != (n,) or not slot_mapping.is_contiguous()):
         raise RuntimeError(f"{what}: slot_mapping must be contiguous int32 [{n}]")
     norm = q_weight is not None or k_weight is not None
@@ -1170,7 +1174,9 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
         qa = _rows_of(what, "query", query, shape, key.dtype)
         if q_out is None:
             q_out = torch.empty(shape, dtype=key.dtype, device=key.device)
-        qo = _rows_of(what, "q_out", q_out, shape, key.dtype)
+            qo = (q_out.data_ptr(), shape[1] * d, d)
+        else:
+            qo = _rows_of(what, "q_out", q_out, shape, key.dtype)
     ko = (None, 0)
     if not transforms:
         if k_out is not None:
@@ -1179,18 +1185,20 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
     else:
         if k_out is None:
             k_out = torch.empty(n, hkv, d, dtype=key.dtype, device=key.device)
-        elif _overlaps(k_out, key):    # a long run's keys are read twice
-            raise RuntimeError(f"{what}: k_out must not overlap key")
-        ko = _rows_of(what, "k_out", k_out, key.shape, key.dtype)
-        if ko[2] != d and hkv > 1:
-            raise RuntimeError(f"{what}: k_out must have contiguous heads")
+            ko = (k_out.data_ptr(), hkv * d)
+        else:
+            if _overlaps(k_out, key):    # a long run's keys are read twice
+                raise RuntimeError(f"{what}: k_out must not overlap key")
+            ko = _rows_of(what, "k_out", k_out, key.shape, key.dtype)
+            if ko[2] != d and hkv > 1:
+                raise RuntimeError(f"{what}: k_out must have contiguous heads")
     if not stored:
         if not transforms:
             return q_out, k_out
         value = k_scale = v_scale = v_cache = slot_mapping = None
     one = hkv * d    # (row strides of single rows mean nothing)
     check(lib().nq_append_kvcache(
-        *qa, ptr(key), key.stride(0) if n > 1 else one, ptr(value), value.stride(0) if stored and n > 1 else one, ptr(positions),
+        *qa, ptr(key), k_strides[0] if n > 1 else one, ptr(value), v_strides[0] if n > 1 else one, ptr(positions),
         ptr(cos_sin_cache), max_pos, int(rotary_dim), ptr(q_weight), ptr(k_weight), float(eps), float(weight_offset), *qo,
         ko[0], ko[1] if n > 1 else one, ptr(k_cache), ptr(v_cache), ptr(k_scale), ptr(v_scale), ptr(slot_mapping),
         k_cache.shape[0] * k_cache.shape[1] if stored else 0, unit, n, 0 if qa[0] is None else query.shape[-2], hkv, d,
