@@ -1236,10 +1236,13 @@ def _decode_blocks(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scal
     unit = _block_scales(what, k_cache, k_scale, v_scale)
     if cache_seqlens.dtype != torch.int32 or cache_seqlens.numel() != B or not cache_seqlens.is_contiguous():
         raise RuntimeError(f"{what}: cache_seqlens must be contiguous int32 [B]")
+    shape = (B, hq, d)
+    qa = _rows_of(what, "q", q, shape, q.dtype)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    shape = (B, hq, d)
-    qa, oa = _rows_of(what, "q", q, shape, q.dtype), _rows_of(what, "out", out, shape, q.dtype)
+        oa = (out.data_ptr(), hq * d, d)
+    else:
+        oa = _rows_of(what, "out", out, shape, q.dtype)
     ga = (None, 0, 0) if gate is None else _rows_of(what, "gate", gate, shape, q.dtype)
     key, need = (dev, raw_stream(dev)), ctypes.c_int64()
     width = block_table.shape[1]
