@@ -997,7 +997,8 @@ int decode_heads_per_wg(int hkv, bool fp8) { return (fp8 && hkv >= 8) ? 8 : 4; }
 // state: two steps deep (bf16: 2 waves/SIMD, fp8: 3).  head_dim 256: twice
 // the raw K/V per step, one step in flight, one wave per SIMD.  There, with block
 // scales and at most two kv heads, workgroups of two waves, two per CU: of four, two
-// would have no head (96 sequences of 0-5000 tokens, 2 kv heads: 84 us with four).
+// would have no head (96 sequences of 0-5000 tokens, 2 kv heads: 84 us with four,
+// 62 with two).
 template <bool FP8, int D, bool BLK = false, class F>
 int with_decode_shape(int hpw, F &&f) {
   if constexpr (D == 256) {
@@ -1120,7 +1121,8 @@ struct DecodeLaunch {
         kern<<<dim3(W, groups), 64 * H, lds, s>>>(k, batch, W, std::max(1, device_cus() * (H == 2 ? 2 : 1) / groups));
         const int rc = check_launch("paged_decode(stream-K)");
         if (rc != NQ_OK) return rc;
-        if (W <= kMergeUnroll / 2 * batch)
+        // (two-wave workgroups: twice the ranges; 9.4 us, against 13.8 with groups, at 5 pieces a sequence)
+        if (W <= (H == 2 ? kMergeUnroll : kMergeUnroll / 2) * batch)
           merge_sk<1>(k, W);
         else
           merge_sk<kMergeGroups>(k, W);

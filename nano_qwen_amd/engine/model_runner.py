@@ -15,7 +15,10 @@ also creates ``kv_scales [2, L, Hkv]`` float32 (initialised to 1) and binds
 ``module.k_scale = kv_scales[0, l]`` / ``module.v_scale = kv_scales[1, l]``;
 ``calibrate_kv_scales`` sets them to absmax/448 per (layer, kv head).  The
 pool is sized from the memory budget with the *cache* dtype's item size, so
-an fp8 pool holds twice the blocks of a bf16 one in the same budget.
+an fp8 pool holds twice the blocks of a bf16 one in the same budget.  With
+``kv_scale_block=64`` (or 32, 128, 256) every 64 tokens of a page have scales of
+their own per head, ``kv_scales [2, L, num_blocks, block_size / 64, Hkv]``, which
+the stores set and nothing calibrates.
 """
 from __future__ import annotations
 
