@@ -748,8 +748,8 @@ int nq_commit_tree(void *kv_cache, int64_t num_slabs, int64_t num_blocks, int bl
  * neither; x / rms(x) * (w + weight_offset)), their first rotary_dim dims
  * rotated by cos_sin_cache[positions[i]] (float32: rotary_dim / 2 cosines, then
  * the sines), in fp32, and rounded once to q_out and k_out (null: keys are
- * stored as they are given out, and not given out; must not overlap k).  A
- * position outside [0, max_position) makes its row NaN.
+ * stored as they are given out, and not given out).  q_out may be q; otherwise
+ * the outputs overlap no input.  A position outside [0, max_position) makes its row NaN.
  *
  * The scale of a block and head becomes the smallest power of two, from 2^-60
  * to 2^60, whose 448-fold no finite value of the call's rows in it exceeds, or,

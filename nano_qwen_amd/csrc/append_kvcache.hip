@@ -441,6 +441,7 @@ extern "C" int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_
   if (!k || (k_cache ? !v || !v_cache || !k_scale || !v_scale || !slot_mapping : !k_out) || (q && (!q_out || num_q_heads == 0)) ||
       (rotary_dim > 0 && (!positions || !cos_sin_cache)))
     return fail(NQ_EINVAL, "%s: null pointer", what);
+  if (rotary_dim > 0 && max_position == 0) return fail(NQ_EINVAL, "%s: no rows in cos_sin_cache", what);
   const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
   if (k_row_stride < row || (k_cache && v_row_stride < row) || (k_out && k_out_row_stride < row))
     return fail(NQ_EINVAL, "%s: rows narrower than their heads", what);

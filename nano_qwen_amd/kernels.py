@@ -1121,7 +1121,8 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
     value; the block's first token sets it anew, later ones can only raise it, and then the block's earlier codes are
     coded again.  A block's tokens are appended in order: those of one call are neighbouring rows with rising slots, no
     slot occurs twice, and nothing is kept of what lies behind them in the block.  Rows with a slot outside the pool
-    are transformed and not stored.  Without a ``k_cache`` the rows are only transformed.
+    are transformed and not stored.  Without a ``k_cache`` the rows are only transformed.  ``q_out`` may be the query
+    itself; otherwise the outputs overlap no input.
     """
     what = "append_kvcache"
     dev = _check_one_device(what, key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, query, positions,
@@ -1208,14 +1209,13 @@ def append_kvcache(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale,
 
 def _decode_counters_and_workspace(key, bytes_of):
     """What a decode's launch takes besides its tensors, with the stream's lock held: its counters (``bytes_of``: as many
-    as it needs during a capture) and workspace, or ``None``."""
+    as it needs during a capture) and workspace, or ``None`` (a captured one's workspace is its graph's own)."""
     if key[1] != 0 and _capturing(key):    # the null stream cannot be captured
         nbytes = bytes_of()
-        counters = _captured_counter_slot(key, nbytes) if 0 < nbytes <= _COUNTER_SLOT_BYTES else None
-    else:
-        counters = _decode_counters.get(key)
-        if counters is None:
-            counters = _decode_counter_slot(key)
+        return _captured_counter_slot(key, nbytes) if 0 < nbytes <= _COUNTER_SLOT_BYTES else None, None
+    counters = _decode_counters.get(key)
+    if counters is None:
+        counters = _decode_counter_slot(key)
     return counters, _workspaces.get(key)
 
 
@@ -1257,7 +1257,10 @@ def _decode_blocks(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scal
                 ptr(counters), 0 if counters is None else counters.numel() * 4, need, key[1])
             if rc != 1:
                 break
-            ws = decode_workspace(q.device, need.value)
+            if key[1] != 0 and _capturing(key):    # the graph's own: replays may overlap other calls
+                ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            else:
+                ws = decode_workspace(q.device, need.value)
     check(rc, what)
     return out
 

@@ -37,6 +37,18 @@ def test_append_refusals(host):
         assert "status -3" not in str(e.value), (list(kw), str(e.value))
 
 
+def test_append_refuses_a_table_without_rows(host):
+    """Rows of positions outside the table are NaN, but are read from its first row all the same."""
+    good, _ = refusals("cpu")
+    rot = 64
+    pos = torch.zeros(good["key"].shape[0], dtype=torch.int64)
+    for rows in (0, 1):
+        kw = good | dict(positions=pos, rotary_dim=rot, cos_sin_cache=torch.zeros(4, rot)[:rows], query=None)
+        with pytest.raises(RuntimeError) as e:
+            kernels.append_kvcache(**kw)
+        assert ("status -3" in str(e.value)) == (rows == 1), str(e.value)
+
+
 def test_append_refuses_tensors_on_the_host():
     good, _ = refusals("cpu")
     with pytest.raises(RuntimeError, match="HIP device"):

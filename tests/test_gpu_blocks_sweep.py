@@ -112,6 +112,29 @@ def test_pool_past_32_bits(cuda, monkeypatch, choice):
     assert (near[2][-1, 1:3] > 2.0 ** -9).all() and (near[0][-1, 100:190] != 0x31).any()
 
 
+@pytest.mark.parametrize("d", [128, 256])
+def test_graphs_replayed_at_once(cuda, d):
+    """Decodes of several pieces in two graphs captured on one stream: each has a workspace of its own."""
+    cases = [Case([1] * 40, [1500 + 7 * j + i for j in range(40)], 16, 2, d, BF, 256, 64, seed=i).to(cuda) for i in range(2)]
+    want = [c.decode() for c in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in cases], []
+    for g, c in zip(graphs, cases):
+        with torch.cuda.graph(g):
+            outs.append(c.decode())
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(7)
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 @pytest.mark.parametrize("what", ["decode", "prefill"])
 def test_threads_on_one_stream(cuda, what):
     cases = [Case([1] * 3 if what == "decode" else [300, 90], [3000, 1500 + 64 * i, 77][:3 if what == "decode" else 2], 16, 2,
