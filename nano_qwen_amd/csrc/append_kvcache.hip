@@ -392,7 +392,7 @@ constexpr int kWaves = std::is_same<T, BF16>::value ? 4 : 3;  // per SIMD
 // 365 MB, 3.7 TB/s; a copy of as much takes 72); a step's few rows by one
 // workgroup's chain of round trips (4.5 us).  Four waves per SIMD, which fp16's
 // registers miss by three.  Two kernels, the query rows' with 57 registers: 97 us
-// too, 6 us more at 1024 tokens.
+// too, 8 us more at 1024 tokens.
 template <class T, int LPU>
 __global__ __launch_bounds__(kThreads, kWaves<T>) void append_kernel(const AppendArgs a) {
   if (static_cast<int>(blockIdx.x) < a.run_wgs)
@@ -483,8 +483,8 @@ extern "C" int nq_append_kvcache(const void *q, int64_t q_row_stride, int64_t q_
   a.hq = num_q_heads;
   a.hkv = num_kv_heads;
   // Rows per workgroup of runs: few rows are a decode step's, every one a run of
-  // its own; of many, most continue the row before them (a prompt's rows 64 at a
-  // time from 8192 rows on: 97 us at 14533; a quarter as many, 110).
+  // its own; of many, most continue the row before them: 64 at a time from 8192 rows
+  // on, so that few workgroups find no run.
   a.chunk = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, num_tokens / 128)));
   const int64_t chunks = (num_tokens + a.chunk - 1) / a.chunk;
   a.spread = static_cast<int>(std::min<int64_t>(chunks, 8));
